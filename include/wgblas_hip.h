@@ -53,6 +53,10 @@ enum { WGB_LEFT = 1, WGB_RIGHT = 2 };
  * never read) */
 enum { WGB_NON_UNIT = 0, WGB_UNIT = 1 };
 
+/* element types of the grouped and 4-bit operators: IEEE binary32, binary16,
+ * bfloat16 */
+enum { WGB_F32 = 0, WGB_F16 = 1, WGB_BF16 = 2 };
+
 typedef struct wgb_ctx wgb_ctx;
 
 /* WGB_ABI_VERSION of the built library (no device work; callable before
@@ -276,6 +280,42 @@ int wgb_dtrmm(wgb_ctx *ctx, int side, int uplo, int transA, int diag,
 int wgb_strsm(wgb_ctx *ctx, int side, int uplo, int transA, int diag,
               int64_t m, int64_t n, float alpha, const float *A, int64_t lda,
               float *B, int64_t ldb);
+
+/* ---- grouped products (expert layers) -------------------------------------- */
+/* Products of ragged groups of columns, each group with a matrix of its own:
+ * the products of a layer whose experts (groups) get as many tokens (columns)
+ * as a router gives them. d_offsets holds groups + 1 boundaries IN DEVICE
+ * MEMORY, never decreasing, from 0 to at most the number of columns; group g
+ * is [d_offsets[g], d_offsets[g + 1]), and may be empty. The host neither
+ * reads nor waits for them. Boundaries outside the columns are taken as the
+ * nearest inside; what decreasing ones give is not defined, but no memory
+ * outside the operands is touched. Operands are all of `type` (WGB_F32,
+ * WGB_F16 or WGB_BF16), C of `ctype`: the same, or WGB_F32. Sums are held in
+ * fp32 and rounded once, to nearest even. beta == 0 never reads C; alpha == 0
+ * reads neither A nor B. Results are reproducible run to run. No counterpart
+ * in the reference, which has no grouped routine. */
+
+/* C(:, j) <- alpha*op(A_g)*B(:, j) + beta*C(:, j) for the columns j of every
+ * group g: B k-by-n and C m-by-n column-major, op(A_g) m-by-k with A_g at
+ * A + g*strideA elements, m-by-k (WGB_NO_TRANS) or k-by-m (WGB_TRANS). Columns
+ * of no group are left as they are. With weights stored out-by-in row-major,
+ * which is in-by-out here, WGB_TRANS is a layer's forward product and
+ * WGB_NO_TRANS the gradient of its input. */
+int wgb_gemm_grouped(wgb_ctx *ctx, int type, int transA, int64_t groups,
+                     int64_t m, int64_t n, int64_t k, float alpha,
+                     const void *A, int64_t lda, int64_t strideA,
+                     const void *B, int64_t ldb, const int64_t *d_offsets,
+                     float beta, void *C, int64_t ldc, int ctype);
+
+/* C_g <- alpha*A(:, g)*B(:, g)^T + beta*C_g for every group g, over its
+ * columns: A m-by-k and B n-by-k column-major, C_g m-by-n at C + g*strideC
+ * elements. The weight gradients of wgb_gemm_grouped's layer; an empty group
+ * gives beta*C_g. */
+int wgb_gemm_grouped_k(wgb_ctx *ctx, int type, int64_t groups, int64_t m,
+                       int64_t n, int64_t k, float alpha, const void *A,
+                       int64_t lda, const void *B, int64_t ldb,
+                       const int64_t *d_offsets, float beta, void *C,
+                       int64_t ldc, int64_t strideC, int ctype);
 
 /* ---- level 2 -------------------------------------------------------------- */
 

@@ -7,6 +7,9 @@ the level-3 routines built on it) and level-1 reductions, behind a C ABI
   * wgblas_amd.native  ctypes binding of the C ABI (tests, bench)
 """
 from .native import (  # noqa: F401
+    BF16,
+    F16,
+    F32,
     LEFT,
     LIB_PATH,
     LOWER,

@@ -1,0 +1,158 @@
+// Grouped products with ragged groups: wgb_gemm_grouped (ragged columns) and
+// wgb_gemm_grouped_k (ragged k), for f32, f16 and bf16 operands.
+//
+// wgblas has no grouped product; an expert layer's products would be one
+// sgemm per expert, with the groups' sizes copied to the host first. Here one
+// launch covers all groups and reads their boundaries on the GPU
+// (ragged_tile.h).
+#include "ragged_tile.h"
+
+namespace {
+
+using namespace wgb_ragged;
+using wgb::fail;
+
+int64_t type_size(int type) { return type == WGB_F32 ? 4 : 2; }
+
+bool known_type(int type) { return type == WGB_F32 || type == WGB_F16 || type == WGB_BF16; }
+
+// Whether 16-byte copies can read a matrix: dword-aligned addresses, and the
+// lane offsets of a 256-column tile inside 32 bits.
+bool copyable(const void *p, int64_t ld_bytes, int64_t stride_bytes) {
+  return ((uintptr_t)p & 3) == 0 && ld_bytes % 4 == 0 && stride_bytes % 4 == 0 && ld_bytes < ((int64_t)1 << 22);
+}
+
+template <class E, bool AMC, bool VEC>
+int run_columns(wgb_ctx *ctx, Args &p) {
+  const int64_t mean = p.n / p.groups;
+  auto go = [&](auto kernel, int bm, int bn) {
+    p.tiles_m = (int)((p.m + bm - 1) / bm);
+    return launch<decltype(kernel)>(ctx, p, column_tiles(p, bn) * p.tiles_m);
+  };
+  if (mean <= 32) return go(Kernel<E, 128, 32, 4, 1, AMC, false, VEC, false, 4>{}, 128, 32);
+  if constexpr (VEC && E::kBits == 16) {
+    if (mean > 128) return go(Kernel<E, 256, 256, 2, 4, AMC, false, VEC, false, 2>{}, 256, 256);
+  }
+  return go(Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>{}, 128, 128);
+}
+
+template <class E, bool VEC>
+int run_k(wgb_ctx *ctx, Args &p) {
+  auto go = [&](auto kernel, int bm, int bn) {
+    p.tiles_m = (int)((p.m + bm - 1) / bm);
+    p.tiles_n = (int)((p.n + bn - 1) / bn);
+    return launch<decltype(kernel)>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
+  };
+  if constexpr (VEC && E::kBits == 16) {
+    if ((p.m + 255) / 256 * ((p.n + 255) / 256) * p.groups >= ctx->num_cus)
+      return go(Kernel<E, 256, 256, 2, 4, true, true, VEC, true, 2>{}, 256, 256);
+  }
+  return go(Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>{}, 128, 128);
+}
+
+template <class E>
+int dispatch_columns(wgb_ctx *ctx, Args &p, bool amc, bool vec) {
+  if (amc) return vec ? run_columns<E, true, true>(ctx, p) : run_columns<E, true, false>(ctx, p);
+  return vec ? run_columns<E, false, true>(ctx, p) : run_columns<E, false, false>(ctx, p);
+}
+
+// Checks shared by both forms. `k` is null-free of meaning where a dimension is zero.
+int check_sizes(int type, int ctype, int64_t groups, int64_t m, int64_t n, int64_t k) {
+  if (!known_type(type)) return fail(WGB_ERR_INVALID_VALUE, "type must be WGB_F32, WGB_F16 or WGB_BF16");
+  if (ctype != type && ctype != WGB_F32)
+    return fail(WGB_ERR_INVALID_VALUE, "the type of C must be the operands' type or WGB_F32");
+  if (groups < 0 || m < 0 || n < 0 || k < 0)
+    return fail(WGB_ERR_INVALID_VALUE, "groups, m, n, and k must be non-negative");
+  if (groups > (1 << 20)) return fail(WGB_ERR_INVALID_VALUE, "groups must be at most 2^20");
+  if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX)
+    return fail(WGB_ERR_INVALID_VALUE, "m, n, and k must be below 2^31");
+  return WGB_OK;
+}
+
+}  // namespace
+
+extern "C" int wgb_gemm_grouped(wgb_ctx *ctx, int type, int transA, int64_t groups, int64_t m, int64_t n, int64_t k,
+                                float alpha, const void *A, int64_t lda, int64_t strideA, const void *B, int64_t ldb,
+                                const int64_t *d_offsets, float beta, void *C, int64_t ldc, int ctype) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_sizes(type, ctype, groups, m, n, k))) return st;
+  if (transA != WGB_NO_TRANS && transA != WGB_TRANS)
+    return fail(WGB_ERR_INVALID_VALUE, "transA must be WGB_NO_TRANS or WGB_TRANS");
+  const int64_t a_rows = transA == WGB_TRANS ? k : m, a_cols = transA == WGB_TRANS ? m : k;
+  if (lda < (a_rows > 1 ? a_rows : 1)) return fail(WGB_ERR_INVALID_VALUE, "lda must be >= max(1, rows of A)");
+  if (strideA < 0 || (groups > 1 && strideA < (a_cols > 0 ? (a_cols - 1) * lda + a_rows : 0)))
+    return fail(WGB_ERR_INVALID_VALUE, "strideA must cover a group's A");
+  if (ldb < (k > 1 ? k : 1)) return fail(WGB_ERR_INVALID_VALUE, "ldb must be >= max(1, k)");
+  if (ldc < (m > 1 ? m : 1)) return fail(WGB_ERR_INVALID_VALUE, "ldc must be >= max(1, m)");
+  if (m == 0 || n == 0 || groups == 0) return WGB_OK;
+  if (!d_offsets) return fail(WGB_ERR_INVALID_VALUE, "d_offsets is null");
+  if (!C) return fail(WGB_ERR_INVALID_VALUE, "C is null");
+  if (k > 0 && alpha != 0.0f && (!A || !B)) return fail(WGB_ERR_INVALID_VALUE, "A or B is null");
+  const int64_t es = type_size(type);
+  Args p = {};
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.A = (const char *)A;
+  p.B = (const char *)B;
+  p.lda = lda * es;
+  p.ldb = ldb * es;
+  p.stride_a = strideA * es;
+  p.off = d_offsets;
+  p.groups = (int)groups;
+  p.C = C;
+  p.ldc = ldc;
+  p.alpha = alpha;
+  p.beta = beta;
+  p.c_f32 = ctype == WGB_F32;
+  const bool vec = copyable(A, p.lda, p.stride_a) && copyable(B, p.ldb, 0);
+  wgb::timing_begin(ctx);
+  const bool amc = transA == WGB_NO_TRANS;
+  st = type == WGB_F32   ? dispatch_columns<F32>(ctx, p, amc, vec)
+       : type == WGB_F16 ? dispatch_columns<F16>(ctx, p, amc, vec)
+                         : dispatch_columns<Bf16>(ctx, p, amc, vec);
+  wgb::timing_end(ctx);
+  return st;
+}
+
+extern "C" int wgb_gemm_grouped_k(wgb_ctx *ctx, int type, int64_t groups, int64_t m, int64_t n, int64_t k, float alpha,
+                                  const void *A, int64_t lda, const void *B, int64_t ldb, const int64_t *d_offsets,
+                                  float beta, void *C, int64_t ldc, int64_t strideC, int ctype) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_sizes(type, ctype, groups, m, n, k))) return st;
+  if (lda < (m > 1 ? m : 1)) return fail(WGB_ERR_INVALID_VALUE, "lda must be >= max(1, m)");
+  if (ldb < (n > 1 ? n : 1)) return fail(WGB_ERR_INVALID_VALUE, "ldb must be >= max(1, n)");
+  if (ldc < (m > 1 ? m : 1)) return fail(WGB_ERR_INVALID_VALUE, "ldc must be >= max(1, m)");
+  if (strideC < 0 || (groups > 1 && strideC < (n > 0 ? (n - 1) * ldc + m : 0)))
+    return fail(WGB_ERR_INVALID_VALUE, "strideC must cover a group's C");
+  if (m == 0 || n == 0 || groups == 0) return WGB_OK;
+  if (!d_offsets) return fail(WGB_ERR_INVALID_VALUE, "d_offsets is null");
+  if (!C) return fail(WGB_ERR_INVALID_VALUE, "C is null");
+  if (k > 0 && alpha != 0.0f && (!A || !B)) return fail(WGB_ERR_INVALID_VALUE, "A or B is null");
+  const int64_t es = type_size(type);
+  Args p = {};
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.A = (const char *)A;
+  p.B = (const char *)B;
+  p.lda = lda * es;
+  p.ldb = ldb * es;
+  p.off = d_offsets;
+  p.groups = (int)groups;
+  p.C = C;
+  p.ldc = ldc;
+  p.stride_c = strideC;
+  p.alpha = alpha;
+  p.beta = beta;
+  p.c_f32 = ctype == WGB_F32;
+  const bool vec = copyable(A, p.lda, 0) && copyable(B, p.ldb, 0);
+  wgb::timing_begin(ctx);
+  st = type == WGB_F32   ? (vec ? run_k<F32, true>(ctx, p) : run_k<F32, false>(ctx, p))
+       : type == WGB_F16 ? (vec ? run_k<F16, true>(ctx, p) : run_k<F16, false>(ctx, p))
+                         : (vec ? run_k<Bf16, true>(ctx, p) : run_k<Bf16, false>(ctx, p));
+  wgb::timing_end(ctx);
+  return st;
+}

@@ -18,6 +18,7 @@ NO_TRANS, TRANS = 0, 1
 LOWER, UPPER = 1, 2
 LEFT, RIGHT = 1, 2
 NON_UNIT, UNIT = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 _i64 = C.c_int64
 _ptr = C.c_void_p
@@ -71,6 +72,10 @@ _SIGNATURES = {
                   _ptr, _i64],
     "wgb_strsm": [_ptr, C.c_int, C.c_int, C.c_int, C.c_int, _i64, _i64, C.c_float, _ptr, _i64,
                   _ptr, _i64],
+    "wgb_gemm_grouped": [_ptr, C.c_int, C.c_int, _i64, _i64, _i64, _i64, C.c_float, _ptr, _i64, _i64, _ptr,
+                         _i64, _ptr, C.c_float, _ptr, _i64, C.c_int],
+    "wgb_gemm_grouped_k": [_ptr, C.c_int, _i64, _i64, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, _ptr,
+                           C.c_float, _ptr, _i64, _i64, C.c_int],
     "wgb_sgemv": [_ptr, C.c_int, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, C.c_float, _ptr,
                   _i64],
     "wgb_sger": [_ptr, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, _ptr, _i64],
@@ -332,6 +337,21 @@ class Context:
     def strsm(self, side, uplo, transA, diag, m, n, alpha, A, lda, B, ldb):
         _check(self.lib.wgb_strsm(self.handle, side, uplo, transA, diag, m, n, alpha, _p(A), lda,
                                   _p(B), ldb), "wgb_strsm")
+
+    # ---- grouped products (offsets: groups + 1 int64 boundaries in device memory) ----
+    def gemm_grouped(self, type, transA, groups, m, n, k, alpha, A, lda, strideA, B, ldb, offsets, beta, C_, ldc,
+                     ctype=None):
+        """C(:, j) = alpha op(A_g) B(:, j) + beta C(:, j) for the columns j of each group g."""
+        _check(self.lib.wgb_gemm_grouped(self.handle, type, transA, groups, m, n, k, alpha, _p(A), lda, strideA,
+                                         _p(B), ldb, _p(offsets), beta, _p(C_), ldc,
+                                         type if ctype is None else ctype), "wgb_gemm_grouped")
+
+    def gemm_grouped_k(self, type, groups, m, n, k, alpha, A, lda, B, ldb, offsets, beta, C_, ldc, strideC,
+                       ctype=None):
+        """C_g = alpha A(:, g) B(:, g)^T + beta C_g for each group g of the columns of A and B."""
+        _check(self.lib.wgb_gemm_grouped_k(self.handle, type, groups, m, n, k, alpha, _p(A), lda, _p(B), ldb,
+                                           _p(offsets), beta, _p(C_), ldc, strideC,
+                                           type if ctype is None else ctype), "wgb_gemm_grouped_k")
 
     # ---- level 2 ----
     def sgemv(self, trans, m, n, alpha, A, lda, x, incx, beta, y, incy):
