@@ -317,6 +317,55 @@ int wgb_gemm_grouped_k(wgb_ctx *ctx, int type, int64_t groups, int64_t m,
                        const int64_t *d_offsets, float beta, void *C,
                        int64_t ldc, int64_t strideC, int ctype);
 
+/* ---- MXFP4: 4-bit matrices and their products -------------------------------- */
+/* A k-by-n matrix of 4-bit floats in blocks of 32 along k (the OCP
+ * microscaling format MXFP4): E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) and a power of two for each block. Column j has its codes at
+ * codes + j*ld/2, two a byte, the first in the low half, and its scales at
+ * scales + j*ld/32: byte s is 2^(s - 127), 0xff NaN. ld, in elements, is a
+ * multiple of 128, at least k and at most 2^23; codes are 16-byte aligned,
+ * scales 4-byte. The elements from k to the next multiple of 128 are stored as
+ * zeros with scale byte 0 (quantising writes them); products read them. No
+ * counterpart in the reference, which has no type below 32 bits. */
+
+/* X (of `type`: WGB_F32, WGB_F16 or WGB_BF16) to MXFP4, blocks along k: X is
+ * k-by-n column-major (WGB_NO_TRANS) or n-by-k (WGB_TRANS: its transpose is
+ * quantised, for products that sum over X's columns). A block's scale is
+ * 2^(floor(log2 max|x|) - 2), at least 2^-127; x/scale goes to the nearest
+ * code, ties to the even code, magnitudes above 6 to 6. A block with an Inf or
+ * a NaN becomes NaN as a whole (scale 0xff, codes 0). */
+int wgb_mxfp4_quantize(wgb_ctx *ctx, int type, int trans, int64_t k, int64_t n,
+                       const void *X, int64_t ldx, uint8_t *codes,
+                       uint8_t *scales, int64_t ld);
+
+/* The values a k-by-n MXFP4 matrix stands for, in `type`, column-major:
+ * exact in WGB_F32 and, but for fp16's range, in the 16-bit types (rounded to
+ * nearest even where not). */
+int wgb_mxfp4_dequantize(wgb_ctx *ctx, int type, int64_t k, int64_t n,
+                         const uint8_t *codes, const uint8_t *scales,
+                         int64_t ld, void *X, int64_t ldx);
+
+/* C <- alpha*A^T*B + beta*C: A k-by-m and B k-by-n in MXFP4 (both along k:
+ * weights stored out-by-in row-major and tokens by row), C m-by-n of `ctype`
+ * (WGB_F32, WGB_F16 or WGB_BF16). Sums are held in fp32 and rounded once.
+ * beta == 0 never reads C; alpha == 0 reads neither A nor B. */
+int wgb_mxfp4_gemm(wgb_ctx *ctx, int64_t m, int64_t n, int64_t k, float alpha,
+                   const uint8_t *A, const uint8_t *scaleA, int64_t lda,
+                   const uint8_t *B, const uint8_t *scaleB, int64_t ldb,
+                   float beta, void *C, int64_t ldc, int ctype);
+
+/* wgb_gemm_grouped's operation (WGB_TRANS) on MXFP4 operands: A_g is the
+ * k-by-m matrix whose codes start strideA elements (strideA/2 bytes, its
+ * scales strideA/32 bytes) after the group before; strideA is a multiple of
+ * 128. A matrix of groups*m columns quantised in one call is that with
+ * strideA = m*lda. */
+int wgb_mxfp4_gemm_grouped(wgb_ctx *ctx, int64_t groups, int64_t m, int64_t n,
+                           int64_t k, float alpha, const uint8_t *A,
+                           const uint8_t *scaleA, int64_t lda, int64_t strideA,
+                           const uint8_t *B, const uint8_t *scaleB, int64_t ldb,
+                           const int64_t *d_offsets, float beta, void *C,
+                           int64_t ldc, int ctype);
+
 /* ---- level 2 -------------------------------------------------------------- */
 
 /* y <- alpha*op(A)*x + beta*y, A m-by-n column-major: op(A) = A (trans ==

@@ -76,6 +76,12 @@ _SIGNATURES = {
                          _i64, _ptr, C.c_float, _ptr, _i64, C.c_int],
     "wgb_gemm_grouped_k": [_ptr, C.c_int, _i64, _i64, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, _ptr,
                            C.c_float, _ptr, _i64, _i64, C.c_int],
+    "wgb_mxfp4_quantize": [_ptr, C.c_int, C.c_int, _i64, _i64, _ptr, _i64, _ptr, _ptr, _i64],
+    "wgb_mxfp4_dequantize": [_ptr, C.c_int, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64],
+    "wgb_mxfp4_gemm": [_ptr, _i64, _i64, _i64, C.c_float, _ptr, _ptr, _i64, _ptr, _ptr, _i64, C.c_float, _ptr,
+                       _i64, C.c_int],
+    "wgb_mxfp4_gemm_grouped": [_ptr, _i64, _i64, _i64, _i64, C.c_float, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64,
+                               _ptr, C.c_float, _ptr, _i64, C.c_int],
     "wgb_sgemv": [_ptr, C.c_int, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, C.c_float, _ptr,
                   _i64],
     "wgb_sger": [_ptr, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, _ptr, _i64],
@@ -352,6 +358,29 @@ class Context:
         _check(self.lib.wgb_gemm_grouped_k(self.handle, type, groups, m, n, k, alpha, _p(A), lda, _p(B), ldb,
                                            _p(offsets), beta, _p(C_), ldc, strideC,
                                            type if ctype is None else ctype), "wgb_gemm_grouped_k")
+
+    # ---- MXFP4 (ld in elements, a multiple of 128; codes ld / 2 and scales ld / 32 bytes a column) ----
+    def mxfp4_quantize(self, type, trans, k, n, X, ldx, codes, scales, ld):
+        """X (k x n, or n x k with trans) to 4-bit codes and block scales along k."""
+        _check(self.lib.wgb_mxfp4_quantize(self.handle, type, trans, k, n, _p(X), ldx, _p(codes), _p(scales), ld),
+               "wgb_mxfp4_quantize")
+
+    def mxfp4_dequantize(self, type, k, n, codes, scales, ld, X, ldx):
+        """The k x n values that codes and scales stand for."""
+        _check(self.lib.wgb_mxfp4_dequantize(self.handle, type, k, n, _p(codes), _p(scales), ld, _p(X), ldx),
+               "wgb_mxfp4_dequantize")
+
+    def mxfp4_gemm(self, m, n, k, alpha, A, scaleA, lda, B, scaleB, ldb, beta, C_, ldc, ctype):
+        """C = alpha A^T B + beta C, A (k x m) and B (k x n) in MXFP4."""
+        _check(self.lib.wgb_mxfp4_gemm(self.handle, m, n, k, alpha, _p(A), _p(scaleA), lda, _p(B), _p(scaleB), ldb,
+                                       beta, _p(C_), ldc, ctype), "wgb_mxfp4_gemm")
+
+    def mxfp4_gemm_grouped(self, groups, m, n, k, alpha, A, scaleA, lda, strideA, B, scaleB, ldb, offsets, beta, C_,
+                           ldc, ctype):
+        """C(:, j) = alpha A_g^T B(:, j) + beta C(:, j) for the columns j of each group g, A_g and B in MXFP4."""
+        _check(self.lib.wgb_mxfp4_gemm_grouped(self.handle, groups, m, n, k, alpha, _p(A), _p(scaleA), lda, strideA,
+                                               _p(B), _p(scaleB), ldb, _p(offsets), beta, _p(C_), ldc, ctype),
+               "wgb_mxfp4_gemm_grouped")
 
     # ---- level 2 ----
     def sgemv(self, trans, m, n, alpha, A, lda, x, incx, beta, y, incy):
