@@ -25,29 +25,20 @@ bool copyable(const void *p, int64_t ld_bytes, int64_t stride_bytes) {
 template <class E, bool AMC, bool VEC>
 int run_columns(wgb_ctx *ctx, Args &p) {
   const int64_t mean = p.n / p.groups;
-  auto go = [&](auto kernel, int bm, int bn) {
-    p.tiles_m = (int)((p.m + bm - 1) / bm);
-    return launch<decltype(kernel)>(ctx, p, column_tiles(p, bn) * p.tiles_m);
-  };
-  if (mean <= 32) return go(Kernel<E, 128, 32, 4, 1, AMC, false, VEC, false, 4>{}, 128, 32);
+  if (mean <= 32) return launch_columns<Kernel<E, 128, 32, 4, 1, AMC, false, VEC, false, 4>>(ctx, p);
   if constexpr (VEC && E::kBits == 16) {
-    if (mean > 128) return go(Kernel<E, 256, 256, 2, 4, AMC, false, VEC, false, 2>{}, 256, 256);
+    if (mean > 128) return launch_columns<TurnKernel<E, AMC, false, false>>(ctx, p);
   }
-  return go(Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>{}, 128, 128);
+  return launch_columns<Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
 }
 
 template <class E, bool VEC>
 int run_k(wgb_ctx *ctx, Args &p) {
-  auto go = [&](auto kernel, int bm, int bn) {
-    p.tiles_m = (int)((p.m + bm - 1) / bm);
-    p.tiles_n = (int)((p.n + bn - 1) / bn);
-    return launch<decltype(kernel)>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
-  };
   if constexpr (VEC && E::kBits == 16) {
     if ((p.m + 255) / 256 * ((p.n + 255) / 256) * p.groups >= ctx->num_cus)
-      return go(Kernel<E, 256, 256, 2, 4, true, true, VEC, true, 2>{}, 256, 256);
+      return launch_k<TurnKernel<E, true, true, true>>(ctx, p);
   }
-  return go(Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>{}, 128, 128);
+  return launch_k<Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>>(ctx, p);
 }
 
 template <class E>

@@ -353,14 +353,10 @@ int check_convert(int type, int64_t k, int64_t n) {
 }
 
 int product(wgb_ctx *ctx, Args &p) {
-  auto go = [&](auto kernel, int bm, int bn) {
-    p.tiles_m = (int)((p.m + bm - 1) / bm);
-    return launch<decltype(kernel)>(ctx, p, column_tiles(p, bn) * p.tiles_m);
-  };
   const int64_t mean = p.n / p.groups;
-  if (mean <= 32) return go(Kernel<Fp4, 128, 32, 4, 1, false, false, true, false, 4>{}, 128, 32);
-  if (mean > 128) return go(Kernel<Fp4, 256, 256, 2, 4, false, false, true, false, 2>{}, 256, 256);
-  return go(Kernel<Fp4, 128, 128, 2, 2, false, false, true, false, 2>{}, 128, 128);
+  if (mean <= 32) return launch_columns<Kernel<Fp4, 128, 32, 4, 1, false, false, true, false, 4>>(ctx, p);
+  if (mean > 128) return launch_columns<TurnKernel<Fp4, false, false, false>>(ctx, p);
+  return launch_columns<Kernel<Fp4, 128, 128, 2, 2, false, false, true, false, 2>>(ctx, p);
 }
 
 int run_product(wgb_ctx *ctx, int64_t groups, int64_t m, int64_t n, int64_t k, float alpha, const uint8_t *A,
