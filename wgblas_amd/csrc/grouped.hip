@@ -22,23 +22,58 @@ bool copyable(const void *p, int64_t ld_bytes, int64_t stride_bytes) {
   return ((uintptr_t)p & 3) == 0 && ld_bytes % 4 == 0 && stride_bytes % 4 == 0 && ld_bytes < ((int64_t)1 << 22);
 }
 
+template <class E>
+constexpr TileCost cost(int T) {
+  return E::kBits == 32 ? (T == 64 ? TileCost{20, 15.2} : TileCost{64, 59.3})
+                        : (T == 64 ? TileCost{5.4, 4.1} : T == 128 ? TileCost{12.5, 9.5} : TileCost{23.5, 23.5});
+}
+
+// The tile (64, 128 or 256 square) whose estimated time is least; 256 needs
+// 16-bit operands that can be copied.
+template <class E, bool VEC>
+int choose(wgb_ctx *ctx, const Args &p, double k, double n64, double n128, double n256) {
+  const double size = p.c_f32 ? 4 : 2;
+  const double t64 = tile_time(ctx, p, 64, cost<E>(64), n64, k, size);
+  const double t128 = tile_time(ctx, p, 128, cost<E>(128), n128, k, size);
+  if (VEC && E::kBits == 16) {
+    const double t256 = tile_time(ctx, p, 256, cost<E>(256), n256, k, size);
+    if (t256 <= t128 && t256 <= t64) return 256;
+  }
+  return t128 <= t64 ? 128 : 64;
+}
+
 template <class E, bool AMC, bool VEC>
 int run_columns(wgb_ctx *ctx, Args &p) {
   const int64_t mean = p.n / p.groups;
-  if (mean <= 32) return launch_columns<Kernel<E, 128, 32, 4, 1, AMC, false, VEC, false, 4>>(ctx, p);
-  if constexpr (VEC && E::kBits == 16) {
-    if (mean > 128) return launch_columns<TurnKernel<E, AMC, false, false>>(ctx, p);
+  if (mean <= 32) {
+    // Few columns: reading A counts. Whole rows of blocks stream it through
+    // LDS (64 experts of 2048 x 1024 in bf16: 27 us, the waves-share-k kernel
+    // 37); with too few blocks for the CUs the waves share k instead (8192 x
+    // 4096, one column: 5.8 against 10 us in fp4).
+    const int64_t blocks = (p.m + 127) / 128 * (p.n < p.groups ? p.n : p.groups);
+    if constexpr (!AMC) {
+      if (blocks < ctx->num_cus)
+        return mean <= 16 ? launch_columns<SkinnyKernel<E, 2, 1>>(ctx, p) : launch_columns<SkinnyKernel<E, 2, 2>>(ctx, p);
+    }
+    return launch_columns<Kernel<E, 128, 32, 4, 1, AMC, false, VEC, false, 4>>(ctx, p);
   }
-  return launch_columns<Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
+  const int T = choose<E, VEC>(ctx, p, (double)p.k, expected_columns(p, 64), expected_columns(p, 128), expected_columns(p, 256));
+  if constexpr (VEC && E::kBits == 16) {
+    if (T == 256) return launch_columns<TurnKernel<E, AMC, false, false>>(ctx, p);
+  }
+  if (T == 128) return launch_columns<Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
+  return launch_columns<Kernel<E, 64, 64, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
 }
 
 template <class E, bool VEC>
 int run_k(wgb_ctx *ctx, Args &p) {
+  auto across = [&](int64_t T) { return (double)((p.n + T - 1) / T * p.groups); };
+  const int T = choose<E, VEC>(ctx, p, (double)p.k / p.groups, across(64), across(128), across(256));
   if constexpr (VEC && E::kBits == 16) {
-    if ((p.m + 255) / 256 * ((p.n + 255) / 256) * p.groups >= ctx->num_cus)
-      return launch_k<TurnKernel<E, true, true, true>>(ctx, p);
+    if (T == 256) return launch_k<TurnKernel<E, true, true, true>>(ctx, p);
   }
-  return launch_k<Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>>(ctx, p);
+  if (T == 128) return launch_k<Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>>(ctx, p);
+  return launch_k<Kernel<E, 64, 64, 2, 2, true, true, VEC, true, 2>>(ctx, p);
 }
 
 template <class E>

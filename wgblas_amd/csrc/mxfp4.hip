@@ -180,79 +180,94 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename E::store *
   }
 }
 
-// Blocks along the strided axis: a lane has two neighbouring columns of one
-// block, 32 loads of two elements (256 contiguous bytes a wave for 16-bit
-// types). The eight waves of a block have eight blocks in a row of the same
-// 128 columns, whose codes fill lines of 128 bytes.
+// Blocks along the strided axis. A lane has two neighbouring columns of one
+// block: 32 loads of two elements (256 contiguous bytes a wave for 16-bit
+// types). The eight waves have eight blocks in a row of the same 128 columns;
+// their codes go through LDS (16-byte chunks at chunk ^ column, no two lanes
+// of a quarter wave in the same banks) and out as 128-byte lines.
 template <class E>
 __global__ __launch_bounds__(512) void quantize_strided_kernel(const typename E::store *X, int64_t ldx, int64_t k,
                                                                int64_t n, uint8_t *codes, uint8_t *scales, int64_t ld,
                                                                int blocks, int groups_k) {
   typedef Pair<E> P;
   typedef typename E::store T;
+  __shared__ v4i lines[128][8];
+  __shared__ __align__(8) uint8_t bytes[128][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int kb = (int)(blockIdx.x % groups_k) * 8 + wave;
-  const int64_t j = (int64_t)(blockIdx.x / groups_k) * 128 + 2 * lane;
-  if (kb >= blocks || j >= n) return;
-  const bool two = j + 1 < n;
-  const int64_t k0 = (int64_t)kb * 32, left = k - k0;
-  const T *x = X + k0 * ldx + j;
-  typename P::V v[32];
-#pragma unroll
-  for (int r = 0; r < 32; ++r) {
-    v[r] = P::zero();
-    if (r < left) {
-      struct __attribute__((packed, aligned(sizeof(T)))) V2 {
-        typename P::V p;
-      };
-      if (two) {
-        v[r] = reinterpret_cast<const V2 *>(x + r * ldx)->p;
-      } else if constexpr (E::kBits == 32) {
-        v[r] = P::make(x[r * ldx], 0.0f);
-      } else {
-        v[r] = P::make(reinterpret_cast<const uint16_t *>(x)[r * ldx], 0);
-      }
-    }
-  }
-  uint32_t bits[2];
-  if constexpr (E::kBits == 32) {
-    uint32_t a = 0, b = 0;
+  const int kb0 = (int)(blockIdx.x % groups_k) * 8, kb = kb0 + wave;
+  const int64_t j0 = (int64_t)(blockIdx.x / groups_k) * 128, j = j0 + 2 * lane;
+  if (kb < blocks && j < n) {
+    const bool two = j + 1 < n;
+    const int64_t k0 = (int64_t)kb * 32, left = k - k0;
+    const T *x = X + k0 * ldx + j;
+    typename P::V v[32];
 #pragma unroll
     for (int r = 0; r < 32; ++r) {
-      const uint32_t p = __float_as_uint(v[r][0]) & 0x7fffffffu, q = __float_as_uint(v[r][1]) & 0x7fffffffu;
-      a = a > p ? a : p;
-      b = b > q ? b : q;
-    }
-    bits[0] = a;
-    bits[1] = b;
-  } else {
-    uint32_t t = 0;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) t = P::top(t, v[r]);
-    bits[0] = P::bits(t & 0xffffu);
-    bits[1] = P::bits(t >> 16);
-  }
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    if (c == 1 && !two) break;
-    const uint32_t byte = scale_byte(bits[c]);
-    v4i out;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      typename P::V w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * q + 2 * i;
-        if constexpr (E::kBits == 32)
-          w[i] = P::make(v[r][c], v[r + 1][c]);
-        else  // the two rows' halves c side by side
-          w[i] = __builtin_amdgcn_perm(v[r + 1], v[r], c == 0 ? 0x05040100u : 0x07060302u);
+      v[r] = P::zero();
+      if (r < left) {
+        struct __attribute__((packed, aligned(sizeof(T)))) V2 {
+          typename P::V p;
+        };
+        if (two) {
+          v[r] = reinterpret_cast<const V2 *>(x + r * ldx)->p;
+        } else if constexpr (E::kBits == 32) {
+          v[r] = P::make(x[r * ldx], 0.0f);
+        } else {
+          v[r] = P::make(reinterpret_cast<const uint16_t *>(x)[r * ldx], 0);
+        }
       }
-      out[q] = (int)codes8<E>(w, byte);
     }
-    *reinterpret_cast<v4i *>(codes + (j + c) * (ld / 2) + kb * 16) = out;
-    scales[(j + c) * (ld / 32) + kb] = (uint8_t)byte;
+    uint32_t bits[2];
+    if constexpr (E::kBits == 32) {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const uint32_t p = __float_as_uint(v[r][0]) & 0x7fffffffu, q = __float_as_uint(v[r][1]) & 0x7fffffffu;
+        a = a > p ? a : p;
+        b = b > q ? b : q;
+      }
+      bits[0] = a;
+      bits[1] = b;
+    } else {
+      uint32_t t = 0;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) t = P::top(t, v[r]);
+      bits[0] = P::bits(t & 0xffffu);
+      bits[1] = P::bits(t >> 16);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t byte = scale_byte(bits[c]);
+      v4i out;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        typename P::V w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * q + 2 * i;
+          if constexpr (E::kBits == 32)
+            w[i] = P::make(v[r][c], v[r + 1][c]);
+          else  // the two rows' halves c side by side
+            w[i] = __builtin_amdgcn_perm(v[r + 1], v[r], c == 0 ? 0x05040100u : 0x07060302u);
+        }
+        out[q] = (int)codes8<E>(w, byte);
+      }
+      lines[2 * lane + c][wave ^ (lane & 7)] = out;
+      bytes[2 * lane + c][wave] = (uint8_t)byte;
+    }
   }
+  __syncthreads();
+  const int here = blocks - kb0 < 8 ? blocks - kb0 : 8;  // a multiple of 4
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int col = (threadIdx.x >> 3) + 64 * q, chunk = threadIdx.x & 7;
+    if (j0 + col < n && chunk < here)
+      *reinterpret_cast<v4i *>(codes + (j0 + col) * (ld / 2) + (kb0 + chunk) * 16) = lines[col][chunk ^ ((col >> 1) & 7)];
+  }
+  const int col = threadIdx.x >> 1, half = threadIdx.x & 1;
+  if (col < 128 && j0 + col < n && 4 * half < here)
+    *reinterpret_cast<int *>(scales + (j0 + col) * (ld / 32) + kb0 + 4 * half) =
+        *reinterpret_cast<const int *>(&bytes[col][4 * half]);
 }
 
 // A lane has 8 codes of a column: value * scale in fp32 (both exact), rounded
@@ -354,9 +369,22 @@ int check_convert(int type, int64_t k, int64_t n) {
 
 int product(wgb_ctx *ctx, Args &p) {
   const int64_t mean = p.n / p.groups;
-  if (mean <= 32) return launch_columns<Kernel<Fp4, 128, 32, 4, 1, false, false, true, false, 4>>(ctx, p);
-  if (mean > 128) return launch_columns<TurnKernel<Fp4, false, false, false>>(ctx, p);
-  return launch_columns<Kernel<Fp4, 128, 128, 2, 2, false, false, true, false, 2>>(ctx, p);
+  if (mean <= 32) {
+    // Few columns, as in the 16-bit products: 64 experts of 4096 x 2048 take
+    // 44 us streamed with two stages (66 with four, which leave one block a
+    // CU), 82 us with the waves sharing k.
+    const int64_t blocks = (p.m + 127) / 128 * (p.n < p.groups ? p.n : p.groups);
+    if (blocks < ctx->num_cus)
+      return mean <= 16 ? launch_columns<SkinnyKernel<Fp4, 2, 1>>(ctx, p) : launch_columns<SkinnyKernel<Fp4, 2, 2>>(ctx, p);
+    return launch_columns<Kernel<Fp4, 128, 32, 4, 1, false, false, true, false, 2>>(ctx, p);
+  }
+  const double k = (double)p.k, size = p.c_f32 ? 4 : 2;
+  const double t64 = tile_time(ctx, p, 64, TileCost{4.0, 1.5}, expected_columns(p, 64), k, size);
+  const double t128 = tile_time(ctx, p, 128, TileCost{5.6, 3.3}, expected_columns(p, 128), k, size);
+  const double t256 = tile_time(ctx, p, 256, TileCost{9.5, 9.5}, expected_columns(p, 256), k, size);
+  if (t256 <= t128 && t256 <= t64) return launch_columns<TurnKernel<Fp4, false, false, false>>(ctx, p);
+  if (t128 <= t64) return launch_columns<Kernel<Fp4, 128, 128, 2, 2, false, false, true, false, 2>>(ctx, p);
+  return launch_columns<Kernel<Fp4, 64, 64, 2, 2, false, false, true, false, 2>>(ctx, p);
 }
 
 int run_product(wgb_ctx *ctx, int64_t groups, int64_t m, int64_t n, int64_t k, float alpha, const uint8_t *A,

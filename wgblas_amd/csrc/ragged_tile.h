@@ -153,14 +153,12 @@ __device__ __forceinline__ void group_range(const int64_t *off, int g, int64_t n
 // The tiles of a ragged-columns launch in order: first the groups' whole
 // column tiles, one group after the other, each in bands (tile_order.h), then
 // the tiles of the columns that are left over in each group, which cost less
-// and even out the end. Either part is dealt to the XCDs in runs. Column tiles
-// are counted over the lanes of each wave; up to 64 groups, one a lane, stay
-// in registers.
-struct ColumnFinder {
-  int whole, total;      // tiles: of whole columns, all
+// and even out the end. Either part is dealt to the XCDs in runs.
+struct ColumnOrder {
+  int whole, total;  // tiles: of whole columns, all
   int bn;
-  int lo, hi;            // lane's group: its columns (below 2^31),
-  int sum, rest;         // whole column tiles, and leftovers, up to and with it
+  int lo, hi;        // lane's group: its columns (below 2^31),
+  int sum, rest;     // whole column tiles, and leftovers, up to and with it
 
   // Groups g0 .. g0 + 63 into the lanes; before, rest_before: counts of the groups before them.
   __device__ __forceinline__ void scan(const Args &p, int g0, int before, int rest_before) {
@@ -200,44 +198,84 @@ struct ColumnFinder {
     total = whole + left * p.tiles_m;
   }
 
-  // Tile w: false if there is none.
-  __device__ __forceinline__ bool find(const Args &p, int w, Tile &t) {
-    if (w >= total) return false;
-    const bool left = w >= whole;
-    const int L = left ? wgb_tiles::xcd_remap(w - whole, total - whole) : wgb_tiles::xcd_remap(w, whole);
-    const int q = L / p.tiles_m;  // the column tile of its kind, over all groups
-    int g0 = 0;
-    uint64_t past = 1;
-    if (!p.off) {
-      t.g = 0;
-      t.lo = 0;
-      t.hi = p.n;
-    } else {
-      int before = 0, rest_before = 0;
-      for (;; g0 += 64) {
-        if (p.groups > 64) scan(p, g0, before, rest_before);
-        past = __ballot((left ? rest : sum) > q);
-        if (past || g0 + 64 >= p.groups) break;
-        before = __builtin_amdgcn_readlane(sum, 63);
-        rest_before = __builtin_amdgcn_readlane(rest, 63);
-      }
-      if (!past) return false;
-    }
-    const int at = __builtin_ctzll(past);
-    if (p.off) {
-      t.g = g0 + at;
-      t.lo = __builtin_amdgcn_readlane(lo, at);
-      t.hi = __builtin_amdgcn_readlane(hi, at);
-    }
+  // Place of tile w < total among the column tiles of its kind (`left`: a leftover), and what is left of it in that.
+  __device__ __forceinline__ int place(const Args &p, int w, bool &left, int &L) const {
+    left = w >= whole;
+    L = left ? wgb_tiles::xcd_remap(w - whole, total - whole) : wgb_tiles::xcd_remap(w, whole);
+    return L / p.tiles_m;
+  }
+  // The tile, once its group is known; `past`: whole column tiles up to and with that group.
+  __device__ __forceinline__ void settle(const Args &p, bool left, int L, int q, int past, Tile &t) const {
     const int tn = (int)(t.hi - t.lo) / bn;
     if (left) {
       t.tm = L - q * p.tiles_m;
       t.tn = tn;
     } else {
-      const int first = p.off ? __builtin_amdgcn_readlane(sum, at) - tn : 0;
-      wgb_tiles::logical_tile(L - first * p.tiles_m, p.tiles_m, tn, 0, t.tm, t.tn);
+      wgb_tiles::logical_tile(L - (past - tn) * p.tiles_m, p.tiles_m, tn, 0, t.tm, t.tn);
     }
+  }
+
+  // Tile w of a wave (w is the same in all lanes): false if there is none.
+  __device__ __forceinline__ bool find(const Args &p, int w, Tile &t) {
+    if (w >= total) return false;
+    bool left;
+    int L;
+    const int q = place(p, w, left, L);
+    t.g = 0;
+    t.lo = 0;
+    t.hi = p.n;
+    int past = (int)(p.n / bn);
+    if (p.off) {
+      int before = 0, rest_before = 0, g0 = 0;
+      uint64_t beyond;
+      for (;; g0 += 64) {
+        if (p.groups > 64) scan(p, g0, before, rest_before);
+        beyond = __ballot((left ? rest : sum) > q);
+        if (beyond || g0 + 64 >= p.groups) break;
+        before = __builtin_amdgcn_readlane(sum, 63);
+        rest_before = __builtin_amdgcn_readlane(rest, 63);
+      }
+      if (!beyond) return false;
+      const int at = __builtin_ctzll(beyond);
+      t.g = g0 + at;
+      t.lo = __builtin_amdgcn_readlane(lo, at);
+      t.hi = __builtin_amdgcn_readlane(hi, at);
+      past = __builtin_amdgcn_readlane(sum, at);
+    }
+    settle(p, left, L, q, past, t);
     return true;
+  }
+
+  // Each lane's tile w < total.
+  __device__ __forceinline__ void find_lanes(const Args &p, int w, Tile &t) {
+    bool left;
+    int L;
+    const int q = place(p, w, left, L);
+    t.g = 0;
+    t.lo = 0;
+    t.hi = p.n;
+    int past = (int)(p.n / bn);
+    if (p.off) {
+      int before = 0, rest_before = 0;
+      bool open = true;
+      for (int g0 = 0; g0 < p.groups; g0 += 64) {
+        if (p.groups > 64) scan(p, g0, before, rest_before);
+        const int count = p.groups - g0 < 64 ? p.groups - g0 : 64;
+        for (int i = 0; i < count; ++i) {
+          const int s = __builtin_amdgcn_readlane(sum, i), r = __builtin_amdgcn_readlane(rest, i);
+          if (open && (left ? r : s) > q) {
+            open = false;
+            t.g = g0 + i;
+            t.lo = __builtin_amdgcn_readlane(lo, i);
+            t.hi = __builtin_amdgcn_readlane(hi, i);
+            past = s;
+          }
+        }
+        before = __builtin_amdgcn_readlane(sum, 63);
+        rest_before = __builtin_amdgcn_readlane(rest, 63);
+      }
+    }
+    settle(p, left, L, q, past, t);
   }
 };
 
@@ -245,47 +283,80 @@ struct ColumnFinder {
 // (up to 64 of them, one a lane; more stay in their order), the rounds of a
 // persistent launch to and fro, so that blocks come out even; each group's
 // tiles are dealt to all XCDs.
-struct KFinder {
+struct KOrder {
   int total, per;
-  int lo, hi, rank;  // lane's group: its part of k (below 2^31), its place
 
   __device__ __forceinline__ void init(const Args &p, int) {
     per = p.tiles_m * p.tiles_n;
     total = per * p.groups;
-    if (p.groups > 64) return;
-    const int lane = threadIdx.x & 63;
-    int64_t l = 0, h = 0;
-    if (lane < p.groups) group_range(p.off, lane, p.k, l, h);
-    lo = (int)l;
-    hi = (int)h;
-    rank = 0;
-    const int size = hi - lo;
-    for (int g = 0; g < p.groups; ++g) {
-      const int other = __builtin_amdgcn_readlane(size, g);
-      rank += other > size || (other == size && g < lane);
-    }
-    if (lane >= p.groups) rank = -1;
   }
-  __device__ __forceinline__ bool find(const Args &p, int w, Tile &t) {
-    if (w >= total) return false;
+  // Each lane's tile w < total (lanes may have the same).
+  __device__ __forceinline__ void find_lanes(const Args &p, int w, Tile &t) {
     const int round = w / (int)gridDim.x, begin = round * (int)gridDim.x;
     const int end = begin + (int)gridDim.x < total ? begin + (int)gridDim.x : total;
     const int at = round & 1 ? begin + end - 1 - w : w;
     const int place = at / per;
     wgb_tiles::logical_tile(wgb_tiles::xcd_remap(at - place * per, per), p.tiles_m, p.tiles_n, 0, t.tm, t.tn);
-    if (p.groups <= 64) {
-      t.g = __builtin_ctzll(__ballot(rank == place));
-      t.lo = __builtin_amdgcn_readlane(lo, t.g);
-      t.hi = __builtin_amdgcn_readlane(hi, t.g);
-      return true;
-    }
     t.g = place;
-    // scalar loads: they do not wait for the copies in flight
-    typedef const __attribute__((address_space(4))) int64_t *Constant;
-    const Constant off = (Constant)(uintptr_t)p.off;
-    t.lo = off[t.g];
-    t.hi = off[t.g + 1];
-    clamp_range(p.k, t.lo, t.hi);
+    if (p.groups > 64) {
+      group_range(p.off, t.g, p.k, t.lo, t.hi);
+      return;
+    }
+    const int lane = threadIdx.x & 63;
+    int64_t l = 0, h = 0;
+    if (lane < p.groups) group_range(p.off, lane, p.k, l, h);
+    const int lo = (int)l, hi = (int)h, size = hi - lo;  // k is below 2^31
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const int other = __builtin_amdgcn_readlane(size, g);
+      rank += other > size || (other == size && g < lane);
+    }
+    for (int g = 0; g < p.groups; ++g)
+      if (__builtin_amdgcn_readlane(rank, g) == place) {
+        t.g = g;
+        t.lo = __builtin_amdgcn_readlane(lo, g);
+        t.hi = __builtin_amdgcn_readlane(hi, g);
+      }
+  }
+  __device__ __forceinline__ bool find(const Args &p, int w, Tile &t) {
+    if (w >= total) return false;
+    find_lanes(p, w, t);
+    t.g = __builtin_amdgcn_readfirstlane(t.g);
+    t.lo = __builtin_amdgcn_readfirstlane((int)t.lo);
+    t.hi = __builtin_amdgcn_readfirstlane((int)t.hi);
+    return true;
+  }
+};
+
+// A persistent block's tiles, one a lane: all of them are found at the start.
+constexpr int kTilesPerBlock = 64;
+template <class Order>
+struct TileTable {
+  int count;  // of this block's tiles
+  int g, tm, tn, lo, hi;
+
+  __device__ __forceinline__ void init(const Args &p, int bn) {
+    Order o;
+    o.init(p, bn);
+    const int first = (int)blockIdx.x, step = (int)gridDim.x;
+    count = first < o.total ? (o.total - first + step - 1) / step : 0;
+    if (count > kTilesPerBlock) count = kTilesPerBlock;  // the launch has blocks enough
+    const int lane = threadIdx.x & 63;
+    Tile t = {0, 0, 0, 0, 0};
+    if (count > 0) o.find_lanes(p, first + (lane < count ? lane : 0) * step, t);
+    g = t.g;
+    tm = t.tm;
+    tn = t.tn;
+    lo = (int)t.lo;
+    hi = (int)t.hi;
+  }
+  __device__ __forceinline__ bool get(int i, Tile &t) const {
+    if (i >= count) return false;
+    t.g = __builtin_amdgcn_readlane(g, i);
+    t.tm = __builtin_amdgcn_readlane(tm, i);
+    t.tn = __builtin_amdgcn_readlane(tn, i);
+    t.lo = __builtin_amdgcn_readlane(lo, i);
+    t.hi = __builtin_amdgcn_readlane(hi, i);
     return true;
   }
 };
@@ -598,10 +669,12 @@ __device__ __forceinline__ v4i eight_rows(uint32_t x0, uint32_t x1, uint32_t y0,
 }
 
 // alpha acc + beta C for a lane's runs of four rows of one column; column
-// blocks are STEP columns apart. fp32 is stored in those runs (16 bytes a
+// blocks are STEP columns apart. STREAM: non-temporal stores, for results too
+// large for the caches (8192 x 16384 in bf16 773 -> 760 us, 8 x 4096 x 2048 in
+// fp32 195 -> 184 us; 12 x 1032 x 520 in f16, which fits, 16.7 -> 21 us). fp32 is stored in those runs (16 bytes a
 // lane), 16-bit values in runs of eight rows (also 16 bytes) where there are
 // two row blocks: with 8 bytes a lane 8192 x 16384 x 4096 took 788 us.
-template <typename T, int MB, int NB, int STEP>
+template <typename T, int MB, int NB, int STEP, bool STREAM>
 __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB][NB], int64_t row0, int64_t rows,
                                          int64_t col0, int64_t cols, int lane) {
   typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -643,7 +716,10 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
         const V8 v = __builtin_bit_cast(V8, eight_rows(x[0], x[1], y[0], y[1]));
         const int64_t row = row0 + 16 * (i + (g & 1)) + 8 * (g >> 1);
         if (row + 8 <= rows) {
-          *reinterpret_cast<V8 *>(cp + row) = v;
+          if constexpr (STREAM)
+            __builtin_nontemporal_store(v, reinterpret_cast<V8 *>(cp + row));
+          else
+            *reinterpret_cast<V8 *>(cp + row) = v;
         } else {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
@@ -656,7 +732,10 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
         const V4 v = value(i);
         const int64_t row = row0 + 16 * i + 4 * g;
         if (row + 4 <= rows) {
-          *reinterpret_cast<V4 *>(cp + row) = v;
+          if constexpr (STREAM)
+            __builtin_nontemporal_store(v, reinterpret_cast<V4 *>(cp + row));
+          else
+            *reinterpret_cast<V4 *>(cp + row) = v;
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -668,18 +747,18 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
 }
 
 // The epilogue in C's type; `at`: element of C where the group's part starts.
-template <class E, int STEP, int MB, int NB>
+template <class E, int STEP, bool STREAM = false, int MB, int NB>
 __device__ __forceinline__ void store_tile(const Args &p, int64_t at, const f4 (&acc)[MB][NB], int64_t row0, int64_t col0,
                                            int64_t cols, int lane) {
   if (E::kBits == 32 || p.c_f32) {
-    epilogue<float, MB, NB, STEP>(p, (float *)p.C + at, acc, row0, p.m, col0, cols, lane);
+    epilogue<float, MB, NB, STEP, STREAM>(p, (float *)p.C + at, acc, row0, p.m, col0, cols, lane);
   } else if constexpr (E::kBits == 4) {
     if (p.c_f16)
-      epilogue<_Float16, MB, NB, STEP>(p, (_Float16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
+      epilogue<_Float16, MB, NB, STEP, STREAM>(p, (_Float16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
     else
-      epilogue<__bf16, MB, NB, STEP>(p, (__bf16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
+      epilogue<__bf16, MB, NB, STEP, STREAM>(p, (__bf16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
   } else if constexpr (E::kBits == 16) {
-    epilogue<typename E::store, MB, NB, STEP>(p, (typename E::store *)p.C + at, acc, row0, p.m, col0, cols, lane);
+    epilogue<typename E::store, MB, NB, STEP, STREAM>(p, (typename E::store *)p.C + at, acc, row0, p.m, col0, cols, lane);
   }
 }
 
@@ -706,9 +785,9 @@ struct Kernel {
   static __device__ __forceinline__ void run(const Args &p, char *smem) {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     Tile tile;
-    typename std::conditional<RK, KFinder, ColumnFinder>::type finder;
-    finder.init(p, BN);
-    if (!finder.find(p, blockIdx.x, tile)) return;
+    typename std::conditional<RK, KOrder, ColumnOrder>::type order;
+    order.init(p, BN);
+    if (!order.find(p, blockIdx.x, tile)) return;
     const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * BN;
     const int64_t cols = RK ? p.n : tile.hi - tile.lo;
     int64_t K = RK ? tile.hi - tile.lo : p.k;
@@ -861,7 +940,7 @@ struct TurnKernel {
   typedef Stager<E, BM, AMC, NT> SA;
   typedef Stager<E, BN, BMC, NT> SB;
   typedef ScaleStager<kScaled ? BM : 64, kScaled ? BN : 64, NW> SS;
-  typedef typename std::conditional<RK, KFinder, ColumnFinder>::type Finder;
+  typedef TileTable<typename std::conditional<RK, KOrder, ColumnOrder>::type> Table;
   static_assert(SA::BYTES == SB::BYTES, "equal units");
   static constexpr int UNIT = SA::BYTES;
   static constexpr int UNITS = kScaled ? 4 : 5;
@@ -876,92 +955,73 @@ struct TurnKernel {
     return at + 2 * UNIT >= UNITS * UNIT ? at + (2 - UNITS) * UNIT : at + 2 * UNIT;
   }
 
-  // The copies of one operand (which one is a scalar, so that both halves of
-  // the waves share the code), k-tile after k-tile and tile after tile.
+  // The copies of one operand, k-tile after k-tile and tile after tile.
+  template <class S, bool IS_A>
   struct Stream {
-    StagerData<SA::LOADS> d;
+    S s;
     const char *from;  // the next k-tile's first byte
-    int64_t step;
-    int w, kt, nt, whole, unit;
+    int i, kt, nt, whole, unit;
     int parts;  // of a k-tile that the tile's columns need
-    bool is_a;
 
-    template <class S>
-    __device__ __forceinline__ void open(const char *P, int64_t ld, int64_t row0, int64_t rows, int K, int t) {
-      S s;
-      s.init(P, ld, row0, rows, K, t);
-      d = s;
-      step = s.step();
-      whole = s.whole_tiles();
-    }
-    // The first tile from w on that has k-tiles; nt == 0: none.
-    __device__ __forceinline__ void seek(const Args &p, Finder &f, int t) {
+    // The first tile from i on that has k-tiles; nt == 0: none.
+    __device__ __forceinline__ void seek(const Args &p, const Table &table, int t) {
       Tile tile;
-      nt = 0;
-      for (; f.find(p, w, tile); w += gridDim.x) {
+      kt = nt = whole = 0;
+      for (; table.get(i, tile); ++i) {
         const int K = depth(p, tile);
         nt = tiles_k(K);
         if (nt == 0) continue;
-        parts = SA::LOADS;
-        if (!is_a && !BMC) {
-          // a part is STEP columns
-          static_assert(BMC || SB::RPS == STEP, "parts");
-          const int64_t cols = (RK ? p.n : tile.hi - tile.lo) - (int64_t)tile.tn * BN;
-          if (cols < BN) parts = (int)((cols + STEP - 1) / STEP);
+        parts = S::LOADS;
+        if constexpr (IS_A) {
+          s.init(RK ? p.A + tile.lo * p.lda : p.A + (int64_t)tile.g * p.stride_a, p.lda, (int64_t)tile.tm * BM, p.m, K, t);
+        } else {
+          const int64_t n0 = (int64_t)tile.tn * BN, cols = RK ? p.n : tile.hi - tile.lo;
+          s.init(p.B + tile.lo * p.ldb, p.ldb, n0, cols, K, t);
+          static_assert(BMC || SB::RPS == STEP, "a part is STEP columns");
+          if (!BMC && cols - n0 < BN) parts = (int)((cols - n0 + STEP - 1) / STEP);
         }
-        if (is_a)
-          open<SA>(RK ? p.A + tile.lo * p.lda : p.A + (int64_t)tile.g * p.stride_a, p.lda, (int64_t)tile.tm * BM, p.m, K, t);
-        else
-          open<SB>(p.B + tile.lo * p.ldb, p.ldb, (int64_t)tile.tn * BN, RK ? p.n : tile.hi - tile.lo, K, t);
-        kt = 0;
-        from = d.origin;
+        whole = s.whole_tiles();
+        from = s.origin;
         break;
       }
     }
-    __device__ __forceinline__ void start(const Args &p, Finder &f, int t, bool a) {
-      is_a = a;
-      w = blockIdx.x;
-      unit = a ? 0 : UNIT;
-      seek(p, f, t);
+    __device__ __forceinline__ void start(const Args &p, const Table &table, int t) {
+      i = 0;
+      unit = IS_A ? 0 : UNIT;
+      seek(p, table, t);
     }
     // k-tiles that can be copied one after the other without a look at what
     // comes: whole, and not the tile's last
     __device__ __forceinline__ int run() const { return (whole < nt - 1 ? whole : nt - 1) - kt; }
-    __device__ __forceinline__ void copy_part(char *smem, int wave, int r) const {
-      copy_chunks(from, d.voff[r], smem + unit + wave * 1024 + r * NT * 16);
+    __device__ __forceinline__ void copy(char *smem, int wave) const {
+#pragma unroll
+      for (int r = 0; r < S::LOADS; ++r)
+        if (IS_A || r == 0 || __builtin_expect(r < parts, 1))
+          copy_chunks(from, s.voff[r], smem + unit + wave * 1024 + r * NT * 16);
     }
     __device__ __forceinline__ void advance() {
       ++kt;
-      from += step;
+      from += s.step();
       unit = rotate(unit);
-    }
-    template <class S>
-    __device__ __forceinline__ void cut(char *smem, int wave) const {
-      S s;
-      (StagerData<SA::LOADS> &)s = d;
-#pragma unroll
-      for (int r = 0; r < S::LOADS; ++r)
-        if constexpr (E::kBits == 4)
-          copy_chunks(from, s.half_voff(r), smem + unit + wave * 1024 + r * NT * 16);
-        else
-          s.put(smem + unit, r, s.load_guarded(kt, r));
     }
     // The next k-tile, whatever it is: a cut one of 16-bit values goes through
     // registers.
-    __device__ __forceinline__ void issue(const Args &p, Finder &f, char *smem, int t, int wave) {
+    __device__ __forceinline__ void issue(const Args &p, const Table &table, char *smem, int t, int wave) {
       if (nt == 0) return;
       if (kt < whole) {
-#pragma unroll
-        for (int r = 0; r < SA::LOADS; ++r) copy_part(smem, wave, r);
-      } else if (is_a) {
-        cut<SA>(smem, wave);
+        copy(smem, wave);
       } else {
-        cut<SB>(smem, wave);
+#pragma unroll
+        for (int r = 0; r < S::LOADS; ++r)
+          if constexpr (E::kBits == 4)
+            copy_chunks(from, s.half_voff(r), smem + unit + wave * 1024 + r * NT * 16);
+          else
+            s.put(smem + unit, r, s.load_guarded(kt, r));
       }
       advance();
       if (kt == nt) {
-        w += gridDim.x;
-        seek(p, f, t);
+        ++i;
+        seek(p, table, t);
       }
     }
   };
@@ -969,12 +1029,12 @@ struct TurnKernel {
   // The scales of both operands (fp4), alike.
   struct ScaleStream {
     SS s;
-    int w, kt, nt, at;
+    int i, kt, nt, at;
 
-    __device__ __forceinline__ void seek(const Args &p, Finder &f, int wave, int lane) {
+    __device__ __forceinline__ void seek(const Args &p, const Table &table, int wave, int lane) {
       Tile tile;
-      nt = 0;
-      for (; f.find(p, w, tile); w += gridDim.x) {
+      kt = nt = 0;
+      for (; table.get(i, tile); ++i) {
         const int K = depth(p, tile);
         nt = tiles_k(K);
         if (nt == 0) continue;
@@ -982,21 +1042,20 @@ struct TurnKernel {
         const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * BN;
         s.init(p.scale_a + (int64_t)tile.g * (p.stride_a / 16) + m0 * lsa, lsa, p.m - m0,
                p.scale_b + (tile.lo + n0) * lsb, lsb, tile.hi - tile.lo - n0, K, wave, lane);
-        kt = 0;
         break;
       }
     }
-    __device__ __forceinline__ void start(const Args &p, Finder &f, int wave, int lane) {
-      w = blockIdx.x;
+    __device__ __forceinline__ void start(const Args &p, const Table &table, int wave, int lane) {
+      i = 0;
       at = UNITS * UNIT;
-      seek(p, f, wave, lane);
+      seek(p, table, wave, lane);
     }
     __device__ __forceinline__ int run() const { return nt - 1 - kt; }
     __device__ __forceinline__ void advance() {
       ++kt;
       at ^= (UNITS * UNIT) ^ (UNITS * UNIT + SS::BYTES);
     }
-    __device__ __forceinline__ void issue(const Args &p, Finder &f, char *smem, int wave, int lane) {
+    __device__ __forceinline__ void issue(const Args &p, const Table &table, char *smem, int wave, int lane) {
       if (nt == 0) return;
       if (kt < nt - 1)
         s.copy(smem + at, kt);
@@ -1004,19 +1063,18 @@ struct TurnKernel {
         s.put_guarded(smem + at, kt, lane);
       advance();
       if (kt == nt) {
-        w += gridDim.x;
-        seek(p, f, wave, lane);
+        ++i;
+        seek(p, table, wave, lane);
       }
     }
   };
 
   static __device__ __forceinline__ void run(const Args &p, char *smem) {
-    constexpr int PARTS = SA::LOADS;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * 16;
     const bool second = wave >= NW / 2;
-    Finder finder;
-    finder.init(p, BN);
+    Table table;
+    table.init(p, BN);
 
     f4 acc[MB][NB];
     v4i a[MB], b[NB];
@@ -1029,17 +1087,20 @@ struct TurnKernel {
     };
     clear();
 
-    Stream ca, cb;
+    Stream<SA, true> ca;
+    Stream<SB, false> cb;
     ScaleStream cs;
-    ca.start(p, finder, t, true);
-    cb.start(p, finder, t, false);
-    if constexpr (kScaled) cs.start(p, finder, wave, lane);
+    ca.start(p, table, t);
+    cb.start(p, table, t);
+    if constexpr (kScaled) cs.start(p, table, wave, lane);
+    auto issue_a = [&]() { ca.issue(p, table, smem, t, wave); };
+    auto issue_b = [&]() { cb.issue(p, table, smem, t, wave); };
     // ahead of the first slot: A 0, B 0 and, with five units, A 1
 #pragma nounroll
     for (int i = 0; i < (UNITS == 5 ? 2 : 1); ++i) {
-      ca.issue(p, finder, smem, t, wave);
-      if (i == 0) cb.issue(p, finder, smem, t, wave);
-      if constexpr (kScaled) cs.issue(p, finder, smem, wave, lane);
+      issue_a();
+      if (i == 0) issue_b();
+      if constexpr (kScaled) cs.issue(p, table, smem, wave, lane);
     }
     wait_barrier<0>();
     if (second) __builtin_amdgcn_s_barrier();
@@ -1054,11 +1115,13 @@ struct TurnKernel {
       }
     };
     auto multiply = [&](int s, int nb) {
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
         if (j == 0 || __builtin_expect(j < nb, 1))
 #pragma unroll
           for (int i = 0; i < MB; ++i) E::mma(a[i], b[j], acc[i][j], s, i, qa[i / 2], j, qb[j / 2]);
+      __builtin_amdgcn_s_setprio(0);
     };
     auto next_k = [&]() {
       ua = rotate(ua);
@@ -1066,41 +1129,8 @@ struct TurnKernel {
       if (kScaled) scales ^= (UNITS * UNIT) ^ (UNITS * UNIT + SS::BYTES);
     };
 
-    auto steady = [&](int used, int count) {
-      for (; count > 0; --count) {
-        read(0, used);
-        if (UNITS == 4)
-#pragma unroll
-          for (int r = 0; r < PARTS; ++r) ca.copy_part(smem, wave, r);
-#pragma unroll
-        for (int r = 0; r < PARTS; ++r)
-          if (r == 0 || __builtin_expect(r < cb.parts, 1)) cb.copy_part(smem, wave, r);
-        if constexpr (kScaled) cs.s.copy(smem + cs.at, cs.kt);
-        wait_barrier<63>();
-        __builtin_amdgcn_s_setprio(1);
-        multiply(0, used);
-        __builtin_amdgcn_s_setprio(0);
-        cb.advance();
-        if (UNITS == 4) ca.advance();
-        if constexpr (kScaled) cs.advance();
-        wait_barrier<63>();
-        read(1, used);
-        if (UNITS == 5)
-#pragma unroll
-          for (int r = 0; r < PARTS; ++r) ca.copy_part(smem, wave, r);
-        // the next k-tile is there; the copies of A just issued may go on
-        wait_barrier<UNITS == 5 ? PARTS : 0>();
-        __builtin_amdgcn_s_setprio(1);
-        multiply(1, used);
-        __builtin_amdgcn_s_setprio(0);
-        if (UNITS == 5) ca.advance();
-        next_k();
-        wait_barrier<63>();
-      }
-    };
-
     Tile tile;
-    for (int w = blockIdx.x; finder.find(p, w, tile); w += gridDim.x) {
+    for (int i = 0; table.get(i, tile); ++i) {
       const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * BN;
       const int64_t cols = RK ? p.n : tile.hi - tile.lo;
       const int nt = tiles_k(depth(p, tile));
@@ -1109,28 +1139,45 @@ struct TurnKernel {
       if (cols - n0 < BN) nb = (int)((cols - n0 + STEP - 1) / STEP);
       int kt = 0;
       while (kt < nt) {
-        // The steady state, without a branch: k-tiles of which every copy is
-        // whole and none the last of its tile.
+        // The steady state: k-tiles while every copy is whole and none the
+        // last of its tile.
         int count = ca.run();
         const int rb = cb.run();
         count = count < rb ? count : rb;
         if (kScaled) count = count < cs.run() ? count : cs.run();
         count = count < nt - kt ? count : nt - kt;
-        if (count > 0) {
-          kt += count;
-          steady(nb, count);
+        if (count > 0) kt += count;
+        for (; count > 0; --count) {
+          read(0, nb);
+          if (UNITS == 4) ca.copy(smem, wave);
+          cb.copy(smem, wave);
+          if constexpr (kScaled) cs.s.copy(smem + cs.at, cs.kt);
+          wait_barrier<63>();
+          multiply(0, nb);
+          cb.advance();
+          if (UNITS == 4) ca.advance();
+          if constexpr (kScaled) cs.advance();
+          wait_barrier<63>();
+          read(1, nb);
+          if (UNITS == 5) ca.copy(smem, wave);
+          // the next k-tile is there; the copies of A just issued may go on
+          wait_barrier<UNITS == 5 ? SA::LOADS : 0>();
+          multiply(1, nb);
+          if (UNITS == 5) ca.advance();
+          next_k();
+          wait_barrier<63>();
         }
         if (kt == nt) break;
         // one k-tile, whatever it and its copies are
         read(0, nb);
-        if (UNITS == 4) ca.issue(p, finder, smem, t, wave);
-        cb.issue(p, finder, smem, t, wave);
-        if constexpr (kScaled) cs.issue(p, finder, smem, wave, lane);
+        if (UNITS == 4) issue_a();
+        issue_b();
+        if constexpr (kScaled) cs.issue(p, table, smem, wave, lane);
         wait_barrier<63>();
         multiply(0, nb);
         wait_barrier<63>();
         read(1, nb);
-        if (UNITS == 5) ca.issue(p, finder, smem, t, wave);
+        if (UNITS == 5) issue_a();
         wait_barrier<0>();
         multiply(1, nb);
         next_k();
@@ -1138,10 +1185,171 @@ struct TurnKernel {
         ++kt;
       }
       const int64_t at = RK ? (int64_t)tile.g * p.stride_c : tile.lo * p.ldc;
-      store_tile<E, STEP>(p, at, acc, m0 + wm, n0 + wn, cols, lane);
+      store_tile<E, STEP, true>(p, at, acc, m0 + wm, n0 + wn, cols, lane);
       clear();
     }
     if (!second) __builtin_amdgcn_s_barrier();
+  }
+};
+
+// Few columns a group (single tokens): bound by reading A once. A block has
+// R row blocks and CB column blocks of 16; its eight waves share k in runs of
+// 256 bytes, load both operands straight into MFMA operand registers, the next
+// run ahead of the present one's MFMAs, and add their sums in LDS in the
+// waves' order. A k-contiguous only. The loads take any alignment.
+template <class E, int R, int CB>
+struct SkinnyKernel {
+  static constexpr int kBM = 16 * R, kBN = 16 * CB;
+  static constexpr int NW = 8, NT = 64 * NW;
+  static constexpr bool kScaled = E::kBits == 4;
+  static constexpr bool kPersistent = false;
+  static constexpr int RUN = 256, STEPS = RUN / 64;  // bytes of k, MFMA steps
+  static constexpr int LDS = NW * R * CB * 1024;
+
+  struct Operands {
+    v4i a[STEPS][R], b[STEPS][CB];
+    v4i qa[R], qb[CB];  // the run's scales of a row: a dword a step
+  };
+
+  // Chunk at `from` of which `left` elements exist.
+  static __device__ __forceinline__ v4i load_cut(const char *from, int64_t left) {
+    constexpr int EPC = 128 / E::kBits;
+    v4i v = {0, 0, 0, 0};
+    if (left >= EPC) {
+      v = *reinterpret_cast<const typename E::chunk *>(from);
+    } else if (left > 0) {
+      if constexpr (E::kBits == 16) {
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        s8 s = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < left) s[i] = reinterpret_cast<const short *>(from)[i];
+        v = __builtin_bit_cast(v4i, s);
+      } else if constexpr (E::kBits == 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < left) v[i] = reinterpret_cast<const int *>(from)[i];
+      }
+    }
+    return v;
+  }
+
+  static __device__ __forceinline__ void run(const Args &p, char *smem) {
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int i16 = lane & 15, g = lane >> 4;
+    Tile tile;
+    ColumnOrder order;
+    order.init(p, kBN);
+    if (!order.find(p, blockIdx.x, tile)) return;
+    const int64_t m0 = (int64_t)tile.tm * kBM, n0 = tile.lo + (int64_t)tile.tn * kBN;
+    const int64_t K = p.alpha == 0.0f ? 0 : p.k;  // alpha == 0 reads neither operand
+    const int64_t bytes = (K * E::kBits + 7) / 8;
+    const int runs = (int)((bytes + RUN - 1) / RUN), whole = (int)(bytes / RUN);
+
+    // this lane's chunk 0 of its rows and columns; past the end the last one
+    // is read again (what it gives is never stored)
+    const char *pa[R], *pb[CB];
+    const uint8_t *sa[R], *sb[CB];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      int64_t row = m0 + 16 * r + i16;
+      if (row >= p.m) row = p.m - 1;
+      pa[r] = p.A + (int64_t)tile.g * p.stride_a + row * p.lda + 16 * g;
+      if constexpr (kScaled) sa[r] = p.scale_a + (int64_t)tile.g * (p.stride_a / 16) + row * (p.lda / 16);
+    }
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      int64_t col = n0 + 16 * c + i16;
+      if (col >= tile.hi) col = tile.hi - 1;
+      pb[c] = p.B + col * p.ldb + 16 * g;
+      if constexpr (kScaled) sb[c] = p.scale_b + col * (p.ldb / 16);
+    }
+    auto load = [&](int run, Operands &o) {
+      const int64_t at = (int64_t)run * RUN;
+      if (run < whole) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) o.a[s][r] = *reinterpret_cast<const typename E::chunk *>(pa[r] + at + 64 * s);
+#pragma unroll
+          for (int c = 0; c < CB; ++c) o.b[s][c] = *reinterpret_cast<const typename E::chunk *>(pb[c] + at + 64 * s);
+        }
+        if constexpr (kScaled) {
+          typedef int v4d __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+          for (int r = 0; r < R; ++r) o.qa[r] = *reinterpret_cast<const v4d *>(sa[r] + at / 16);
+#pragma unroll
+          for (int c = 0; c < CB; ++c) o.qb[c] = *reinterpret_cast<const v4d *>(sb[c] + at / 16);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          const int64_t left = K - (at + 64 * s + 16 * g) * 8 / E::kBits;
+#pragma unroll
+          for (int r = 0; r < R; ++r) o.a[s][r] = load_cut(pa[r] + at + 64 * s, left);
+#pragma unroll
+          for (int c = 0; c < CB; ++c) o.b[s][c] = load_cut(pb[c] + at + 64 * s, left);
+          if constexpr (kScaled) {
+            // fp4: whole steps, K is a multiple of 128
+            const bool in = at + 64 * s < bytes;
+#pragma unroll
+            for (int r = 0; r < R; ++r) o.qa[r][s] = in ? *reinterpret_cast<const int *>(sa[r] + at / 16 + 4 * s) : 0;
+#pragma unroll
+            for (int c = 0; c < CB; ++c) o.qb[c][s] = in ? *reinterpret_cast<const int *>(sb[c] + at / 16 + 4 * s) : 0;
+          }
+        }
+      }
+    };
+    f4 acc[R][CB];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < CB; ++c) acc[r][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const Operands &o) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < CB; ++c) {
+            int qa = 0, qb = 0;
+            if constexpr (kScaled) {  // the lane group's byte
+              qa = (int)((uint32_t)o.qa[r][s] >> (8 * g));
+              qb = (int)((uint32_t)o.qb[c][s] >> (8 * g));
+            }
+            E::mma(o.a[s][r], o.b[s][c], acc[r][c], 0, 0, qa, 0, qb);
+          }
+    };
+    Operands x, y;
+    int run = wave;
+    if (run < runs) load(run, x);
+    while (run < runs) {
+      if (run + NW < runs) load(run + NW, y);
+      multiply(x);
+      run += NW;
+      if (run >= runs) break;
+      if (run + NW < runs) load(run + NW, x);
+      multiply(y);
+      run += NW;
+    }
+
+    // the waves' sums, one block (r, c) after the other: lane's f4 as it is
+    f4 *sums = reinterpret_cast<f4 *>(smem);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < CB; ++c) sums[(wave * R * CB + r * CB + c) * 64 + lane] = acc[r][c];
+    __syncthreads();
+    const int64_t cols = tile.hi - n0;
+#pragma unroll
+    for (int q = 0; q < (R * CB + NW - 1) / NW; ++q) {
+      const int at = wave + q * NW;
+      if (at >= R * CB) return;
+      f4 total[1][1] = {{sums[at * 64 + lane]}};
+#pragma unroll
+      for (int v = 1; v < NW; ++v) total[0][0] += sums[(v * R * CB + at) * 64 + lane];
+      store_tile<E, 16>(p, n0 * p.ldc, total, m0 + 16 * (at / CB), 16 * (at % CB), cols, lane);
+    }
   }
 };
 
@@ -1156,7 +1364,12 @@ template <class K>
 int launch(wgb_ctx *ctx, const Args &p, int64_t tiles) {
   if (tiles == 0) return WGB_OK;
   if (tiles > INT32_MAX) return wgb::fail(WGB_ERR_INVALID_VALUE, "grouped product: too many tiles");
-  const int64_t blocks = K::kPersistent && tiles > ctx->num_cus ? ctx->num_cus : tiles;
+  // a persistent launch: a block a CU, more where one could not keep its tiles
+  int64_t blocks = tiles;
+  if (K::kPersistent && tiles > ctx->num_cus) {
+    blocks = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
+    if (blocks < ctx->num_cus) blocks = ctx->num_cus;
+  }
   static const hipError_t attr =
       hipFuncSetAttribute((const void *)ragged_kernel<K>, hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
   if (attr != hipSuccess) return wgb::fail_hip(attr, "LDS size of a grouped product");
@@ -1173,6 +1386,36 @@ int launch_columns(wgb_ctx *ctx, Args &p) {
   p.tiles_m = (int)((p.m + K::kBM - 1) / K::kBM);
   const int64_t across = !p.off ? (p.n + bn - 1) / bn : p.n / bn + (p.n < p.groups ? p.n : p.groups);
   return launch<K>(ctx, p, across * p.tiles_m);
+}
+
+// Estimated time of a launch of T x T tiles, to choose among sizes: `first` us
+// for a tile of k = 1024 alone on its CU, `next` for each further one there
+// (several small blocks run at once; 256 x 256 tiles come in whole rounds),
+// and the time to write C at the 4.5 TB/s that large results reach. Measured:
+//   first / next      64 x 64       128 x 128     256 x 256
+//   16-bit            5.4 / 4.1     12.5 / 9.5    23.5
+//   fp4               4.0 / 1.5     5.6 / 3.3     9.5
+//   fp32              20 / 15.2     64 / 59.3     -
+// (us on 256 CUs; bf16 1024^3 8 / 13 / 26 us, 2048^3 33 / 28 / 45 us, 8192 x
+// 16384 x 4096 - / 1008 / 759 us; fp4 2048^3 19 / 13 / 25 us, 8192^3 - / 365 /
+// 302 us; fp32 1024^3 25 / 68 us, 8192 x 8192 x 2048 1944 / 1891 us).
+struct TileCost {
+  double first, next;
+};
+inline double tile_time(const wgb_ctx *ctx, const Args &p, int T, TileCost c, double tiles_n, double k, double c_size) {
+  const double tiles = (double)((p.m + T - 1) / T) * tiles_n / ctx->num_cus;
+  const double store = T * T * c_size / 17.6e3, depth = k / 1024;
+  if (T == 256) {
+    // a group's last tiles are cut short, and come last
+    const double rounds = tiles <= 1 ? 1 : (double)(int64_t)(tiles + 0.999) - (p.off && p.groups > 1 ? 0.3 : 0.0);
+    return rounds * (c.first * depth + store);
+  }
+  return c.first * depth + store + (tiles > 1 ? tiles - 1 : 0) * (c.next * depth + store);
+}
+// Column tiles of a ragged launch to expect: every group's last one is half full.
+inline double expected_columns(const Args &p, int T) {
+  if (!p.off || p.groups == 1) return (double)((p.n + T - 1) / T);
+  return (double)p.n / T + 0.5 * (double)(p.n < p.groups ? p.n : p.groups);
 }
 
 template <class K>
