@@ -33,10 +33,10 @@ constexpr TileCost cost(int T) {
 template <class E, bool VEC>
 int choose(wgb_ctx *ctx, const Args &p, double k, double n64, double n128, double n256) {
   const double size = p.c_f32 ? 4 : 2;
-  const double t64 = tile_time(ctx, p, 64, cost<E>(64), n64, k, size);
-  const double t128 = tile_time(ctx, p, 128, cost<E>(128), n128, k, size);
+  const double t64 = small_time(64, cost<E>(64), per_cu(ctx, p, 64, n64), k, size);
+  const double t128 = small_time(128, cost<E>(128), per_cu(ctx, p, 128, n128), k, size);
   if (VEC && E::kBits == 16) {
-    const double t256 = tile_time(ctx, p, 256, cost<E>(256), n256, k, size);
+    const double t256 = rounds_time(cost<E>(256), cost<E>(128), per_cu(ctx, p, 256, n256), k, size);
     if (t256 <= t128 && t256 <= t64) return 256;
   }
   return t128 <= t64 ? 128 : 64;
@@ -59,7 +59,8 @@ int run_columns(wgb_ctx *ctx, Args &p) {
   }
   const int T = choose<E, VEC>(ctx, p, (double)p.k, expected_columns(p, 64), expected_columns(p, 128), expected_columns(p, 256));
   if constexpr (VEC && E::kBits == 16) {
-    if (T == 256) return launch_columns<TurnKernel<E, AMC, false, false>>(ctx, p);
+    if (T == 256)
+      return launch_columns_rounds<TurnKernel<E, AMC, false, false>, Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
   }
   if (T == 128) return launch_columns<Kernel<E, 128, 128, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
   return launch_columns<Kernel<E, 64, 64, 2, 2, AMC, false, VEC, false, 2>>(ctx, p);
@@ -70,7 +71,8 @@ int run_k(wgb_ctx *ctx, Args &p) {
   auto across = [&](int64_t T) { return (double)((p.n + T - 1) / T * p.groups); };
   const int T = choose<E, VEC>(ctx, p, (double)p.k / p.groups, across(64), across(128), across(256));
   if constexpr (VEC && E::kBits == 16) {
-    if (T == 256) return launch_k<TurnKernel<E, true, true, true>>(ctx, p);
+    if (T == 256)
+      return launch_k_rounds<TurnKernel<E, true, true, true>, Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>>(ctx, p);
   }
   if (T == 128) return launch_k<Kernel<E, 128, 128, 2, 2, true, true, VEC, true, 2>>(ctx, p);
   return launch_k<Kernel<E, 64, 64, 2, 2, true, true, VEC, true, 2>>(ctx, p);

@@ -127,6 +127,9 @@ struct Args {
   void *C;
   int64_t ldc, stride_c;  // elements; stride_c: ragged k only
   float alpha, beta;
+  // CUs of a persistent launch of 256 x 256 tiles, which leaves a last round
+  // that would use at most half of them to 128 x 128 tiles; 0: no such launch
+  int round;
   int c_f32;  // C holds fp32 (else the operands' type; fp4: bf16, or f16 with c_f16)
   int c_f16;
 };
@@ -292,8 +295,9 @@ struct KOrder {
   }
   // Each lane's tile w < total (lanes may have the same).
   __device__ __forceinline__ void find_lanes(const Args &p, int w, Tile &t) {
-    const int round = w / (int)gridDim.x, begin = round * (int)gridDim.x;
-    const int end = begin + (int)gridDim.x < total ? begin + (int)gridDim.x : total;
+    const int blocks = p.round ? p.round : (int)gridDim.x;
+    const int round = w / blocks, begin = round * blocks;
+    const int end = begin + blocks < total ? begin + blocks : total;
     const int at = round & 1 ? begin + end - 1 - w : w;
     const int place = at / per;
     wgb_tiles::logical_tile(wgb_tiles::xcd_remap(at - place * per, per), p.tiles_m, p.tiles_n, 0, t.tm, t.tn);
@@ -328,6 +332,14 @@ struct KOrder {
   }
 };
 
+// Of `total` 256 x 256 tiles those that the persistent launch computes: whole
+// rounds, and the rest if it is more than half a round.
+__device__ __forceinline__ int whole_rounds(const Args &p, int total) {
+  if (!p.round) return total;
+  const int cut = total / p.round * p.round;
+  return total - cut > p.round / 2 ? total : cut;
+}
+
 // A persistent block's tiles, one a lane: all of them are found at the start.
 constexpr int kTilesPerBlock = 64;
 template <class Order>
@@ -339,7 +351,8 @@ struct TileTable {
     Order o;
     o.init(p, bn);
     const int first = (int)blockIdx.x, step = (int)gridDim.x;
-    count = first < o.total ? (o.total - first + step - 1) / step : 0;
+    const int total = whole_rounds(p, o.total);
+    count = first < total ? (total - first + step - 1) / step : 0;
     if (count > kTilesPerBlock) count = kTilesPerBlock;  // the launch has blocks enough
     const int lane = threadIdx.x & 63;
     Tile t = {0, 0, 0, 0, 0};
@@ -772,7 +785,6 @@ struct Kernel {
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int MB = BM / WM / 16, NB = BN / WN / 16;
   static constexpr bool kScaled = E::kBits == 4;
-  static constexpr bool kPersistent = false;  // a block a tile
   typedef Stager<E, BM, AMC, NT> SA;
   typedef Stager<E, BN, BMC, NT> SB;
   typedef ScaleStager<kScaled ? BM : 64, kScaled ? BN : 64, NW> SS;
@@ -786,10 +798,19 @@ struct Kernel {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     Tile tile;
     typename std::conditional<RK, KOrder, ColumnOrder>::type order;
-    order.init(p, BN);
-    if (!order.find(p, blockIdx.x, tile)) return;
+    if (BM == 128 && BN == 128 && p.round) {
+      // a quarter of a 256 x 256 tile that the persistent launch left
+      order.init(p, 256);
+      if (!order.find(p, whole_rounds(p, order.total) + blockIdx.x / 4, tile)) return;
+      tile.tm = 2 * tile.tm + (blockIdx.x & 1);
+      tile.tn = 2 * tile.tn + ((blockIdx.x >> 1) & 1);
+    } else {
+      order.init(p, BN);
+      if (!order.find(p, blockIdx.x, tile)) return;
+    }
     const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * BN;
     const int64_t cols = RK ? p.n : tile.hi - tile.lo;
+    if (m0 >= p.m || n0 >= cols) return;
     int64_t K = RK ? tile.hi - tile.lo : p.k;
     if (p.alpha == 0.0f) K = 0;  // reads neither operand
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
@@ -936,7 +957,6 @@ struct TurnKernel {
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int MB = BM / WM / 16, NB = BN / WN / 16, STEP = 16 * WN;
   static constexpr bool kScaled = E::kBits == 4;
-  static constexpr bool kPersistent = true;  // at most one block a CU
   typedef Stager<E, BM, AMC, NT> SA;
   typedef Stager<E, BN, BMC, NT> SB;
   typedef ScaleStager<kScaled ? BM : 64, kScaled ? BN : 64, NW> SS;
@@ -1202,7 +1222,6 @@ struct SkinnyKernel {
   static constexpr int kBM = 16 * R, kBN = 16 * CB;
   static constexpr int NW = 8, NT = 64 * NW;
   static constexpr bool kScaled = E::kBits == 4;
-  static constexpr bool kPersistent = false;
   static constexpr int RUN = 256, STEPS = RUN / 64;  // bytes of k, MFMA steps
   static constexpr int LDS = NW * R * CB * 1024;
 
@@ -1359,17 +1378,10 @@ __global__ __launch_bounds__(K::NT, 2) void ragged_kernel(Args p) {
   K::run(p, ragged_smem);
 }
 
-// `tiles`: at most.
 template <class K>
-int launch(wgb_ctx *ctx, const Args &p, int64_t tiles) {
-  if (tiles == 0) return WGB_OK;
-  if (tiles > INT32_MAX) return wgb::fail(WGB_ERR_INVALID_VALUE, "grouped product: too many tiles");
-  // a persistent launch: a block a CU, more where one could not keep its tiles
-  int64_t blocks = tiles;
-  if (K::kPersistent && tiles > ctx->num_cus) {
-    blocks = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
-    if (blocks < ctx->num_cus) blocks = ctx->num_cus;
-  }
+int launch(wgb_ctx *ctx, const Args &p, int64_t blocks) {
+  if (blocks == 0) return WGB_OK;
+  if (blocks > INT32_MAX) return wgb::fail(WGB_ERR_INVALID_VALUE, "grouped product: too many tiles");
   static const hipError_t attr =
       hipFuncSetAttribute((const void *)ragged_kernel<K>, hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
   if (attr != hipSuccess) return wgb::fail_hip(attr, "LDS size of a grouped product");
@@ -1380,12 +1392,49 @@ int launch(wgb_ctx *ctx, const Args &p, int64_t tiles) {
 
 // Tiles that a ragged-columns launch has at most: a group of c columns has
 // ceil(c / bn) column tiles, at most one of them partly filled.
+inline int64_t most_columns(const Args &p, int64_t bn) {
+  return !p.off ? (p.n + bn - 1) / bn : p.n / bn + (p.n < p.groups ? p.n : p.groups);
+}
+
 template <class K>
 int launch_columns(wgb_ctx *ctx, Args &p) {
-  const int64_t bn = K::kBN;
   p.tiles_m = (int)((p.m + K::kBM - 1) / K::kBM);
-  const int64_t across = !p.off ? (p.n + bn - 1) / bn : p.n / bn + (p.n < p.groups ? p.n : p.groups);
-  return launch<K>(ctx, p, across * p.tiles_m);
+  return launch<K>(ctx, p, most_columns(p, K::kBN) * p.tiles_m);
+}
+
+template <class K>
+int launch_k(wgb_ctx *ctx, Args &p) {
+  p.tiles_m = (int)((p.m + K::kBM - 1) / K::kBM);
+  p.tiles_n = (int)((p.n + K::kBN - 1) / K::kBN);
+  return launch<K>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
+}
+
+// `Turn` on at most `tiles` 256 x 256 tiles, a block a CU (more where one
+// could not keep its tiles), then `Rest` (128 x 128 tiles, a quarter of one
+// each) on what that leaves. Which tiles there are is only known on the GPU.
+template <class Turn, class Rest>
+int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles) {
+  int64_t blocks = tiles;
+  if (tiles > ctx->num_cus) {
+    blocks = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
+    if (blocks <= ctx->num_cus) blocks = p.round = ctx->num_cus;
+  }
+  const int st = launch<Turn>(ctx, p, blocks);
+  if (st || !p.round) return st;
+  return launch<Rest>(ctx, p, (int64_t)(p.round / 2) * 4);
+}
+
+template <class Turn, class Rest>
+int launch_columns_rounds(wgb_ctx *ctx, Args &p) {
+  p.tiles_m = (int)((p.m + Turn::kBM - 1) / Turn::kBM);
+  return launch_rounds<Turn, Rest>(ctx, p, most_columns(p, Turn::kBN) * p.tiles_m);
+}
+
+template <class Turn, class Rest>
+int launch_k_rounds(wgb_ctx *ctx, Args &p) {
+  p.tiles_m = (int)((p.m + Turn::kBM - 1) / Turn::kBM);
+  p.tiles_n = (int)((p.n + Turn::kBN - 1) / Turn::kBN);
+  return launch_rounds<Turn, Rest>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
 }
 
 // Estimated time of a launch of T x T tiles, to choose among sizes: `first` us
@@ -1402,27 +1451,25 @@ int launch_columns(wgb_ctx *ctx, Args &p) {
 struct TileCost {
   double first, next;
 };
-inline double tile_time(const wgb_ctx *ctx, const Args &p, int T, TileCost c, double tiles_n, double k, double c_size) {
-  const double tiles = (double)((p.m + T - 1) / T) * tiles_n / ctx->num_cus;
+// `tiles`: on each CU.
+inline double small_time(int T, TileCost c, double tiles, double k, double c_size) {
   const double store = T * T * c_size / 17.6e3, depth = k / 1024;
-  if (T == 256) {
-    // a group's last tiles are cut short, and come last
-    const double rounds = tiles <= 1 ? 1 : (double)(int64_t)(tiles + 0.999) - (p.off && p.groups > 1 ? 0.3 : 0.0);
-    return rounds * (c.first * depth + store);
-  }
   return c.first * depth + store + (tiles > 1 ? tiles - 1 : 0) * (c.next * depth + store);
+}
+// 256 x 256 tiles: whole rounds, then the rest as launch_rounds has it.
+inline double rounds_time(TileCost c256, TileCost c128, double tiles, double k, double c_size) {
+  const double store = 256 * 256 * c_size / 17.6e3, round = c256.first * (k / 1024) + store;
+  const double whole = (double)(int64_t)tiles, rest = tiles - whole;
+  if (rest < 0.01) return whole * round;
+  return whole * round + (rest > 0.5 || whole == 0 ? round : small_time(128, c128, 4 * rest, k, c_size));
+}
+inline double per_cu(const wgb_ctx *ctx, const Args &p, int T, double tiles_n) {
+  return (double)((p.m + T - 1) / T) * tiles_n / ctx->num_cus;
 }
 // Column tiles of a ragged launch to expect: every group's last one is half full.
 inline double expected_columns(const Args &p, int T) {
   if (!p.off || p.groups == 1) return (double)((p.n + T - 1) / T);
   return (double)p.n / T + 0.5 * (double)(p.n < p.groups ? p.n : p.groups);
-}
-
-template <class K>
-int launch_k(wgb_ctx *ctx, Args &p) {
-  p.tiles_m = (int)((p.m + K::kBM - 1) / K::kBM);
-  p.tiles_n = (int)((p.n + K::kBN - 1) / K::kBN);
-  return launch<K>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
 }
 
 }  // namespace wgb_ragged
