@@ -81,7 +81,7 @@ def test_k(ctx, t, ct, beta, m, n, sizes):
 
 @pytest.mark.parametrize("ct", ["bf16", "f32", "f16"])
 @pytest.mark.parametrize("m,k,sizes", [(8200, 1504, [1300, 0, 1, 2047, 300, 77]), (4096, 1536, [4096]), (4100, 1408, [850] * 4),
-                                       (8192, 640, [4000, 300])])
+                                       (8192, 640, [4000, 300]), (4100, 384, [10] * 20), (4100, 448, [25] * 20)])
 def test_mxfp4(ctx, ct, m, k, sizes):
     rng = np.random.default_rng(m + k)
     off = R.boundaries(sizes)
@@ -107,6 +107,63 @@ def test_mxfp4(ctx, ct, m, k, sizes):
         if lo < hi:
             W, x = values(ca[g * m + rows], sa[g * m + rows]).T, values(cb[lo:hi], sb[lo:hi])
             R.assert_product(R.decode(got[lo:hi, rows], ct), x @ W, np.abs(x) @ np.abs(W), k, ct)
+
+
+@pytest.mark.parametrize("trans", [NO_TRANS, TRANS])
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,k,sizes,pad,shift", [
+    (4096, 1024, [4096], 0, 0), (2049, 513, [2049], 0, 0), (2049, 513, [2049], 0, 1), (4100, 384, [10] * 20, 0, 0),
+    (4100, 383, [10] * 20, 0, 0), (1500, 400, [3000, 2000, 500], 1, 0), (1500, 401, [3000, 2000, 500], 1, 1),
+    (600, 90, [20, 30, 700, 3], 1 << 20, 0)])
+def test_columns_other_tiles_and_alignments(ctx, t, trans, m, k, sizes, pad, shift):
+    """128 x 128 and 128 x 32 tiles, operands moved to an aligned workspace, leading dimensions past the copies' offsets."""
+    rng = np.random.default_rng(m + k + shift)
+    off = R.boundaries(sizes)
+    n, groups = int(off[-1]), len(sizes)
+    rows, cols = (k, m) if trans == TRANS else (m, k)
+    wide = pad >= 1 << 20
+    lda, ldb = (rows, k + pad) if wide else (rows + pad, k + pad)
+    A, B = values16(rng, (groups, cols, lda), t), values16(rng, (n, k if wide else ldb), t)
+    dA, dO, dC = ctx.upload(np.concatenate([A.reshape(-1)[:shift], A.reshape(-1)])), ctx.upload(off), ctx.empty((n, m), np.float32)
+    if wide:
+        dB = ctx.empty(n * ldb, R.STORE[t])
+        for j in range(n):
+            ctx.h2d(dB.offset(j * ldb), B[j])
+    else:
+        dB = ctx.upload(np.concatenate([B.reshape(-1)[:shift], B.reshape(-1)]))
+    ctx.gemm_grouped(R.TYPES[t], trans, groups, m, n, k, 1.0, dA.offset(shift), lda, cols * lda, dB.offset(shift), ldb, dO, 0.0,
+                     dC, m, R.TYPES["f32"])
+    got = dC.to_host()
+    for d in (dA, dB, dC, dO):
+        d.free()
+    pick = sample(rng, m, 60)
+    for g in range(groups):
+        lo, hi = off[g], off[g + 1]
+        W = R.decode(A[g, pick, :k].T if trans == TRANS else A[g][:, pick], t)
+        x = R.decode(B[lo:hi, :k], t)
+        R.assert_product(got[lo:hi, pick].astype(np.float64), x @ W, np.abs(x) @ np.abs(W), k, "f32")
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,n,sizes,pad,shift", [(4096, 4096, [1024], 0, 0), (2049, 2051, [600], 0, 0), (2049, 2051, [600], 0, 1),
+                                                 (1500, 3001, [900, 300, 0, 40], 1, 1)])
+def test_k_other_tiles_and_alignments(ctx, t, m, n, sizes, pad, shift):
+    rng = np.random.default_rng(m + n + shift)
+    off = R.boundaries(sizes)
+    k, groups = int(off[-1]), len(sizes)
+    A, B = values16(rng, (k, m + pad), t), values16(rng, (k, n + pad), t)
+    dA = ctx.upload(np.concatenate([A.reshape(-1)[:shift], A.reshape(-1)]))
+    dB = ctx.upload(np.concatenate([B.reshape(-1)[:shift], B.reshape(-1)]))
+    dO, dC = ctx.upload(off), ctx.empty((groups, n, m), np.float32)
+    ctx.gemm_grouped_k(R.TYPES[t], groups, m, n, k, 1.0, dA.offset(shift), m + pad, dB.offset(shift), n + pad, dO, 0.0, dC, m,
+                       n * m, R.TYPES["f32"])
+    got = dC.to_host()
+    for d in (dA, dB, dC, dO):
+        d.free()
+    pick = sample(rng, m, 60)
+    for g in range(groups):
+        a, b = R.decode(A[off[g]:off[g + 1]][:, pick], t), R.decode(B[off[g]:off[g + 1], :n], t)
+        R.assert_product(got[g][:, pick].astype(np.float64), b.T @ a, np.abs(b).T @ np.abs(a), sizes[g], "f32")
 
 
 def test_more_tiles_than_a_block_lists(ctx):

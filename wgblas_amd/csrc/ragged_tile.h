@@ -322,9 +322,18 @@ struct KOrder {
         t.hi = __builtin_amdgcn_readlane(hi, g);
       }
   }
+  // Tile w of a wave: false if there is none. A launch of its own takes the
+  // groups as they are (ranking 64 of them costs every block a microsecond);
+  // the rest of a persistent launch has to keep that one's order.
   __device__ __forceinline__ bool find(const Args &p, int w, Tile &t) {
     if (w >= total) return false;
-    find_lanes(p, w, t);
+    if (p.round) {
+      find_lanes(p, w, t);
+    } else {
+      t.g = w / per;
+      wgb_tiles::logical_tile(wgb_tiles::xcd_remap(w - t.g * per, per), p.tiles_m, p.tiles_n, 0, t.tm, t.tn);
+      group_range(p.off, t.g, p.k, t.lo, t.hi);
+    }
     t.g = __builtin_amdgcn_readfirstlane(t.g);
     t.lo = __builtin_amdgcn_readfirstlane((int)t.lo);
     t.hi = __builtin_amdgcn_readfirstlane((int)t.hi);
