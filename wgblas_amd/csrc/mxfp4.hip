@@ -379,7 +379,7 @@ int product(wgb_ctx *ctx, Args &p) {
     return launch_columns<Kernel<Fp4, 128, 32, 4, 1, false, false, true, false, 2>>(ctx, p);
   }
   const double k = (double)p.k, size = p.c_f32 ? 4 : 2;
-  const TileCost c64 = {4.0, 1.5}, c128 = {5.6, 3.3}, c256 = {9.5, 9.5};
+  const TileCost c64 = {4.0, 1.5}, c128 = {5.6, 3.3}, c256 = {10.5, 10.5};
   const double t64 = small_time(64, c64, per_cu(ctx, p, 64, expected_columns(p, 64)), k, size);
   const double t128 = small_time(128, c128, per_cu(ctx, p, 128, expected_columns(p, 128)), k, size);
   const double t256 = rounds_time(c256, c128, per_cu(ctx, p, 256, expected_columns(p, 256)), k, size);

@@ -130,7 +130,8 @@ struct Args {
   // CUs of a persistent launch of 256 x 256 tiles, which leaves a last round
   // that would use at most half of them to 128 x 128 tiles; 0: no such launch
   int round;
-  int c_f32;  // C holds fp32 (else the operands' type; fp4: bf16, or f16 with c_f16)
+  int stream;  // C's columns start at 64-byte boundaries: large results bypass the caches
+  int c_f32;   // C holds fp32 (else the operands' type; fp4: bf16, or f16 with c_f16)
   int c_f16;
 };
 
@@ -496,6 +497,19 @@ struct Stager : StagerData<BT * TB / 16 / NT> {
     for (int r = 0; r < LOADS; ++r) copy_chunks(from, voff[r], stage + wave * 1024 + r * NT * 16);
   }
 
+  // A last k-tile that K cuts can be copied too, chunks past K reading one
+  // that exists: whoever reads the operands then clears what is past K
+  // (tail_mask). Not where a cut chunk could reach past the matrix: at its
+  // last row (k-contiguous), or with cut rows (row-contiguous).
+  __device__ __forceinline__ bool soft_tail() const {
+    return MC ? rows_left >= BT : K % EPC == 0 || (rows_left > BT && K >= EPC);
+  }
+  __device__ __forceinline__ uint32_t tail_voff(int r) const {
+    const int left = (int)(K % BK);
+    if (MC) return voff[r] - (slot_row(r) < left ? 0u : (uint32_t)(slot_row(r) * ld));
+    return voff[r] - (slot_chunk(r) * EPC < left ? 0u : (uint32_t)(slot_chunk(r) * 16));
+  }
+
   // fp4, a last k-tile of which only the first 64 bytes exist: the other four
   // chunks of a row read those again. What they hold does not matter (a code
   // is never Inf or NaN), for their scales are staged as 2^-127 in both
@@ -596,6 +610,30 @@ struct Stager : StagerData<BT * TB / 16 / NT> {
   }
 };
 
+// Of a lane's chunk of which `left` elements are before the end of k: all
+// ones there, zeros after.
+template <class E>
+__device__ __forceinline__ v4i tail_mask(int left) {
+  v4i m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (E::kBits == 32)
+      m[i] = left > i ? -1 : 0;
+    else
+      m[i] = left >= 2 * i + 2 ? -1 : left == 2 * i + 1 ? 0xffff : 0;
+  }
+  return m;
+}
+// The operands of step s of a k-tile with `left` elements of k.
+template <class E, int MB, int NB>
+__device__ __forceinline__ void clear_tail(int left, int s, int lane, v4i (&a)[MB], v4i (&b)[NB]) {
+  const v4i m = tail_mask<E>(left - (4 * s + (lane >> 4)) * (128 / E::kBits));
+#pragma unroll
+  for (int i = 0; i < MB; ++i) a[i] &= m;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) b[j] &= m;
+}
+
 // The scales of a k-tile: 8 bytes a row, A's rows then B's, copied 4
 // bytes a lane. The waves share the copies evenly (a wave past the last one
 // copies the last again, the same bytes to the same place), so that every
@@ -693,7 +731,8 @@ __device__ __forceinline__ v4i eight_rows(uint32_t x0, uint32_t x1, uint32_t y0,
 // alpha acc + beta C for a lane's runs of four rows of one column; column
 // blocks are STEP columns apart. STREAM: non-temporal stores, for results too
 // large for the caches (8192 x 16384 in bf16 773 -> 760 us, 8 x 4096 x 2048 in
-// fp32 195 -> 184 us; 12 x 1032 x 520 in f16, which fits, 16.7 -> 21 us). fp32 is stored in those runs (16 bytes a
+// fp32 195 -> 184 us; 12 x 1032 x 520 in f16, which fits, 16.7 -> 21 us) and whose
+// columns do not cut lines (12872 columns of 2249 fp32 values 109 -> 168 us). fp32 is stored in those runs (16 bytes a
 // lane), 16-bit values in runs of eight rows (also 16 bytes) where there are
 // two row blocks: with 8 bytes a lane 8192 x 16384 x 4096 took 788 us.
 template <typename T, int MB, int NB, int STEP, bool STREAM>
@@ -850,6 +889,8 @@ struct Kernel {
         const int wb = sb.whole_tiles();
         whole = whole < wb ? whole : wb;
       }
+      const int cut = kScaled ? 0 : (int)(K % SA::BK);  // elements of k in a cut last k-tile
+      const bool soft = VEC && cut && whole == nt - 1 && sa.soft_tail() && sb.soft_tail();
 
       auto guarded = [&](int kt) {
         char *st = smem + (kt % S) * STAGE;
@@ -876,10 +917,18 @@ struct Kernel {
         if constexpr (kScaled) ss.copy(st + SA::BYTES + SB::BYTES, kt);
       };
       auto fill = [&](int kt) {
-        if (VEC && kt < whole)
+        if (VEC && kt < whole) {
           copy(kt);
-        else
+        } else if (soft) {
+          char *st = smem + (kt % S) * STAGE;
+          const char *fa = sa.origin + (int64_t)kt * sa.step(), *fb = sb.origin + (int64_t)kt * sb.step();
+#pragma unroll
+          for (int r = 0; r < SA::LOADS; ++r) copy_chunks(fa, sa.tail_voff(r), st + wave * 1024 + r * NT * 16);
+#pragma unroll
+          for (int r = 0; r < SB::LOADS; ++r) copy_chunks(fb, sb.tail_voff(r), st + SA::BYTES + wave * 1024 + r * NT * 16);
+        } else {
           guarded(kt);
+        }
       };
       auto fetch = [&](int kt, int s, v4i (&a)[MB], v4i (&b)[NB]) {
         const char *st = smem + (kt % S) * STAGE;
@@ -913,6 +962,7 @@ struct Kernel {
       fetch(0, 0, xa, xb);
       fetch_scales(0, qa, qb);
       int kt = 0;
+      if (soft && nt == 1) clear_tail<E>(cut, 0, lane, xa, xb);
       // steady: tile kt + S exists and is whole, so are those before it
       const int steady = (whole < nt ? whole : nt) - S;
       for (; kt < steady; ++kt) {
@@ -926,10 +976,12 @@ struct Kernel {
       }
       for (; kt < nt; ++kt) {
         fetch(kt, 1, ya, yb);
+        if (soft && kt == nt - 1) clear_tail<E>(cut, 1, lane, ya, yb);
         mma(0, xa, xb, qa, qb);
         wait_barrier<0>();
         if (kt + S < nt) fill(kt + S);
         if (kt + 1 < nt) fetch(kt + 1, 0, xa, xb);
+        if (soft && kt + 1 == nt - 1) clear_tail<E>(cut, 0, lane, xa, xb);
         mma(1, ya, yb, qa, qb);
         if (kt + 1 < nt) fetch_scales(kt + 1, qa, qb);
       }
@@ -1039,13 +1091,13 @@ struct TurnKernel {
       if (nt == 0) return;
       if (kt < whole) {
         copy(smem, wave);
-      } else {
+      } else if (kScaled || (kt == nt - 1 && s.soft_tail())) {
 #pragma unroll
         for (int r = 0; r < S::LOADS; ++r)
-          if constexpr (E::kBits == 4)
-            copy_chunks(from, s.half_voff(r), smem + unit + wave * 1024 + r * NT * 16);
-          else
-            s.put(smem + unit, r, s.load_guarded(kt, r));
+          copy_chunks(from, kScaled ? s.half_voff(r) : s.tail_voff(r), smem + unit + wave * 1024 + r * NT * 16);
+      } else {
+#pragma unroll
+        for (int r = 0; r < S::LOADS; ++r) s.put(smem + unit, r, s.load_guarded(kt, r));
       }
       advance();
       if (kt == nt) {
@@ -1162,7 +1214,8 @@ struct TurnKernel {
     for (int i = 0; table.get(i, tile); ++i) {
       const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * BN;
       const int64_t cols = RK ? p.n : tile.hi - tile.lo;
-      const int nt = tiles_k(depth(p, tile));
+      const int K = depth(p, tile), nt = tiles_k(K);
+      const int cut = kScaled ? 0 : K % SA::BK;  // elements of k in a cut last k-tile, which is not a steady one
       // column blocks in use: a group's last tile costs what its columns need
       int nb = NB;
       if (cols - n0 < BN) nb = (int)((cols - n0 + STEP - 1) / STEP);
@@ -1174,7 +1227,8 @@ struct TurnKernel {
         const int rb = cb.run();
         count = count < rb ? count : rb;
         if (kScaled) count = count < cs.run() ? count : cs.run();
-        count = count < nt - kt ? count : nt - kt;
+        const int rest = nt - kt - (cut ? 1 : 0);
+        count = count < rest ? count : rest;
         if (count > 0) kt += count;
         for (; count > 0; --count) {
           read(0, nb);
@@ -1198,7 +1252,9 @@ struct TurnKernel {
         }
         if (kt == nt) break;
         // one k-tile, whatever it and its copies are
+        const bool last = cut && kt == nt - 1;
         read(0, nb);
+        if (last) clear_tail<E>(cut, 0, lane, a, b);
         if (UNITS == 4) issue_a();
         issue_b();
         if constexpr (kScaled) cs.issue(p, table, smem, wave, lane);
@@ -1206,6 +1262,7 @@ struct TurnKernel {
         multiply(0, nb);
         wait_barrier<63>();
         read(1, nb);
+        if (last) clear_tail<E>(cut, 1, lane, a, b);
         if (UNITS == 5) issue_a();
         wait_barrier<0>();
         multiply(1, nb);
@@ -1214,7 +1271,10 @@ struct TurnKernel {
         ++kt;
       }
       const int64_t at = RK ? (int64_t)tile.g * p.stride_c : tile.lo * p.ldc;
-      store_tile<E, STEP, true>(p, at, acc, m0 + wm, n0 + wn, cols, lane);
+      if (p.stream)
+        store_tile<E, STEP, true>(p, at, acc, m0 + wm, n0 + wn, cols, lane);
+      else
+        store_tile<E, STEP, false>(p, at, acc, m0 + wm, n0 + wn, cols, lane);
       clear();
     }
     if (!second) __builtin_amdgcn_s_barrier();
@@ -1423,6 +1483,7 @@ int launch_k(wgb_ctx *ctx, Args &p) {
 // each) on what that leaves. Which tiles there are is only known on the GPU.
 template <class Turn, class Rest>
 int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles) {
+  p.stream = ((uintptr_t)p.C & 63) == 0 && p.ldc * (p.c_f32 ? 4 : 2) % 64 == 0 && p.stride_c * (p.c_f32 ? 4 : 2) % 64 == 0;
   int64_t blocks = tiles;
   if (tiles > ctx->num_cus) {
     blocks = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
@@ -1452,7 +1513,7 @@ int launch_k_rounds(wgb_ctx *ctx, Args &p) {
 // and the time to write C at the 4.5 TB/s that large results reach. Measured:
 //   first / next      64 x 64       128 x 128     256 x 256
 //   16-bit            5.4 / 4.1     12.5 / 9.5    23.5
-//   fp4               4.0 / 1.5     5.6 / 3.3     9.5
+//   fp4               4.0 / 1.5     5.6 / 3.3     10.5
 //   fp32              20 / 15.2     64 / 59.3     -
 // (us on 256 CUs; bf16 1024^3 8 / 13 / 26 us, 2048^3 33 / 28 / 45 us, 8192 x
 // 16384 x 4096 - / 1008 / 759 us; fp4 2048^3 19 / 13 / 25 us, 8192^3 - / 365 /
@@ -1470,7 +1531,7 @@ inline double rounds_time(TileCost c256, TileCost c128, double tiles, double k, 
   const double store = 256 * 256 * c_size / 17.6e3, round = c256.first * (k / 1024) + store;
   const double whole = (double)(int64_t)tiles, rest = tiles - whole;
   if (rest < 0.01) return whole * round;
-  return whole * round + (rest > 0.5 || whole == 0 ? round : small_time(128, c128, 4 * rest, k, c_size));
+  return whole * round + (rest > 0.5 || whole == 0 ? round : small_time(128, c128, 4 * rest, k, c_size) + 4);
 }
 inline double per_cu(const wgb_ctx *ctx, const Args &p, int T, double tiles_n) {
   return (double)((p.m + T - 1) / T) * tiles_n / ctx->num_cus;
