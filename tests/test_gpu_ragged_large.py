@@ -166,6 +166,71 @@ def test_k_other_tiles_and_alignments(ctx, t, m, n, sizes, pad, shift):
         R.assert_product(got[g][:, pick].astype(np.float64), b.T @ a, np.abs(b).T @ np.abs(a), sizes[g], "f32")
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("trans", [NO_TRANS, TRANS])
+@pytest.mark.parametrize("m,k,sizes", [(100, 200, [70, 90, 65]), (100, 203, [70, 90, 65]), (700, 150, [300, 200, 129]),
+                                       (700, 157, [300, 200, 129]), (2304, 1003, [1100, 1300, 520]), (2304, 1000, [1100, 1300, 520]),
+                                       (300, 5, [90, 70, 64]), (4100, 203, [9] * 20)])
+def test_what_is_past_k_is_never_used(ctx, t, trans, m, k, sizes):
+    """NaN and Inf in the padding behind every column and in the middle group's tokens: the other groups' results are
+    finite and right, the middle group's are NaN."""
+    rng = np.random.default_rng(m + k)
+    off = R.boundaries(sizes)
+    n, groups, bad = int(off[-1]), len(sizes), 1
+    rows, cols = (k, m) if trans == TRANS else (m, k)
+    lda, ldb = rows + 2 + rows % 2, k + 2 + k % 2
+    nan, inf = R.encode(np.array([np.nan, np.inf], np.float32), t)
+    A, B = values16(rng, (groups, cols, lda), t), values16(rng, (n, ldb), t)
+    A[:, :, rows:], B[:, k:] = nan, inf
+    B[off[bad]:off[bad + 1], :k] = nan
+    dA, dB, dO, dC = ctx.upload(A), ctx.upload(B), ctx.upload(off), ctx.empty((n, m), np.float32)
+    ctx.gemm_grouped(R.TYPES[t], trans, groups, m, n, k, 1.0, dA, lda, cols * lda, dB, ldb, dO, 0.0, dC, m, R.TYPES["f32"])
+    got = dC.to_host()
+    pick = sample(rng, m, 40)
+    for g in range(groups):
+        lo, hi = off[g], off[g + 1]
+        if g == bad:
+            assert np.isnan(got[lo:hi]).all()
+            continue
+        W = R.decode(A[g, pick, :k].T if trans == TRANS else A[g][:, pick], t)
+        x = R.decode(B[lo:hi, :k], t)
+        R.assert_product(got[lo:hi, pick].astype(np.float64), x @ W, np.abs(x) @ np.abs(W), k, "f32")
+    # the weight gradient: k is the tokens, whose ends are the next group's tokens
+    Y = values16(rng, (n, m + 2 + m % 2), t)
+    Y[:, m:] = nan
+    dY, dW = ctx.upload(Y), ctx.empty((groups, m, k), np.float32)
+    ctx.gemm_grouped_k(R.TYPES[t], groups, k, m, n, 1.0, dB, ldb, dY, Y.shape[1], dO, 0.0, dW, k, m * k, R.TYPES["f32"])
+    grad = dW.to_host()
+    for d in (dA, dB, dO, dC, dY, dW):
+        d.free()
+    for g in range(groups):
+        if g == bad:
+            assert np.isnan(grad[g]).all()
+            continue
+        x, y = R.decode(B[off[g]:off[g + 1], :k], t), R.decode(Y[off[g]:off[g + 1]][:, pick], t)
+        R.assert_product(grad[g][pick].astype(np.float64), y.T @ x, np.abs(y).T @ np.abs(x), sizes[g], "f32")
+
+
+def test_calls_in_turn_on_two_contexts(ctx):
+    """Each context has its own stream and workspace; products of odd leading dimensions (moved to the workspace) of two
+    contexts, started before either is waited for, do not disturb one another."""
+    from wgblas_amd import Context
+
+    rng = np.random.default_rng(2)
+    m, k, n = 1501, 801, 1700
+    with Context(0) as other:
+        work = []
+        for c in (ctx, other):
+            A, B = values16(rng, (m, k), "bf16"), values16(rng, (n, k), "bf16")
+            work.append((c, A, B, c.upload(A), c.upload(B), c.upload(np.array([0, n], np.int64)), c.empty((n, m), np.float32)))
+        for _ in range(3):
+            for c, A, B, dA, dB, dO, dC in work:
+                c.gemm_grouped(R.TYPES["bf16"], TRANS, 1, m, n, k, 1.0, dA, k, m * k, dB, k, dO, 0.0, dC, m, R.TYPES["f32"])
+        for c, A, B, dA, dB, dO, dC in work:
+            W, x = R.decode(A, "bf16").T, R.decode(B, "bf16")
+            R.assert_product(dC.to_host().astype(np.float64), x @ W, np.abs(x) @ np.abs(W), k, "f32")
+
+
 def test_more_tiles_than_a_block_lists(ctx):
     """64 tiles a block are listed: 132 x 129 tiles of 256 need more blocks than CUs."""
     rng = np.random.default_rng(1)
