@@ -36,12 +36,12 @@ napi_value throw_status(napi_env env, int status, const char *what) {
   } while (0)
 
 struct Args {
-  napi_value v[16];
-  size_t n = 16;
+  napi_value v[20];
+  size_t n = 20;
 };
 
 bool get_args(napi_env env, napi_callback_info info, Args &a, size_t want) {
-  a.n = 16;
+  a.n = 20;
   if (napi_get_cb_info(env, info, &a.n, a.v, nullptr, nullptr) != napi_ok) return false;
   if (a.n < want) {
     napi_throw_type_error(env, nullptr, "wgblas_hip addon: too few arguments");
@@ -618,6 +618,118 @@ napi_value Reduce(napi_env env, napi_callback_info info) {
   return num(env, (double)r);
 }
 
+// ---- grouped and 4-bit products ---------------------------------------------
+
+// gemmGrouped(ctx, type, transA, groups, m, n, k, alpha, A, lda, strideA, B,
+// ldb, offsets, beta, C, ldc, ctype)
+napi_value GemmGrouped(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 18)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, ta, ctype;
+  int64_t groups, m, n, k, lda, strideA, ldb, ldc;
+  double alpha, beta;
+  void *A, *B, *off, *C;
+  if (!get_i32(env, a.v[1], &type) || !get_i32(env, a.v[2], &ta) || !get_i64(env, a.v[3], &groups) ||
+      !get_i64(env, a.v[4], &m) || !get_i64(env, a.v[5], &n) || !get_i64(env, a.v[6], &k) ||
+      !get_f64(env, a.v[7], &alpha) || !get_ptr(env, a.v[8], &A) || !get_i64(env, a.v[9], &lda) ||
+      !get_i64(env, a.v[10], &strideA) || !get_ptr(env, a.v[11], &B) || !get_i64(env, a.v[12], &ldb) ||
+      !get_ptr(env, a.v[13], &off) || !get_f64(env, a.v[14], &beta) || !get_ptr(env, a.v[15], &C) ||
+      !get_i64(env, a.v[16], &ldc) || !get_i32(env, a.v[17], &ctype))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_gemm_grouped(ctx, type, ta, groups, m, n, k, (float)alpha, A, lda, strideA, B, ldb,
+                                   (const int64_t *)off, (float)beta, C, ldc, ctype), "wgb_gemm_grouped");
+  return nullptr;
+}
+
+// gemmGroupedK(ctx, type, groups, m, n, k, alpha, A, lda, B, ldb, offsets,
+// beta, C, ldc, strideC, ctype)
+napi_value GemmGroupedK(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 17)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, ctype;
+  int64_t groups, m, n, k, lda, ldb, ldc, strideC;
+  double alpha, beta;
+  void *A, *B, *off, *C;
+  if (!get_i32(env, a.v[1], &type) || !get_i64(env, a.v[2], &groups) || !get_i64(env, a.v[3], &m) ||
+      !get_i64(env, a.v[4], &n) || !get_i64(env, a.v[5], &k) || !get_f64(env, a.v[6], &alpha) ||
+      !get_ptr(env, a.v[7], &A) || !get_i64(env, a.v[8], &lda) || !get_ptr(env, a.v[9], &B) ||
+      !get_i64(env, a.v[10], &ldb) || !get_ptr(env, a.v[11], &off) || !get_f64(env, a.v[12], &beta) ||
+      !get_ptr(env, a.v[13], &C) || !get_i64(env, a.v[14], &ldc) || !get_i64(env, a.v[15], &strideC) ||
+      !get_i32(env, a.v[16], &ctype))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_gemm_grouped_k(ctx, type, groups, m, n, k, (float)alpha, A, lda, B, ldb, (const int64_t *)off,
+                                     (float)beta, C, ldc, strideC, ctype), "wgb_gemm_grouped_k");
+  return nullptr;
+}
+
+// mxfp4Quantize(ctx, type, trans, k, n, X, ldx, codes, scales, ld)
+napi_value Mxfp4Quantize(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 10)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, trans;
+  int64_t k, n, ldx, ld;
+  void *X, *codes, *scales;
+  if (!get_i32(env, a.v[1], &type) || !get_i32(env, a.v[2], &trans) || !get_i64(env, a.v[3], &k) ||
+      !get_i64(env, a.v[4], &n) || !get_ptr(env, a.v[5], &X) || !get_i64(env, a.v[6], &ldx) ||
+      !get_ptr(env, a.v[7], &codes) || !get_ptr(env, a.v[8], &scales) || !get_i64(env, a.v[9], &ld))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_mxfp4_quantize(ctx, type, trans, k, n, X, ldx, (uint8_t *)codes, (uint8_t *)scales, ld),
+                  "wgb_mxfp4_quantize");
+  return nullptr;
+}
+
+// mxfp4Dequantize(ctx, type, k, n, codes, scales, ld, X, ldx)
+napi_value Mxfp4Dequantize(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 9)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type;
+  int64_t k, n, ldx, ld;
+  void *X, *codes, *scales;
+  if (!get_i32(env, a.v[1], &type) || !get_i64(env, a.v[2], &k) || !get_i64(env, a.v[3], &n) ||
+      !get_ptr(env, a.v[4], &codes) || !get_ptr(env, a.v[5], &scales) || !get_i64(env, a.v[6], &ld) ||
+      !get_ptr(env, a.v[7], &X) || !get_i64(env, a.v[8], &ldx))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_mxfp4_dequantize(ctx, type, k, n, (const uint8_t *)codes, (const uint8_t *)scales, ld, X, ldx),
+                  "wgb_mxfp4_dequantize");
+  return nullptr;
+}
+
+// mxfp4Gemm(ctx, groups (-1: one matrix), m, n, k, alpha, A, scaleA, lda,
+// strideA, B, scaleB, ldb, offsets, beta, C, ldc, ctype)
+napi_value Mxfp4Gemm(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 18)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int ctype;
+  int64_t groups, m, n, k, lda, strideA, ldb, ldc;
+  double alpha, beta;
+  void *A, *sA, *B, *sB, *off, *C;
+  if (!get_i64(env, a.v[1], &groups) || !get_i64(env, a.v[2], &m) || !get_i64(env, a.v[3], &n) ||
+      !get_i64(env, a.v[4], &k) || !get_f64(env, a.v[5], &alpha) || !get_ptr(env, a.v[6], &A) ||
+      !get_ptr(env, a.v[7], &sA) || !get_i64(env, a.v[8], &lda) || !get_i64(env, a.v[9], &strideA) ||
+      !get_ptr(env, a.v[10], &B) || !get_ptr(env, a.v[11], &sB) || !get_i64(env, a.v[12], &ldb) ||
+      !get_ptr(env, a.v[13], &off) || !get_f64(env, a.v[14], &beta) || !get_ptr(env, a.v[15], &C) ||
+      !get_i64(env, a.v[16], &ldc) || !get_i32(env, a.v[17], &ctype))
+    return nullptr;
+  const uint8_t *a4 = (const uint8_t *)A, *as = (const uint8_t *)sA, *b4 = (const uint8_t *)B, *bs = (const uint8_t *)sB;
+  if (groups < 0)
+    WGB_OK_OR_THROW(wgb_mxfp4_gemm(ctx, m, n, k, (float)alpha, a4, as, lda, b4, bs, ldb, (float)beta, C, ldc, ctype),
+                    "wgb_mxfp4_gemm");
+  else
+    WGB_OK_OR_THROW(wgb_mxfp4_gemm_grouped(ctx, groups, m, n, k, (float)alpha, a4, as, lda, strideA, b4, bs, ldb,
+                                           (const int64_t *)off, (float)beta, C, ldc, ctype), "wgb_mxfp4_gemm_grouped");
+  return nullptr;
+}
+
 napi_value ModuleInit(napi_env env, napi_value exports) {
   if (wgb_abi_version() != WGB_ABI_VERSION) {
     std::string msg = "wgblas_hip addon: libwgblas_hip implements C ABI version " +
@@ -636,6 +748,8 @@ napi_value ModuleInit(napi_env env, napi_value exports) {
       {"upload", Upload}, {"download", Download}, {"gemm", Gemm},
       {"ssyrk", Ssyrk}, {"ssyr2k", Ssyr2k}, {"ssymm", Ssymm},
       {"tri", Tri}, {"sgemv", Sgemv}, {"ger", Ger}, {"syr", Syr}, {"symv", Symv}, {"trmv", Trmv}, {"reduce", Reduce},
+      {"gemmGrouped", GemmGrouped}, {"gemmGroupedK", GemmGroupedK}, {"mxfp4Quantize", Mxfp4Quantize},
+      {"mxfp4Dequantize", Mxfp4Dequantize}, {"mxfp4Gemm", Mxfp4Gemm},
   };
   for (const Fn &f : fns) {
     napi_value v;
