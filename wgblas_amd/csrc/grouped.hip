@@ -104,8 +104,9 @@ int align_operands(wgb_ctx *ctx, Args &p, double now, double then, int64_t a_row
                 bytes_b = move_b ? b_cols * b_chunks * 16 : 0;
   if (a_chunks * 16 >= (int64_t)1 << 22 || b_chunks * 16 >= (int64_t)1 << 22) return WGB_OK;
   if (then + 2.0 * (double)(bytes_a + bytes_b) / 4.5e6 + 3.0 >= now) return WGB_OK;
-  const int st = wgb::ensure_op_workspace(ctx, (size_t)(bytes_a + bytes_b));
+  const int st = wgb::ensure_op_workspace(ctx, (size_t)(bytes_a + bytes_b) + parts_bytes(ctx));
   if (st) return st;
+  p.parts = (float *)((char *)ctx->op_ws + bytes_a + bytes_b);
   auto move = [&](const char *X, int64_t ld, int64_t stride, int64_t cols, int64_t total, int64_t rows, int64_t chunks,
                   char *Y) {
     const int64_t want = (total * chunks + 255) / 256, most = (int64_t)ctx->num_cus * 32;

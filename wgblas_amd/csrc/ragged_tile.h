@@ -130,6 +130,8 @@ struct Args {
   // CUs of a persistent launch of 256 x 256 tiles, which leaves a last round
   // that would use at most half of them to 128 x 128 tiles; 0: no such launch
   int round;
+  int pieces;     // of k that a tile of that rest is cut into at most, each a block's; their sums go to
+  float *parts;   // this array, 128 x 128 a block
   int stream;  // C's columns start at 64-byte boundaries: large results bypass the caches
   int c_f32;   // C holds fp32 (else the operands' type; fp4: bf16, or f16 with c_f16)
   int c_f16;
@@ -349,6 +351,29 @@ __device__ __forceinline__ int whole_rounds(const Args &p, int total) {
   const int cut = total / p.round * p.round;
   return total - cut > p.round / 2 ? total : cut;
 }
+
+// A quarter (128 x 128) of a tile that the persistent launch left, by a block
+// of the launch for those: false if there is none. Few quarters are cut along
+// k, as many pieces as keep all blocks at once on the GPU: 60 of them at k =
+// 4096, one a CU, take 65 us whole, for a CU's copies are the limit there.
+struct Quarter {
+  int at, piece, pieces;
+
+  template <class Order>
+  __device__ __forceinline__ bool find(const Args &p, Order &order, int block, bool fold, Tile &t) {
+    order.init(p, 256);
+    const int whole = whole_rounds(p, order.total), left = order.total - whole;
+    if (left <= 0) return false;
+    pieces = p.round / (2 * left);
+    pieces = pieces > p.pieces ? p.pieces : pieces < 1 ? 1 : pieces;
+    at = fold ? block : block / pieces;
+    piece = fold ? 0 : block - at * pieces;
+    if (at >= 4 * left || !order.find(p, whole + at / 4, t)) return false;
+    t.tm = 2 * t.tm + (at & 1);
+    t.tn = 2 * t.tn + ((at >> 1) & 1);
+    return true;
+  }
+};
 
 // A persistent block's tiles, one a lane: all of them are found at the start.
 constexpr int kTilesPerBlock = 64;
@@ -829,7 +854,12 @@ __device__ __forceinline__ void store_tile(const Args &p, int64_t at, const f4 (
 // through registers. RK: ragged k. S: stages of LDS.
 template <class E, int BM, int BN, int WM, int WN, bool AMC, bool BMC, bool VEC, bool RK, int S>
 struct Kernel {
-  static constexpr int kBM = BM, kBN = BN;
+  typedef E Element;
+  typedef typename std::conditional<RK, KOrder, ColumnOrder>::type Order;
+  static constexpr int kBM = BM, kBN = BN, kWM = WM, kWN = WN;
+  static constexpr bool kRK = RK;
+  // computes what a launch of 256 x 256 tiles leaves, too
+  static constexpr bool REST = BM == 128 && BN == 128 && VEC && E::kBits != 32;
   static constexpr int NW = WM * WN, NT = 64 * NW;
   static constexpr int MB = BM / WM / 16, NB = BN / WN / 16;
   static constexpr bool kScaled = E::kBits == 4;
@@ -845,13 +875,10 @@ struct Kernel {
   static __device__ __forceinline__ void run(const Args &p, char *smem) {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     Tile tile;
-    typename std::conditional<RK, KOrder, ColumnOrder>::type order;
-    if (BM == 128 && BN == 128 && p.round) {
-      // a quarter of a 256 x 256 tile that the persistent launch left
-      order.init(p, 256);
-      if (!order.find(p, whole_rounds(p, order.total) + blockIdx.x / 4, tile)) return;
-      tile.tm = 2 * tile.tm + (blockIdx.x & 1);
-      tile.tn = 2 * tile.tn + ((blockIdx.x >> 1) & 1);
+    Order order;
+    Quarter quarter = {0, 0, 1};
+    if (REST && p.round) {
+      if (!quarter.find(p, order, blockIdx.x, false, tile)) return;
     } else {
       order.init(p, BN);
       if (!order.find(p, blockIdx.x, tile)) return;
@@ -869,7 +896,14 @@ struct Kernel {
 #pragma unroll
       for (int j = 0; j < NB; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int nt = (int)((K + SA::BK - 1) / SA::BK);
+    int nt = (int)((K + SA::BK - 1) / SA::BK), first = 0;
+    if (REST && quarter.pieces > 1) {
+      const int most = (nt + quarter.pieces - 1) / quarter.pieces;
+      first = quarter.piece * most;
+      nt = nt - first < most ? nt - first : most;
+      K -= (int64_t)first * SA::BK;
+      if (K > (int64_t)most * SA::BK) K = (int64_t)most * SA::BK;
+    }
     if (nt > 0) {
       SA sa;
       SB sb;
@@ -878,10 +912,14 @@ struct Kernel {
       const char *B = RK ? p.B + tile.lo * p.ldb : p.B + tile.lo * p.ldb;
       sa.init(A, p.lda, m0, p.m, K, t);
       sb.init(B, p.ldb, n0, cols, K, t);
+      if constexpr (REST) {
+        sa.origin += first * sa.step();
+        sb.origin += first * sb.step();
+      }
       if constexpr (kScaled) {
         const int64_t lsa = p.lda / 16, lsb = p.ldb / 16;
-        ss.init(p.scale_a + (int64_t)tile.g * (p.stride_a / 16) + m0 * lsa, lsa, p.m - m0,
-                p.scale_b + (tile.lo + n0) * lsb, lsb, cols - n0, K, wave, lane);
+        ss.init(p.scale_a + (int64_t)tile.g * (p.stride_a / 16) + m0 * lsa + first * SS::RB, lsa, p.m - m0,
+                p.scale_b + (tile.lo + n0) * lsb + first * SS::RB, lsb, cols - n0, K, wave, lane);
       }
       int whole = 0;
       if constexpr (VEC) {
@@ -987,8 +1025,49 @@ struct Kernel {
       }
     }
 
+    if (REST && quarter.pieces > 1) {
+      f4 *part = reinterpret_cast<f4 *>(p.parts) + ((int64_t)blockIdx.x * NW + wave) * (MB * NB * 64) + lane;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) part[(j * MB + i) * 64] = acc[i][j];
+      return;
+    }
     const int64_t at = RK ? (int64_t)tile.g * p.stride_c : tile.lo * p.ldc;
     store_tile<E, 16>(p, at, acc, m0 + wm, n0 + wn, cols, lane);
+  }
+};
+
+// Adds up the pieces of quarters that were cut along k, in their order (the
+// result is the same every time): block 4 q + j column block j of each wave's
+// part of quarter q.
+template <class K>
+struct FoldKernel {
+  static constexpr int NT = K::NT, LDS = 0;
+
+  static __device__ __forceinline__ void run(const Args &p, char *) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Tile tile;
+    typename K::Order order;
+    Quarter quarter;
+    if (!quarter.find(p, order, blockIdx.x / K::NB, true, tile) || quarter.pieces == 1) return;
+    const int64_t m0 = (int64_t)tile.tm * K::kBM, n0 = (int64_t)tile.tn * K::kBN;
+    const int64_t cols = K::kRK ? p.n : tile.hi - tile.lo;
+    if (m0 >= p.m || n0 >= cols) return;
+    const int j = blockIdx.x % K::NB;
+    const f4 *part = reinterpret_cast<const f4 *>(p.parts) +
+                     (((int64_t)quarter.at * quarter.pieces * K::NW + wave) * K::NB + j) * (K::MB * 64) + lane;
+    f4 total[K::MB][1];
+#pragma unroll
+    for (int i = 0; i < K::MB; ++i) total[i][0] = part[i * 64];
+    for (int q = 1; q < quarter.pieces; ++q) {
+      part += K::NW * K::NB * K::MB * 64;
+#pragma unroll
+      for (int i = 0; i < K::MB; ++i) total[i][0] += part[i * 64];
+    }
+    const int wm = (wave % K::kWM) * (K::kBM / K::kWM), wn = (wave / K::kWM) * (K::kBN / K::kWN);
+    const int64_t at = K::kRK ? (int64_t)tile.g * p.stride_c : tile.lo * p.ldc;
+    store_tile<typename K::Element, 16>(p, at, total, m0 + wm, n0 + wn + 16 * j, cols, lane);
   }
 };
 
@@ -1478,33 +1557,54 @@ int launch_k(wgb_ctx *ctx, Args &p) {
   return launch<K>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
 }
 
+// Bytes of Args::parts: what the rest's blocks that run at once (two a CU) may hold.
+inline size_t parts_bytes(const wgb_ctx *ctx) { return (size_t)ctx->num_cus * 2 * 128 * 128 * 4; }
+
 // `Turn` on at most `tiles` 256 x 256 tiles, a block a CU (more where one
 // could not keep its tiles), then `Rest` (128 x 128 tiles, a quarter of one
-// each) on what that leaves. Which tiles there are is only known on the GPU.
+// each) on what that leaves, and if that was cut along k (at least 8 k-tiles a
+// piece, and 3 pieces, for the sums cost a launch), their sums. Which tiles
+// there are is only known on the GPU, unless `exact`. k: of a tile, to expect.
 template <class Turn, class Rest>
-int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles) {
+int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles, bool exact, int64_t k) {
   p.stream = ((uintptr_t)p.C & 63) == 0 && p.ldc * (p.c_f32 ? 4 : 2) % 64 == 0 && p.stride_c * (p.c_f32 ? 4 : 2) % 64 == 0;
   int64_t blocks = tiles;
   if (tiles > ctx->num_cus) {
     blocks = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
     if (blocks <= ctx->num_cus) blocks = p.round = ctx->num_cus;
   }
-  const int st = launch<Turn>(ctx, p, blocks);
-  if (st || !p.round) return st;
-  return launch<Rest>(ctx, p, (int64_t)(p.round / 2) * 4);
+  int64_t rest = p.round / 2;  // at most
+  if (p.round && exact) {
+    const int64_t over = tiles % p.round;
+    rest = over > rest ? 0 : over;
+  }
+  const int64_t pieces = k / (8 * Rest::SA::BK) < 8 ? k / (8 * Rest::SA::BK) : 8;
+  p.pieces = pieces < 3 ? 1 : (int)pieces;
+  if (rest && exact && p.round / (2 * rest) < 3) p.pieces = 1;
+  if (rest && p.pieces > 1 && !p.parts) {
+    const int st = wgb::ensure_op_workspace(ctx, parts_bytes(ctx));
+    if (st) return st;
+    p.parts = (float *)ctx->op_ws;
+  }
+  int st = launch<Turn>(ctx, p, blocks);
+  if (st || !rest) return st;
+  const int64_t slots = 2 * (int64_t)p.round;
+  st = launch<Rest>(ctx, p, p.pieces == 1 ? 4 * rest : slots);
+  if (st || p.pieces == 1) return st;
+  return launch<FoldKernel<Rest>>(ctx, p, (slots / 2 < 4 * rest ? slots / 2 : 4 * rest) * Rest::NB);
 }
 
 template <class Turn, class Rest>
 int launch_columns_rounds(wgb_ctx *ctx, Args &p) {
   p.tiles_m = (int)((p.m + Turn::kBM - 1) / Turn::kBM);
-  return launch_rounds<Turn, Rest>(ctx, p, most_columns(p, Turn::kBN) * p.tiles_m);
+  return launch_rounds<Turn, Rest>(ctx, p, most_columns(p, Turn::kBN) * p.tiles_m, !p.off, p.k);
 }
 
 template <class Turn, class Rest>
 int launch_k_rounds(wgb_ctx *ctx, Args &p) {
   p.tiles_m = (int)((p.m + Turn::kBM - 1) / Turn::kBM);
   p.tiles_n = (int)((p.n + Turn::kBN - 1) / Turn::kBN);
-  return launch_rounds<Turn, Rest>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
+  return launch_rounds<Turn, Rest>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups, true, p.k / p.groups);
 }
 
 // Estimated time of a launch of T x T tiles, to choose among sizes: `first` us
