@@ -43,7 +43,8 @@ int choose(wgb_ctx *ctx, const Args &p, bool vec, double k, double n64, double n
   const double t128 = small_time(128, cost_of(128), per_cu(ctx, p, 128, n128), k, size);
   time = t128 <= t64 ? t128 : t64;
   if (vec && E::kBits == 16) {
-    const double t256 = rounds_time(cost_of(256), cost_of(128), per_cu(ctx, p, 256, n256), k, size);
+    const double t256 = rounds_time(cost_of(256), cost_of(128), per_cu(ctx, p, 256, n256), k, size,
+                                    most_pieces((int64_t)k, 64));
     if (t256 <= time) {
       time = t256;
       return 256;

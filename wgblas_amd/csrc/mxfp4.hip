@@ -382,7 +382,7 @@ int product(wgb_ctx *ctx, Args &p) {
   const TileCost c64 = {4.0, 1.5}, c128 = {5.6, 3.3}, c256 = {10.5, 10.5};
   const double t64 = small_time(64, c64, per_cu(ctx, p, 64, expected_columns(p, 64)), k, size);
   const double t128 = small_time(128, c128, per_cu(ctx, p, 128, expected_columns(p, 128)), k, size);
-  const double t256 = rounds_time(c256, c128, per_cu(ctx, p, 256, expected_columns(p, 256)), k, size);
+  const double t256 = rounds_time(c256, c128, per_cu(ctx, p, 256, expected_columns(p, 256)), k, size, most_pieces(p.k, 256));
   if (t256 <= t128 && t256 <= t64)
     return launch_columns_rounds<TurnKernel<Fp4, false, false, false>, Kernel<Fp4, 128, 128, 2, 2, false, false, true, false, 2>>(ctx, p);
   if (t128 <= t64) return launch_columns<Kernel<Fp4, 128, 128, 2, 2, false, false, true, false, 2>>(ctx, p);

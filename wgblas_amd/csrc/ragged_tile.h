@@ -1557,14 +1557,20 @@ int launch_k(wgb_ctx *ctx, Args &p) {
   return launch<K>(ctx, p, (int64_t)p.tiles_m * p.tiles_n * p.groups);
 }
 
+// Pieces that k elements are cut into at most: at least 8 k-tiles (of bk) each,
+// and 3 of them, for their sums cost a launch.
+inline int most_pieces(int64_t k, int bk) {
+  const int64_t pieces = k / (8 * bk);
+  return pieces < 3 ? 1 : pieces < 8 ? (int)pieces : 8;
+}
 // Bytes of Args::parts: what the rest's blocks that run at once (two a CU) may hold.
 inline size_t parts_bytes(const wgb_ctx *ctx) { return (size_t)ctx->num_cus * 2 * 128 * 128 * 4; }
 
 // `Turn` on at most `tiles` 256 x 256 tiles, a block a CU (more where one
 // could not keep its tiles), then `Rest` (128 x 128 tiles, a quarter of one
-// each) on what that leaves, and if that was cut along k (at least 8 k-tiles a
-// piece, and 3 pieces, for the sums cost a launch), their sums. Which tiles
-// there are is only known on the GPU, unless `exact`. k: of a tile, to expect.
+// each) on what that leaves, and if that may be cut along k, their sums. Which
+// tiles there are is only known on the GPU, unless `exact`. k: of a tile, to
+// expect.
 template <class Turn, class Rest>
 int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles, bool exact, int64_t k) {
   p.stream = ((uintptr_t)p.C & 63) == 0 && p.ldc * (p.c_f32 ? 4 : 2) % 64 == 0 && p.stride_c * (p.c_f32 ? 4 : 2) % 64 == 0;
@@ -1578,8 +1584,7 @@ int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles, bool exact, int64_t k) {
     const int64_t over = tiles % p.round;
     rest = over > rest ? 0 : over;
   }
-  const int64_t pieces = k / (8 * Rest::SA::BK) < 8 ? k / (8 * Rest::SA::BK) : 8;
-  p.pieces = pieces < 3 ? 1 : (int)pieces;
+  p.pieces = most_pieces(k, Rest::SA::BK);
   if (rest && exact && p.round / (2 * rest) < 3) p.pieces = 1;
   if (rest && p.pieces > 1 && !p.parts) {
     const int st = wgb::ensure_op_workspace(ctx, parts_bytes(ctx));
@@ -1626,11 +1631,17 @@ inline double small_time(int T, TileCost c, double tiles, double k, double c_siz
   const double store = T * T * c_size / 17.6e3, depth = k / 1024;
   return c.first * depth + store + (tiles > 1 ? tiles - 1 : 0) * (c.next * depth + store);
 }
-// 256 x 256 tiles: whole rounds, then the rest as launch_rounds has it.
-inline double rounds_time(TileCost c256, TileCost c128, double tiles, double k, double c_size) {
+// 256 x 256 tiles: whole rounds, then the rest as launch_rounds has it (cut
+// along k, a piece more than fills its share: 60 quarters at k = 4096 in 16
+// bits 30 us and 8 for the sums).
+inline double rounds_time(TileCost c256, TileCost c128, double tiles, double k, double c_size, int most) {
   const double store = 256 * 256 * c_size / 17.6e3, round = c256.first * (k / 1024) + store;
   const double whole = (double)(int64_t)tiles, rest = tiles - whole;
   if (rest < 0.01) return whole * round;
+  if (whole > 0 && rest <= 0.17 && most > 1) {
+    const double pieces = 0.5 / rest < most ? 0.5 / rest : most;
+    return whole * round + (c128.first + c128.next) * (k / 1024) / pieces + 15;
+  }
   return whole * round + (rest > 0.5 || whole == 0 ? round : small_time(128, c128, 4 * rest, k, c_size) + 4);
 }
 inline double per_cu(const wgb_ctx *ctx, const Args &p, int T, double tiles_n) {
