@@ -769,7 +769,8 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t col = col0 + STEP * j + i16;
-    if (col >= cols) continue;
+    const bool in = col < cols;
+    if (!STREAM && !in) continue;
     T *cp = C + col * p.ldc;
     // a lane's four rows of row block i
     auto value = [&](int i) {
@@ -777,7 +778,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
       f4 x = acc[i][j];
 #pragma unroll
       for (int q = 0; q < 4; ++q) x[q] *= p.alpha;
-      if (p.beta != 0.0f) {
+      if (p.beta != 0.0f && in) {
         if (row + 4 <= rows) {
           const V4 c = *reinterpret_cast<const V4 *>(cp + row);
 #pragma unroll
@@ -793,7 +794,48 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
       for (int q = 0; q < 4; ++q) v[q] = (T)x[q];
       return v;
     };
-    if constexpr (PAIRS) {
+    if constexpr (STREAM) {
+      // two runs of 64 bytes of 16 columns become 128 bytes of 8 columns each:
+      // lanes 0 - 7 of 16 give the second run, lanes 8 - 15 the first
+      constexpr int ROWS = 16 / sizeof(T), BLOCKS = PAIRS ? 4 : 2;
+      typedef T Run __attribute__((ext_vector_type(ROWS), aligned(sizeof(T))));
+      const bool low = i16 < 8;
+#pragma unroll
+      for (int i = 0; i < MB; i += BLOCKS) {
+        v4i x[2], y[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (PAIRS) {
+            typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+            const u2 a = __builtin_bit_cast(u2, value(i + 2 * h)), b = __builtin_bit_cast(u2, value(i + 2 * h + 1));
+            x[h] = eight_rows(a[0], a[1], b[0], b[1]);
+          } else {
+            x[h] = __builtin_bit_cast(v4i, value(i + h));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int other = __builtin_amdgcn_mov_dpp(low ? x[1][c] : x[0][c], 0x128, 0xf, 0xf, true);  // lane ^ 8
+          y[0][c] = low ? x[0][c] : other;
+          y[1][c] = low ? other : x[1][c];
+        }
+        const int64_t row = row0 + 16 * i + (PAIRS ? 32 * (i16 >> 3) + 16 * (g & 1) + 8 * (g >> 1) : 16 * (i16 >> 3) + 4 * g);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t to = col0 + STEP * j + 8 * h + (i16 & 7);
+          if (to >= cols) continue;
+          T *at = C + to * p.ldc + row;
+          const Run v = __builtin_bit_cast(Run, y[h]);
+          if (row + ROWS <= rows) {
+            __builtin_nontemporal_store(v, reinterpret_cast<Run *>(at));
+          } else {
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+              if (row + q < rows) at[q] = v[q];
+          }
+        }
+      }
+    } else if constexpr (PAIRS) {
       typedef T V8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
       typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -802,10 +844,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
         const V8 v = __builtin_bit_cast(V8, eight_rows(x[0], x[1], y[0], y[1]));
         const int64_t row = row0 + 16 * (i + (g & 1)) + 8 * (g >> 1);
         if (row + 8 <= rows) {
-          if constexpr (STREAM)
-            __builtin_nontemporal_store(v, reinterpret_cast<V8 *>(cp + row));
-          else
-            *reinterpret_cast<V8 *>(cp + row) = v;
+          *reinterpret_cast<V8 *>(cp + row) = v;
         } else {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
@@ -818,10 +857,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
         const V4 v = value(i);
         const int64_t row = row0 + 16 * i + 4 * g;
         if (row + 4 <= rows) {
-          if constexpr (STREAM)
-            __builtin_nontemporal_store(v, reinterpret_cast<V4 *>(cp + row));
-          else
-            *reinterpret_cast<V4 *>(cp + row) = v;
+          *reinterpret_cast<V4 *>(cp + row) = v;
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
