@@ -1,7 +1,9 @@
 /*
  * wgblas_hip.h — C ABI of libwgblas_hip, the MI355X (gfx950) implementation
  * of wgblas's data-parallel hot path: the GEMM family (sgemm, sgemmtr, ssyrk,
- * dgemm) and the level-1 reductions (sdot, sasum, snrm2, isamax).
+ * dgemm) and the level-1 reductions (sdot, sasum, snrm2, isamax), and of the
+ * products of expert layers: grouped products in fp32, fp16 and bf16, and 4-bit
+ * (MXFP4) matrices with theirs.
  *
  * Every entry point takes plain pointers and sizes. Matrices are
  * COLUMN-MAJOR (element (i, j) of an ld-strided matrix sits at p[i + j*ld]);
@@ -292,8 +294,13 @@ int wgb_strsm(wgb_ctx *ctx, int side, int uplo, int transA, int diag,
  * outside the operands is touched. Operands are all of `type` (WGB_F32,
  * WGB_F16 or WGB_BF16), C of `ctype`: the same, or WGB_F32. Sums are held in
  * fp32 and rounded once, to nearest even. beta == 0 never reads C; alpha == 0
- * reads neither A nor B. Results are reproducible run to run. No counterpart
- * in the reference, which has no grouped routine. */
+ * reads neither A nor B. Results are reproducible run to run. C must not
+ * overlap A or B. 16-bit and MXFP4 products of many tiles, and 16-bit ones at
+ * odd leading dimensions, use the context's workspace (32 MiB for sums, copies
+ * of the operands at odd leading dimensions): calls of a context must not
+ * overlap, and a call that is to be captured into a graph has to have run
+ * once before, so that the workspace is there. No counterpart in the
+ * reference, which has no grouped routine. */
 
 /* C(:, j) <- alpha*op(A_g)*B(:, j) + beta*C(:, j) for the columns j of every
  * group g: B k-by-n and C m-by-n column-major, op(A_g) m-by-k with A_g at

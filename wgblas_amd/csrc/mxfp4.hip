@@ -138,7 +138,8 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 }
 
 // Blocks along the contiguous axis: a lane has 8 elements of a column, a quad
-// a block. Bound by memory: one pass, loads of 16 bytes a lane.
+// a block. Bound by memory: one pass, loads of 16 bytes a lane. 16384 columns of
+// 4096 bf16 values: 30 us, 5.6 TB/s; 17 columns: 2.5 us, a launch.
 template <class E>
 __global__ __launch_bounds__(256) void quantize_kernel(const typename E::store *X, int64_t ldx, int64_t k, int64_t n,
                                                        uint8_t *codes, uint8_t *scales, int64_t ld, int segs) {
@@ -184,7 +185,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename E::store *
 // block: 32 loads of two elements (256 contiguous bytes a wave for 16-bit
 // types). The eight waves have eight blocks in a row of the same 128 columns;
 // their codes go through LDS (16-byte chunks at chunk ^ column, no two lanes
-// of a quarter wave in the same banks) and out as 128-byte lines.
+// of a quarter wave in the same banks) and out as 128-byte lines. Bound by
+// memory: 8192 x 16384 in bf16 93 us, 3.8 TB/s (the two-element loads keep
+// fewer bytes in flight than the 16-byte ones above).
 template <class E>
 __global__ __launch_bounds__(512) void quantize_strided_kernel(const typename E::store *X, int64_t ldx, int64_t k,
                                                                int64_t n, uint8_t *codes, uint8_t *scales, int64_t ld,
@@ -271,7 +274,8 @@ __global__ __launch_bounds__(512) void quantize_strided_kernel(const typename E:
 }
 
 // A lane has 8 codes of a column: value * scale in fp32 (both exact), rounded
-// once to the output's type.
+// once to the output's type. Bound by memory: 8192 x 16384 to bf16 64 us, 5.2
+// TB/s.
 template <class E>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t *codes, const uint8_t *scales, int64_t ld,
                                                          int64_t k, int64_t n, typename E::store *X, int64_t ldx,

@@ -754,12 +754,15 @@ __device__ __forceinline__ v4i eight_rows(uint32_t x0, uint32_t x1, uint32_t y0,
 }
 
 // alpha acc + beta C for a lane's runs of four rows of one column; column
-// blocks are STEP columns apart. STREAM: non-temporal stores, for results too
-// large for the caches (8192 x 16384 in bf16 773 -> 760 us, 8 x 4096 x 2048 in
-// fp32 195 -> 184 us; 12 x 1032 x 520 in f16, which fits, 16.7 -> 21 us) and whose
-// columns do not cut lines (12872 columns of 2249 fp32 values 109 -> 168 us). fp32 is stored in those runs (16 bytes a
+// blocks are STEP columns apart. fp32 is stored in those runs (16 bytes a
 // lane), 16-bit values in runs of eight rows (also 16 bytes) where there are
-// two row blocks: with 8 bytes a lane 8192 x 16384 x 4096 took 788 us.
+// two row blocks: with 8 bytes a lane 8192 x 16384 x 4096 took 4% longer.
+// STREAM: non-temporal stores, for results too large for the caches (12 x 1032
+// x 520 in f16, which fits, 16.7 -> 21 us) and whose columns do not cut lines
+// (12872 columns of 2249 fp32 values 109 -> 168 us), in whole lines: as runs
+// of 64 bytes, weight gradients of 8 x 4096 x 2048 in fp32 wrote 399 MB for the
+// 268 of C and took 195 us instead of 175, forward products of 16384 columns of
+// 8192 bf16 values 1020 instead of 983.
 template <typename T, int MB, int NB, int STEP, bool STREAM>
 __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB][NB], int64_t row0, int64_t rows,
                                          int64_t col0, int64_t cols, int lane) {
@@ -884,7 +887,12 @@ __device__ __forceinline__ void store_tile(const Args &p, int64_t at, const f4 (
   }
 }
 
-// One BM x BN tile of C a block, WM x WN waves. AMC / BMC: the operand is
+// One BM x BN tile of C a block, WM x WN waves: what the larger tiles would
+// leave CUs idle for. Bound by the copies into LDS, about 40 bytes a cycle and
+// CU (bf16 4096^3 on 128 x 128 tiles 1.0 PFLOP/s), and with few columns (128 x
+// 32 tiles) by reading A (64 experts of 2048 x 1024 in bf16, 64 columns: 27 us,
+// 6.4 TB/s); in fp32 by the matrix cores (64 x 64 tiles: 1000 x 1537 x 777 in 5
+// groups 31 us, 77 TFLOP/s, their last round half empty). AMC / BMC: the operand is
 // row-contiguous in memory. VEC: both operands can be copied by 16-byte
 // (4-byte aligned) loads at 32-bit offsets; otherwise every k-tile goes
 // through registers. RK: ragged k. S: stages of LDS.
@@ -1126,6 +1134,11 @@ struct FoldKernel {
 // A k + 2 in "multiply 0" of k; three or four slots before they are read. fp4
 // also keeps scales and has four units: waves 0 - 3 copy all of k + 1 in
 // "multiply 0" of k, waves 4 - 7 in "multiply 1" of k - 1.
+// 16-bit is bound by the matrix cores and the power that they draw: 8192^3 in
+// bf16 735 us, 1.5 PFLOP/s; 16 groups of 1024 columns 8192 x 16384 x 4096 in
+// 830 us (A is read once for each group) and ragged ones in 980. fp4 is bound by
+// the copies and reads of its slots, whose MFMAs take half as long: 8192^3 302
+// us, 3.6 PFLOP/s.
 template <class E, bool AMC, bool BMC, bool RK>
 struct TurnKernel {
   static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
@@ -1400,7 +1413,9 @@ struct TurnKernel {
 // R row blocks and CB column blocks of 16; its eight waves share k in runs of
 // 256 bytes, load both operands straight into MFMA operand registers, the next
 // run ahead of the present one's MFMAs, and add their sums in LDS in the
-// waves' order. A k-contiguous only. The loads take any alignment.
+// waves' order. A k-contiguous only. The loads take any alignment. One column
+// of 8192 x 4096 fp4 weights: 5.8 us, 3.1 TB/s of the 18 MB (a launch alone
+// is 2 us).
 template <class E, int R, int CB>
 struct SkinnyKernel {
   static constexpr int kBM = 16 * R, kBN = 16 * CB;
