@@ -298,3 +298,17 @@ def test_refusals(ctx):
     gemm(m=0, A=None, sA=None, B=None, sB=None, C=None)
     grouped(groups=0, A=None, sA=None, B=None, sB=None, C=None, off=None)
     ctx.synchronize()
+
+
+@pytest.mark.parametrize("k", [(1 << 23) + 1, 1 << 31, (1 << 63) - 100, (1 << 63) - 1])
+def test_refuses_k_too_large_to_round_up(ctx, k):
+    d = ctx.upload(np.zeros(1 << 10, np.uint8))
+    o = ctx.upload(np.array([0, 1], np.int64))
+    ld = 1 << 23
+    for call in (lambda: ctx.mxfp4_quantize(R.TYPES["f32"], TRANS, k, 1, d, 1, d, d, ld),
+                 lambda: ctx.mxfp4_quantize(R.TYPES["f32"], NO_TRANS, k, 1, d, k, d, d, ld),
+                 lambda: ctx.mxfp4_dequantize(R.TYPES["f32"], k, 1, d, d, ld, d, k),
+                 lambda: ctx.mxfp4_gemm(1, 1, k, 1.0, d, d, ld, d, d, ld, 0.0, d, 1, R.TYPES["f32"]),
+                 lambda: ctx.mxfp4_gemm_grouped(1, 1, 1, k, 1.0, d, d, ld, ld, d, d, ld, o, 0.0, d, 1, R.TYPES["f32"])):
+        with pytest.raises(WgblasError, match="status -1"):
+            call()

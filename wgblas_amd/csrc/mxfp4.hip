@@ -352,7 +352,8 @@ int dequantize(wgb_ctx *ctx, int64_t k, int64_t n, const uint8_t *codes, const u
 }
 
 int check_packed(const char *what, int64_t k, const void *codes, const void *scales, int64_t ld, bool needed) {
-  if (ld < runs128(k > 1 ? k : 1) || ld % 128 != 0 || ld > ((int64_t)1 << 23))
+  // against k itself, which may be too large to be rounded up
+  if (ld <= 0 || ld < k || ld % 128 != 0 || ld > ((int64_t)1 << 23))
     return fail(WGB_ERR_INVALID_VALUE,
                 std::string("the leading dimension of ") + what + " must be a multiple of 128, at least k, at most 2^23");
   if (!needed) return WGB_OK;
