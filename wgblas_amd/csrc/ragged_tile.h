@@ -1135,7 +1135,7 @@ struct FoldKernel {
 // also keeps scales and has four units: waves 0 - 3 copy all of k + 1 in
 // "multiply 0" of k, waves 4 - 7 in "multiply 1" of k - 1.
 // 16-bit is bound by the matrix cores and the power that they draw: 8192^3 in
-// bf16 735 us, 1.5 PFLOP/s; 16 groups of 1024 columns 8192 x 16384 x 4096 in
+// bf16 735 to 745 us, 1.5 PFLOP/s; 16 groups of 1024 columns 8192 x 16384 x 4096 in
 // 830 us (A is read once for each group) and ragged ones in 980. fp4 is bound by
 // the copies and reads of its slots, whose MFMAs take half as long: 8192^3 302
 // us, 3.6 PFLOP/s.
