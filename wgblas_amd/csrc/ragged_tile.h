@@ -30,6 +30,7 @@
 #pragma once
 
 #include "common.h"
+#include "copy_plan.h"
 #include "tile_order.h"
 
 #include <type_traits>
@@ -435,136 +436,33 @@ __device__ __forceinline__ void copy_chunks(const char *from, uint32_t at, char 
   copy16_to_lds(scalar_at(from, at), lds);
 }
 
-// Chunk keys of the row-contiguous layout, for k-row r of a tile whose rows
-// have `chunks` chunks: 16-bit transposing reads touch k-rows 8 g .. 8 g + 3
-// (32 bytes of each), fp32 reads k-rows 4 g (64 bytes of each).
-template <int BITS, int CHUNKS>
-__device__ __forceinline__ int mc_key(int r) {
-  const int key = BITS == 16 ? ((r & 3) << 1) | (((r >> 3) & 1) << 3) : ((r >> 2) & 3) << 2;
-  return key & (CHUNKS - 1);
-}
-
-// k-tiles are 128 bytes of k: a whole cache line of every row. (Of 64 bytes,
-// each line came from L2 twice, once for either half: 8192 x 16384 x 4096 in
-// bf16 886 us, of which 180 were the copies'.)
-constexpr int TB = 128;
-
-template <int LOADS>
-struct StagerData {
-  const char *origin;    // element (row0, k = 0)
-  int64_t ld;            // bytes
-  int64_t rows_left;     // rows from row0 to the end of the matrix
-  int64_t K;             // elements
-  uint32_t voff[LOADS];  // this lane's chunks of k-tile 0, in bytes from origin
-  int t;
-};
-
 template <class E, int BT, bool MC, int NT>
-struct Stager : StagerData<BT * TB / 16 / NT> {
-  static constexpr int EPC = 128 / E::kBits;         // elements in a 16-byte chunk
-  static constexpr int BK = TB * 8 / E::kBits;       // elements of k in a k-tile
-  static constexpr int BYTES = BT * TB;              // of a staged tile
-  static constexpr int LOADS = BYTES / 16 / NT;      // chunks a thread stages
-  static constexpr int CPR = MC ? BT / EPC : TB / 16;  // chunks in a staged row
-  static constexpr int RPS = NT / CPR;               // staged rows in one step of all threads
-  static_assert(BYTES % (16 * NT) == 0 && NT % CPR == 0, "whole steps");
-
-  typedef StagerData<LOADS> Data;
-  using Data::origin;
-  using Data::ld;
-  using Data::rows_left;
-  using Data::K;
-  using Data::voff;
-  using Data::t;
-
-  __device__ __forceinline__ int slot_row(int r) const { return t / CPR + r * RPS; }
-  __device__ __forceinline__ int slot_chunk(int r) const {
-    const int row = slot_row(r);
-    return (t % CPR) ^ (MC ? mc_key<E::kBits, CPR>(row) : row & 7);
-  }
-
-  __device__ __forceinline__ void init(const char *P, int64_t ld_, int64_t row0, int64_t rows, int64_t K_, int t_) {
-    t = t_;
-    ld = ld_;
-    rows_left = rows - row0;
-    K = K_;
-    origin = MC ? P + row0 * E::kBits / 8 : P + row0 * ld;
-#pragma unroll
-    for (int r = 0; r < LOADS; ++r) {
-      int row = slot_row(r), chunk = slot_chunk(r);
-      // lanes past the matrix read its last row (last chunk of rows): what
-      // they read only reaches elements of C that are never written
-      if (MC) {
-        const int64_t last = (rows_left - 1) / EPC;
-        if (chunk > last) chunk = (int)last;
-      } else if (row >= rows_left) {
-        row = (int)(rows_left - 1);
-      }
-      voff[r] = (uint32_t)(row * ld + chunk * 16);
-    }
-  }
-
-  // k-tiles whose copies stay inside the matrix: in the row-contiguous layout
-  // a last chunk that the end of the rows cuts reads on into the next k-row,
-  // which the last one does not have.
-  __device__ __forceinline__ int whole_tiles() const {
-    const bool cut = MC && rows_left < BT;
-    return (int)((cut ? (K > 0 ? K - 1 : 0) : K) / BK);
-  }
-
-  // Bytes from one k-tile to the next.
-  __device__ __forceinline__ int64_t step() const { return MC ? BK * ld : TB; }
+struct Stager : CopyPlan<E::kBits, BT, MC, NT> {
+  typedef CopyPlan<E::kBits, BT, MC, NT> Plan;
+  using Plan::CPR;
+  using Plan::EPC;
+  using Plan::LOADS;
+  using Plan::origin;
+  using Plan::voff;
+  using Plan::t;
 
   // k-tile kt.
   __device__ __forceinline__ void copy(char *stage, int kt, int wave) const {
-    const char *from = origin + (int64_t)kt * step();
+    const char *from = origin + (int64_t)kt * this->step();
 #pragma unroll
     for (int r = 0; r < LOADS; ++r) copy_chunks(from, voff[r], stage + wave * 1024 + r * NT * 16);
-  }
-
-  // A last k-tile that K cuts can be copied too, chunks past K reading one
-  // that exists: whoever reads the operands then clears what is past K
-  // (tail_mask). Not where a cut chunk could reach past the matrix: at its
-  // last row (k-contiguous), or with cut rows (row-contiguous).
-  __device__ __forceinline__ bool soft_tail() const {
-    return MC ? rows_left >= BT : K % EPC == 0 || (rows_left > BT && K >= EPC);
-  }
-  __device__ __forceinline__ uint32_t tail_voff(int r) const {
-    const int left = (int)(K % BK);
-    if (MC) return voff[r] - (slot_row(r) < left ? 0u : (uint32_t)(slot_row(r) * ld));
-    return voff[r] - (slot_chunk(r) * EPC < left ? 0u : (uint32_t)(slot_chunk(r) * 16));
-  }
-
-  // fp4, a last k-tile of which only the first 64 bytes exist: the other four
-  // chunks of a row read those again. What they hold does not matter (a code
-  // is never Inf or NaN), for their scales are staged as 2^-127 in both
-  // operands, and 36 * 2^-254 is nothing in fp32.
-  __device__ __forceinline__ uint32_t half_voff(int r) const {
-    return voff[r] - (slot_chunk(r) >= 4 ? 64u : 0u);
   }
 
   // Chunk r of k-tile kt through registers: rows past the matrix and k past
   // K read as zeros, at any alignment of the elements.
   __device__ __forceinline__ v4i load_guarded(int kt, int r) const {
     typedef typename E::chunk v4u;  // 16 bytes at the elements' alignment
-    const int row = slot_row(r), chunk = slot_chunk(r);
-    int64_t left, at;
-    bool in;
-    if (MC) {
-      const int64_t kk = (int64_t)kt * BK + row;
-      in = kk < K;
-      left = rows_left - (int64_t)chunk * EPC;
-      at = kk * ld + chunk * 16;
-    } else {
-      const int64_t kk = (int64_t)kt * BK + (int64_t)chunk * EPC;
-      in = row < rows_left;
-      left = K - kk;
-      at = row * ld + (int64_t)kt * TB + chunk * 16;
-    }
+    int64_t at;
+    const int64_t left = this->guarded(kt, r, at);
     v4i v = {0, 0, 0, 0};
-    if (in && left >= EPC) {
+    if (left >= EPC) {
       v = *reinterpret_cast<const v4u *>(origin + at);
-    } else if (in && left > 0) {
+    } else if (left > 0) {
       if constexpr (E::kBits == 16) {
         typedef short s8 __attribute__((ext_vector_type(8)));
         s8 s = {0, 0, 0, 0, 0, 0, 0, 0};
