@@ -1,0 +1,71 @@
+// host_runtime.cc with more of a machine behind it, for the host side of the
+// grouped and 4-bit products: two devices, memory that can run out, frees,
+// kernel attributes and the kernels' argument blocks in the list of calls.
+#include <hip/hip_runtime_api.h>
+
+#define hipMalloc standin_base_malloc
+#define hipFree standin_base_free
+#define hipLaunchKernel standin_base_launch
+#define hipGetDeviceCount standin_base_count
+#define hipSetDevice standin_base_set_device
+#include "host_runtime.cc"
+#undef hipMalloc
+#undef hipFree
+#undef hipLaunchKernel
+#undef hipGetDeviceCount
+#undef hipSetDevice
+
+namespace {
+size_t g_limit = ~(size_t)0;  // the largest allocation that there is memory for
+int g_device = 0;
+bool g_attributes = true;  // whether kernel attributes can be set
+int g_arguments = 0;       // bytes of the product kernels' arguments that a launch's line gives, in hexadecimal
+}  // namespace
+
+extern "C" {
+
+void standin_memory(size_t largest) { g_limit = largest; }
+void standin_attributes(int work) { g_attributes = work != 0; }
+void standin_arguments(int bytes) { g_arguments = bytes; }
+
+hipError_t hipMalloc(void **ptr, size_t bytes) {
+  if (bytes > g_limit) {
+    note("out_of_memory %zu", bytes);
+    return hipErrorOutOfMemory;
+  }
+  const hipError_t e = standin_base_malloc(ptr, bytes);
+  note("at %zx", (size_t)*ptr);
+  return e;
+}
+hipError_t hipFree(void *ptr) {
+  note("free %zx", (size_t)ptr);
+  return hipSuccess;
+}
+hipError_t hipLaunchKernel(const void *host, dim3 grid, dim3 block, void **args, size_t shared, hipStream_t stream) {
+  const hipError_t e = standin_base_launch(host, grid, block, args, shared, stream);
+  note("device %d shared %zu", g_device, shared);
+  if (g_arguments && g_kernels[host].find("ragged_kernel") != std::string::npos) {
+    g_log += "arguments ";
+    for (int i = 0; i < g_arguments; ++i) {
+      char hex[3];
+      std::snprintf(hex, sizeof(hex), "%02x", ((const unsigned char *)args[0])[i]);
+      g_log += hex;
+    }
+    g_log += '\n';
+  }
+  return e;
+}
+hipError_t hipFuncSetAttribute(const void *host, hipFuncAttribute, int value) {
+  note("attribute %d %d %s", g_device, value, g_kernels[host].c_str());
+  return g_attributes ? hipSuccess : hipErrorInvalidValue;
+}
+hipError_t hipGetDeviceCount(int *count) {
+  *count = 2;
+  return hipSuccess;
+}
+hipError_t hipSetDevice(int device) {
+  g_device = device;
+  return hipSuccess;
+}
+
+}  // extern "C"

@@ -1,0 +1,94 @@
+"""The host side of the grouped and 4-bit products without a GPU, through a
+stand-in for the HIP runtime (tests/native/ragged_runtime.cc) that runs no
+kernel and keeps a list of what was asked of it: the context's workspace."""
+import json
+import os
+import shutil
+import subprocess
+import sys
+
+import pytest
+
+from tests.test_host_side import PRELUDE
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+ROOT = os.path.dirname(HERE)
+
+CALLS = """
+from wgblas_amd import BF16, F16, F32, NO_TRANS, TRANS
+ctx = wg.Context(0)
+
+def columns(m, n, k, groups=1, t=BF16, trans=TRANS, pad=0, on=None, A=P):
+    lda = (k if trans == TRANS else m) + pad
+    (on or ctx).gemm_grouped(t, trans, groups, m, n, k, 1.0, A, lda, lda * (m if trans == TRANS else k), P + (1 << 30), k + pad,
+                             P, 0.0, P, m)
+
+def ragged_k(m, n, k, groups=1, t=BF16, pad=0, on=None):
+    (on or ctx).gemm_grouped_k(t, groups, m, n, k, 1.0, P, m + pad, P + (1 << 30), n + pad, P, 0.0, P, m, m * n, F32)
+
+def of(log, kind):
+    return [line.split()[1] for line in log if line.split()[0] == kind]
+"""
+
+
+@pytest.fixture(scope="module")
+def runtime(tmp_path_factory):
+    gxx, hipcc = shutil.which("g++"), shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc))), "include")
+    if gxx is None or not os.path.exists(os.path.join(include, "hip", "hip_runtime_api.h")):
+        pytest.skip("g++ or the HIP headers are not available")
+    so = str(tmp_path_factory.mktemp("runtime") / "ragged_runtime.so")
+    subprocess.run([gxx, "-O1", "-std=c++17", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I", include,
+                    os.path.join(HERE, "native", "ragged_runtime.cc"), "-o", so], check=True)
+    return so
+
+
+@pytest.fixture(scope="module")
+def child(runtime):
+    def run(script):
+        res = subprocess.run([sys.executable, "-c", PRELUDE.format(runtime=runtime) + CALLS + script], cwd=ROOT,
+                             capture_output=True, text=True, timeout=300)
+        assert res.returncode == 0, res.stderr
+        return json.loads(res.stdout)
+
+    return run
+
+
+def test_a_workspace_that_a_graph_holds_is_kept_when_it_grows(child):
+    """A captured call records the workspace's address. A later call that needs a larger one may not free it: replays
+    would write into memory that is someone else's by then. It goes with the context."""
+    got = child("""
+small, large = (lambda: columns(1501, 1700, 801)), (lambda: columns(4001, 4100, 4097))
+log, error = calls(small)
+assert error is None and len(of(log, "at")) == 1, (log, error)
+first = of(log, "at")[0]
+runtime.standin_capture(1)
+captured, error = calls(small)
+assert error is None, error
+runtime.standin_capture(0)
+grown, error = calls(large)
+assert error is None, error
+second = of(grown, "at")[0]
+again, error = calls(lambda: columns(8001, 8100, 8097))
+gone, error = calls(ctx.close)
+print(json.dumps([first, second, of(captured, "at"), of(captured, "free"), of(grown, "free"), of(again, "free"), of(gone, "free")]))
+""")
+    first, second, *rest = got
+    assert rest[:2] == [[], []]
+    assert first not in rest[2]  # the graph's
+    assert rest[3] == [second]  # no graph holds this one
+    assert first in rest[4] and second not in rest[4]
+
+
+def test_a_captured_call_may_not_grow_the_workspace(child):
+    """It is refused before it asks for anything that would end the capture."""
+    got = child("""
+runtime.standin_capture(1)
+log, error = calls(lambda: columns(1501, 1700, 801))
+runtime.standin_capture(0)
+print(json.dumps([log, error, calls(lambda: columns(1501, 1700, 801))[1]]))
+""")
+    log, error, after = got
+    assert error and "captur" in error, error
+    assert not any(line.split()[0] in ("launch", "malloc", "synchronize", "free") for line in log), log
+    assert after is None

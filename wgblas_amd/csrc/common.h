@@ -9,6 +9,12 @@
 
 #include "../../include/wgblas_hip.h"
 
+// A workspace that a captured graph still holds.
+struct wgb_kept {
+  void *ptr;
+  wgb_kept *next;
+};
+
 struct wgb_ctx {
   int device = 0;
   hipStream_t stream = nullptr;
@@ -30,6 +36,10 @@ struct wgb_ctx {
   // its copy of B (grown on demand, reused in stream order).
   void *op_ws = nullptr;
   size_t op_ws_bytes = 0;
+  // Whether a captured call uses op_ws, and those that captured calls used
+  // before it grew: their graphs may be replayed as long as the context lives.
+  bool op_ws_captured = false;
+  wgb_kept *kept_ws = nullptr;
   // Pinned host slot the host-result reductions store their scalar into, and
   // the number of the last such call.
   void *host_result = nullptr;
@@ -60,8 +70,11 @@ constexpr int kMaxReduceBlocks = 4096;
 constexpr size_t kScratchBytes = (size_t)kMaxReduceBlocks * 32 + 256;  // 32-byte partial slots + counter
 
 // Grows the context's operand workspace (ctx->op_ws) to at least `bytes`;
-// the stream is drained first, since an earlier launch may still read it.
-// Shared by the level-2 and level-3 routines (one stream orders them).
+// the stream is drained first, since an earlier launch may still read it. While
+// the stream is capturing it cannot grow, and one that a captured call was given
+// stays allocated when a later call grows it (wgb_destroy frees it).
+// Shared by the level-2 and level-3 routines and the products of expert layers
+// (one stream orders them).
 int ensure_op_workspace(wgb_ctx *ctx, size_t bytes);
 
 // GEMM k-band: which operand is triangular (zero outside its triangle).

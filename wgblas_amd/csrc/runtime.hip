@@ -43,17 +43,32 @@ void timing_end(wgb_ctx *ctx) {
 }
 
 int ensure_op_workspace(wgb_ctx *ctx, size_t bytes) {
-  if (ctx->op_ws_bytes >= bytes) return WGB_OK;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  WGB_CHECK_HIP(hipStreamIsCapturing(ctx->stream, &status));
+  const bool capturing = status != hipStreamCaptureStatusNone;
+  if (ctx->op_ws_bytes >= bytes) {
+    if (capturing) ctx->op_ws_captured = true;
+    return WGB_OK;
+  }
+  if (capturing)
+    return fail(WGB_ERR_HIP, "the context's workspace cannot grow while its stream is capturing: run the call once before");
   const size_t round = (size_t)16 << 20;
   bytes = (bytes + round - 1) / round * round;
   WGB_CHECK_HIP(hipStreamSynchronize(ctx->stream));
-  if (ctx->op_ws) WGB_CHECK_HIP(hipFree(ctx->op_ws));
+  if (ctx->op_ws_captured) {
+    wgb_kept *kept = new (std::nothrow) wgb_kept{ctx->op_ws, ctx->kept_ws};
+    if (!kept) return fail(WGB_ERR_ALLOC, "host allocation of the workspaces' list failed");
+    ctx->kept_ws = kept;
+  } else if (ctx->op_ws) {
+    WGB_CHECK_HIP(hipFree(ctx->op_ws));
+  }
   ctx->op_ws = nullptr;
   ctx->op_ws_bytes = 0;
+  ctx->op_ws_captured = false;
   if (hipMalloc(&ctx->op_ws, bytes) != hipSuccess) {
     (void)hipGetLastError();
     ctx->op_ws = nullptr;
-    return fail(WGB_ERR_ALLOC, "hipMalloc of the level-2/3 operand workspace failed");
+    return fail(WGB_ERR_ALLOC, "hipMalloc of the context's workspace failed");
   }
   ctx->op_ws_bytes = bytes;
   return WGB_OK;
@@ -141,6 +156,12 @@ extern "C" int wgb_destroy(wgb_ctx *ctx) {
   if (ctx->scratch) (void)hipFree(ctx->scratch);
   if (ctx->gemm_ws) (void)hipFree(ctx->gemm_ws);
   if (ctx->op_ws) (void)hipFree(ctx->op_ws);
+  while (ctx->kept_ws) {
+    wgb_kept *kept = ctx->kept_ws;
+    ctx->kept_ws = kept->next;
+    (void)hipFree(kept->ptr);
+    delete kept;
+  }
   if (ctx->host_result) (void)hipHostFree(ctx->host_result);
   if (ctx->ev_start) (void)hipEventDestroy(ctx->ev_start);
   if (ctx->ev_stop) (void)hipEventDestroy(ctx->ev_stop);
