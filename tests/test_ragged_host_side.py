@@ -92,3 +92,30 @@ print(json.dumps([log, error, calls(lambda: columns(1501, 1700, 801))[1]]))
     assert error and "captur" in error, error
     assert not any(line.split()[0] in ("launch", "malloc", "synchronize", "free") for line in log), log
     assert after is None
+
+
+def test_every_device_gets_the_kernels_lds_size(child):
+    """The kernels use more LDS than a launch has by default, which is allowed for each device by itself; where that
+    fails, the next call tries again."""
+    got = child("""
+second, out = wg.Context(1), []
+runtime.standin_attributes(0)
+out.append(calls(lambda: columns(4096, 4096, 1024)))
+runtime.standin_attributes(1)
+for on in (ctx, second, ctx, second):
+    out.append(calls(lambda: columns(4096, 4096, 1024, on=on)))
+print(json.dumps(out))
+""")
+    failed, *rest = got
+    assert failed[1] and not any(line.startswith("launch") for line in failed[0]), failed
+    seen = set()
+    for (log, error), device in zip(rest, "0101"):
+        assert error is None, error
+        for line in log:
+            word = line.split()
+            if word[0] == "attribute":
+                assert word[1] == device and (device, word[3]) not in seen, log
+                seen.add((device, word[3]))
+            elif word[0] == "launch" and "ragged_kernel" in word[5]:
+                assert (device, word[5]) in seen, (log, seen)
+    assert len(seen) >= 2 and len(seen) % 2 == 0

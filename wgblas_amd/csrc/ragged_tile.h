@@ -33,6 +33,7 @@
 #include "copy_plan.h"
 #include "tile_order.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace wgb_ragged {
@@ -1479,9 +1480,18 @@ template <class K>
 int launch(wgb_ctx *ctx, const Args &p, int64_t blocks) {
   if (blocks == 0) return WGB_OK;
   if (blocks > INT32_MAX) return wgb::fail(WGB_ERR_INVALID_VALUE, "grouped product: too many tiles");
-  static const hipError_t attr =
-      hipFuncSetAttribute((const void *)ragged_kernel<K>, hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
-  if (attr != hipSuccess) return wgb::fail_hip(attr, "LDS size of a grouped product");
+  // a kernel's LDS size is allowed for each device by itself: a bit for each one where it is
+  static std::atomic<uint64_t> allowed{0};
+  const uint64_t device = ctx->device < 64 ? (uint64_t)1 << ctx->device : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & device)) {
+    const hipError_t e =
+        hipFuncSetAttribute((const void *)ragged_kernel<K>, hipFuncAttributeMaxDynamicSharedMemorySize, K::LDS);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return wgb::fail_hip(e, "LDS size of a grouped product");
+    }
+    allowed.fetch_or(device, std::memory_order_relaxed);
+  }
   ragged_kernel<K><<<(unsigned)blocks, K::NT, K::LDS, ctx->stream>>>(p);
   WGB_CHECK_LAUNCH("ragged_kernel");
   return WGB_OK;
