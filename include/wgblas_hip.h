@@ -301,8 +301,9 @@ int wgb_strsm(wgb_ctx *ctx, int side, int uplo, int transA, int diag,
  * overlap (replays of a graph that holds one included), and a call that is to
  * be captured into a graph has to have run once before, so that the workspace
  * is there. A graph may be replayed until wgb_destroy: a workspace that it
- * holds stays allocated when a later call needs a larger one. No counterpart in
- * the reference, which has no grouped routine. */
+ * holds stays allocated when a later call needs a larger one. Where there is no
+ * memory for the workspace a call runs without it, slower, its sums of k in
+ * another order. No counterpart in the reference, which has no grouped routine. */
 
 /* C(:, j) <- alpha*op(A_g)*B(:, j) + beta*C(:, j) for the columns j of every
  * group g: B k-by-n and C m-by-n column-major, op(A_g) m-by-k with A_g at

@@ -119,3 +119,27 @@ print(json.dumps(out))
             elif word[0] == "launch" and "ragged_kernel" in word[5]:
                 assert (device, word[5]) in seen, (log, seen)
     assert len(seen) >= 2 and len(seen) % 2 == 0
+
+
+def test_no_memory_for_the_workspace_is_no_error(child):
+    """What it is for only makes a call faster: copies of operands at odd leading dimensions, and the sums of tiles that
+    are cut along k. Without it the operands are loaded through registers, the tiles are not cut."""
+    got = child("""
+out = []
+for limit in (1 << 20, 1 << 50):
+    runtime.standin_memory(ctypes.c_size_t(limit))
+    for call in (lambda: columns(1501, 1700, 801), lambda: ragged_k(1501, 1701, 8001), lambda: columns(2048, 8448, 4096, groups=2)):
+        log, error = calls(call)
+        out.append([error, [line.split() for line in log if line.startswith("launch")], of(log, "out_of_memory")])
+print(json.dumps(out))
+""")
+    for (error, launches, failed), odd in zip(got, (True, True, False) * 2):
+        assert error is None, error
+        kernels = [line[5] for line in launches]
+        assert all(int(line[1]) > 0 for line in launches)
+        if failed:
+            assert not any("align" in name or "Fold" in name for name in kernels), kernels
+        else:
+            assert any(("align" if odd else "Fold") in name for name in kernels), kernels
+        assert any("ragged_kernel" in name for name in kernels)
+    assert all(failed for _, _, failed in got[:3]) and not any(failed for _, _, failed in got[3:])

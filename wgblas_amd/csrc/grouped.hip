@@ -95,7 +95,8 @@ __global__ __launch_bounds__(256) void align_kernel(const uint16_t *X, int64_t l
 // Operands that cannot be copied (16-bit values at odd leading dimensions or
 // addresses) are first moved into the context's workspace where that and the
 // faster product take less time than the slower product: `now` and `then` are
-// the products' estimates, the move is a read and a write at 4.5 TB/s.
+// the products' estimates, the move is a read and a write at 4.5 TB/s. Where
+// there is no memory for the copies the slower product runs, which needs none.
 // a_cols: columns of a group's A. Sets vec where it did.
 int align_operands(wgb_ctx *ctx, Args &p, double now, double then, int64_t a_rows, int64_t a_cols, int64_t a_groups,
                    int64_t b_rows, int64_t b_cols, bool &vec) {
@@ -106,7 +107,7 @@ int align_operands(wgb_ctx *ctx, Args &p, double now, double then, int64_t a_row
   if (a_chunks * 16 >= (int64_t)1 << 22 || b_chunks * 16 >= (int64_t)1 << 22) return WGB_OK;
   if (then + 2.0 * (double)(bytes_a + bytes_b) / 4.5e6 + 3.0 >= now) return WGB_OK;
   const int st = wgb::ensure_op_workspace(ctx, (size_t)(bytes_a + bytes_b) + parts_bytes(ctx));
-  if (st) return st;
+  if (st) return st == WGB_ERR_ALLOC ? WGB_OK : st;
   p.parts = (float *)((char *)ctx->op_ws + bytes_a + bytes_b);
   auto move = [&](const char *X, int64_t ld, int64_t stride, int64_t cols, int64_t total, int64_t rows, int64_t chunks,
                   char *Y) {

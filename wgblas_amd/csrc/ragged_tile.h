@@ -1547,8 +1547,12 @@ int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles, bool exact, int64_t k) {
   if (rest && exact && p.round / (2 * rest) < 3) p.pieces = 1;
   if (rest && p.pieces > 1 && !p.parts) {
     const int st = wgb::ensure_op_workspace(ctx, parts_bytes(ctx));
-    if (st) return st;
-    p.parts = (float *)ctx->op_ws;
+    if (st == WGB_ERR_ALLOC)
+      p.pieces = 1;  // no memory for the sums: nothing is cut
+    else if (st)
+      return st;
+    else
+      p.parts = (float *)ctx->op_ws;
   }
   int st = launch<Turn>(ctx, p, blocks);
   if (st || !rest) return st;
