@@ -143,3 +143,61 @@ print(json.dumps(out))
             assert any(("align" if odd else "Fold") in name for name in kernels), kernels
         assert any("ragged_kernel" in name for name in kernels)
     assert all(failed for _, _, failed in got[:3]) and not any(failed for _, _, failed in got[3:])
+
+
+TILES = """
+import re
+
+def tiles(f):
+    "Of each product launch of f: its kind and the sides of its tiles."
+    log, error = calls(f)
+    assert error is None, error
+    out = []
+    for line in log:
+        word = line.split()
+        if word[0] != "launch":
+            continue
+        if "FoldKernel" in word[5]:
+            out.append("fold")
+        elif "TurnKernel" in word[5]:
+            out.append("256")
+        elif "SkinnyKernel" in word[5]:
+            out.append("few")
+        elif "ragged_kernel" in word[5]:
+            out.append("x".join(re.search("6KernelI.*?Li([0-9]+)ELi([0-9]+)E", word[5]).groups()))
+        else:
+            out.append(re.search("align|quantize", word[5]).group(0))
+    return out
+
+def mxfp4(m, n, k, groups=0, ct=BF16):
+    ld = (k + 127) // 128 * 128
+    if groups:
+        ctx.mxfp4_gemm_grouped(groups, m, n, k, 1.0, P, P, ld, m * ld, P, P, ld, P, 0.0, P, m, ct)
+    else:
+        ctx.mxfp4_gemm(m, n, k, 1.0, P, P, ld, P, P, ld, 0.0, P, m, ct)
+"""
+
+
+def test_small_products_take_small_tiles(child):
+    """One to three tiles of 256 x 256 would leave nearly all CUs idle for as long as one of them takes."""
+    got = child(TILES + """
+out = {}
+for m, n in ((256, 256), (512, 256), (256, 768), (200, 180), (40, 50)):
+    for k in (512, 4096, 8192):
+        out[f"columns {m} {n} {k}"] = tiles(lambda: columns(m, n, k))
+        out[f"no-transpose {m} {n} {k}"] = tiles(lambda: columns(m, n, k, trans=NO_TRANS, t=F16))
+        out[f"ragged k {m} {n} {k}"] = tiles(lambda: ragged_k(m, n, k))
+        out[f"mxfp4 {m} {n} {k}"] = tiles(lambda: mxfp4(m, n, k))
+print(json.dumps(out))
+""")
+    assert len(got) == 60
+    for case, kinds in got.items():
+        assert kinds == ["64x64"], (case, kinds)
+
+
+def test_small_operands_are_not_moved_on_a_false_estimate(child):
+    """At odd leading dimensions the copies cost a launch (about 3 us), which products this small do not get back."""
+    got = child(TILES + """
+print(json.dumps([tiles(lambda: columns(m, n, k, pad=1)) for m, n, k in ((64, 64, 256), (256, 64, 256), (200, 180, 128))]))
+""")
+    assert got == [["64x64"]] * 3

@@ -1600,7 +1600,7 @@ inline double small_time(int T, TileCost c, double tiles, double k, double c_siz
 inline double rounds_time(TileCost c256, TileCost c128, double tiles, double k, double c_size, int most) {
   const double store = 256 * 256 * c_size / 17.6e3, round = c256.first * (k / 1024) + store;
   const double whole = (double)(int64_t)tiles, rest = tiles - whole;
-  if (rest < 0.01) return whole * round;
+  if (whole > 0 && rest < 0.01) return whole * round;
   if (whole > 0 && rest <= 0.17 && most > 1) {
     const double pieces = 0.5 / rest < most ? 0.5 / rest : most;
     return whole * round + (c128.first + c128.next) * (k / 1024) / pieces + 15;
