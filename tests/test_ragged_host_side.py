@@ -201,3 +201,22 @@ def test_small_operands_are_not_moved_on_a_false_estimate(child):
 print(json.dumps([tiles(lambda: columns(m, n, k, pad=1)) for m, n, k in ((64, 64, 256), (256, 64, 256), (200, 180, 128))]))
 """)
     assert got == [["64x64"]] * 3
+
+
+def test_the_cases_of_the_256_tiles_take_them(child):
+    """tests/test_gpu_ragged_turns.py holds the 256 x 256 kernel to what it computes: all its cases have to reach it."""
+    from tests import test_gpu_ragged_turns as cases
+
+    mxfp4 = [(m, sum(sizes), k, len(sizes)) for m, k, sizes, _ in cases.MXFP4]
+    columns = [(m, sum(sizes), k, len(sizes)) for m, k, sizes, _ in cases.COLUMNS]
+    ragged_k = [(m, n, sum(sizes), len(sizes)) for m, n, sizes, _ in cases.K]
+    got = child(TILES + f"""
+print(json.dumps([
+    [tiles(lambda: mxfp4(*c, ct=ct)) for c in {mxfp4} for ct in (BF16, F32)],
+    [tiles(lambda: columns(*c, t=t, trans=trans)) for c in {columns} for t in (BF16, F16) for trans in (NO_TRANS, TRANS)],
+    [tiles(lambda: ragged_k(*c, t=t)) for c in {ragged_k} for t in (BF16, F16)]]))
+""")
+    for rows, listed, each in zip(got, (cases.MXFP4, cases.COLUMNS, cases.K), (2, 4, 2)):
+        assert len(rows) == each * len(listed)
+        for i, kinds in enumerate(rows):
+            assert "256" in kinds and ("fold" in kinds) == listed[i // each][3], (listed[i // each], kinds)
