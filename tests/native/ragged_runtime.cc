@@ -19,7 +19,32 @@ namespace {
 size_t g_limit = ~(size_t)0;  // the largest allocation that there is memory for
 int g_device = 0;
 bool g_attributes = true;  // whether kernel attributes can be set
-int g_arguments = 0;       // bytes of the product kernels' arguments that a launch's line gives, in hexadecimal
+int g_arguments = 0;       // bytes of the product kernels' argument block that are listed with a launch
+
+void note_bytes(const void *from, int count) {
+  g_log += "arguments ";
+  for (int i = 0; i < count; ++i) {
+    char hex[3];
+    std::snprintf(hex, sizeof(hex), "%02x", ((const unsigned char *)from)[i]);
+    g_log += hex;
+  }
+  g_log += '\n';
+}
+
+// A program that cannot call the functions below (node) is given what to list
+// and where to write the list at its end in its environment.
+struct Environment {
+  Environment() {
+    if (const char *bytes = std::getenv("STANDIN_ARGUMENTS")) g_arguments = std::atoi(bytes);
+  }
+  ~Environment() {
+    if (const char *path = std::getenv("STANDIN_LOG"))
+      if (std::FILE *file = std::fopen(path, "w")) {
+        std::fwrite(g_log.data(), 1, g_log.size(), file);
+        std::fclose(file);
+      }
+  }
+} g_environment;
 }  // namespace
 
 extern "C" {
@@ -44,14 +69,11 @@ hipError_t hipFree(void *ptr) {
 hipError_t hipLaunchKernel(const void *host, dim3 grid, dim3 block, void **args, size_t shared, hipStream_t stream) {
   const hipError_t e = standin_base_launch(host, grid, block, args, shared, stream);
   note("device %d shared %zu", g_device, shared);
-  if (g_arguments && g_kernels[host].find("ragged_kernel") != std::string::npos) {
-    g_log += "arguments ";
-    for (int i = 0; i < g_arguments; ++i) {
-      char hex[3];
-      std::snprintf(hex, sizeof(hex), "%02x", ((const unsigned char *)args[0])[i]);
-      g_log += hex;
-    }
-    g_log += '\n';
+  const std::string &name = g_kernels[host];
+  if (g_arguments && name.find("ragged_kernel") != std::string::npos) {
+    note_bytes(args[0], g_arguments);
+  } else if (g_arguments && name.find("quantize") != std::string::npos) {
+    for (int i = 0; i < 7; ++i) note_bytes(args[i], 8);  // pointers and sizes come first in all of them
   }
   return e;
 }
