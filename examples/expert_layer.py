@@ -52,8 +52,14 @@ class ExpertLayer:
         self.dw = ctx.empty(weights.shape, np.float32)
         self.offsets = ctx.empty(self.experts + 1, np.int64)
 
+    def count(self, x):
+        """Tokens of x, which the buffers have to hold."""
+        if len(x) > self.tokens:
+            raise ValueError(f"{len(x)} tokens, there is room for {self.tokens}")
+        return len(x)
+
     def forward(self, x, offsets):
-        n, ctx = len(x), self.ctx
+        n, ctx = self.count(x), self.ctx
         ctx.h2d(self.x.ptr, to_bf16(x))
         ctx.h2d(self.offsets.ptr, offsets)
         ctx.gemm_grouped(BF16, TRANS, self.experts, self.out, n, self.inner, 1.0, self.weights, self.inner,
@@ -62,7 +68,7 @@ class ExpertLayer:
 
     def backward(self, dy):
         """(gradient of the weights, gradient of the input) of the last forward's tokens."""
-        n, ctx = len(dy), self.ctx
+        n, ctx = self.count(dy), self.ctx
         ctx.h2d(self.dy.ptr, to_bf16(dy))
         ctx.gemm_grouped(BF16, NO_TRANS, self.experts, self.inner, n, self.out, 1.0, self.weights, self.inner,
                          self.out * self.inner, self.dy, self.out, self.offsets, 0.0, self.dx, self.inner, F32)
@@ -90,7 +96,7 @@ class ServedLayer:
         return ctx.empty((columns, self.ld // 2), np.uint8), ctx.empty((columns, self.ld // 32), np.uint8)
 
     def forward(self, x, offsets):
-        n, s, ctx = len(x), self.layer, self.layer.ctx
+        n, s, ctx = self.layer.count(x), self.layer, self.layer.ctx
         ctx.h2d(s.x.ptr, to_bf16(x))
         ctx.h2d(s.offsets.ptr, offsets)
         ctx.mxfp4_quantize(BF16, NO_TRANS, s.inner, n, s.x, s.inner, self.x_codes, self.x_scales, self.ld)
