@@ -106,7 +106,7 @@ class ServedLayer:
 
 
 def main(steps=60, experts=6, inner=192, out=160, tokens=1500, seed=0, log=print):
-    """Trains the layer on a teacher's outputs; returns (first loss, last loss, relative error of the 4-bit layer)."""
+    """Trains the layer on a teacher's outputs; returns (first loss, last loss, largest relative difference of the 4-bit layer)."""
     rng = np.random.default_rng(seed)
     directions = rng.standard_normal((experts, inner)) + 0.1 * rng.standard_normal(inner)
     teacher = rng.standard_normal((experts, out, inner)).astype(np.float32) / np.sqrt(inner)
@@ -135,8 +135,9 @@ def main(steps=60, experts=6, inner=192, out=160, tokens=1500, seed=0, log=print
             order, offsets = route(x, directions)
             x = x[order]
             exact, got = layer.forward(x, offsets).copy(), served.forward(x, offsets)
-            worst = max(worst, float(np.linalg.norm(got - exact) / np.linalg.norm(exact)))
-            log(f"{count:3d} tokens from 4-bit weights: relative difference {worst:.3f}")
+            difference = float(np.linalg.norm(got - exact) / np.linalg.norm(exact))
+            worst = max(worst, difference)
+            log(f"{count:3d} tokens from 4-bit weights: relative difference {difference:.3f}")
     return losses[0], losses[-1], worst
 
 

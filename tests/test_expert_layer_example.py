@@ -62,3 +62,15 @@ def test_more_tokens_than_there_is_room_for_are_refused(example):
     assert ctx.names == []
     layer.forward(np.zeros((10, 16)), np.array([0, 4, 10]))
     assert "gemm_grouped" in ctx.names
+
+
+def test_each_line_gives_its_own_difference(example, monkeypatch):
+    """Single tokens and the prompt have their own figures; the largest is what main returns."""
+    differences = {1: 0.5, 3: 0.25, 200: 0.375}
+    monkeypatch.setattr(example, "Context", Calls)
+    monkeypatch.setattr(example.ExpertLayer, "forward", lambda self, x, offsets: np.ones((len(x), 4)))
+    monkeypatch.setattr(example.ServedLayer, "forward", lambda self, x, offsets: np.full((len(x), 4), 1 + differences[len(x)]))
+    lines = []
+    worst = example.main(steps=1, out=4, tokens=200, log=lines.append)[2]
+    assert [line.split()[-1] for line in lines[1:]] == ["0.500", "0.250", "0.375"]
+    assert worst == 0.5
