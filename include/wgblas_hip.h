@@ -349,8 +349,9 @@ int wgb_mxfp4_quantize(wgb_ctx *ctx, int type, int trans, int64_t k, int64_t n,
                        uint8_t *scales, int64_t ld);
 
 /* The values a k-by-n MXFP4 matrix stands for, in `type`, column-major:
- * exact in WGB_F32 and, but for fp16's range, in the 16-bit types (rounded to
- * nearest even where not). */
+ * exact in WGB_F32 and WGB_BF16 up to their largest number (scales of 2^126 and
+ * 2^127 can pass it, which quantising never gives: Inf), in WGB_F16 in its range
+ * (rounded to nearest even below it, Inf above). */
 int wgb_mxfp4_dequantize(wgb_ctx *ctx, int type, int64_t k, int64_t n,
                          const uint8_t *codes, const uint8_t *scales,
                          int64_t ld, void *X, int64_t ldx);

@@ -1,6 +1,7 @@
 """The host side of the grouped and 4-bit products without a GPU, through a
 stand-in for the HIP runtime (tests/native/ragged_runtime.cc) that runs no
-kernel and keeps a list of what was asked of it: the context's workspace."""
+kernel and keeps a list of what was asked of it: the context's workspace, the
+kernels' LDS sizes, which tiles a call takes."""
 import json
 import os
 import shutil

@@ -1017,8 +1017,8 @@ struct FoldKernel {
 // The 256 x 256 tile of the large products: 8 waves of 128 x 64 each (the
 // columns in blocks of 16, 64 apart), two on every SIMD, which take turns.
 // Time runs in slots between barriers: while one wave of a SIMD runs the 32
-// MFMAs of a step (512 cycles of the matrix core) with the copies spread among
-// them, the other reads its operands of the next step from LDS. Waves 4 - 7
+// MFMAs of a step (512 cycles of the matrix core), the other reads its operands
+// of the next step from LDS and issues its share of the copies. Waves 4 - 7
 // run one slot behind waves 0 - 3 (k-tile k, steps 0 and 1):
 //   slot           4 k             4 k + 1     4 k + 2     4 k + 3     4 k + 4
 //   waves 0 - 3    read 0          multiply 0  read 1      multiply 1  read 0
@@ -1028,16 +1028,21 @@ struct FoldKernel {
 // a tile is finished, and one half of the waves stores its part of C while
 // the other multiplies. 16-bit: A's and B's k-tiles rotate through five units
 // of 32 KB, all of LDS (A 0, B 0, A 1, B 1, ...). Both units of k-tile k - 1
-// are free from slot 4 k on: waves 0 - 3 copy B k + 1 in "multiply 0" of k and
-// A k + 2 in "multiply 1", waves 4 - 7 B k + 1 in "multiply 1" of k - 1 and
-// A k + 2 in "multiply 0" of k; three or four slots before they are read. fp4
-// also keeps scales and has four units: waves 0 - 3 copy all of k + 1 in
-// "multiply 0" of k, waves 4 - 7 in "multiply 1" of k - 1.
-// 16-bit is bound by the matrix cores and the power that they draw: 8192^3 in
-// bf16 735 to 745 us, 1.5 PFLOP/s; 16 groups of 1024 columns 8192 x 16384 x 4096 in
-// 830 us (A is read once for each group) and ragged ones in 980. fp4 is bound by
-// the copies and reads of its slots, whose MFMAs take half as long: 8192^3 302
-// us, 3.6 PFLOP/s.
+// are free from slot 4 k on, when waves 4 - 7 have read its step 1: either half
+// of the waves issues its copies of B k + 1 in "read 0" of k and of A k + 2 in
+// "read 1", and waits for them at the end of "read 1" of k (B) and of k + 1 (A),
+// two and four slots later, before the first read of k + 1 and k + 2. fp4 also
+// keeps scales and has four units: either half issues all of k + 1 in "read 0"
+// of k and waits for all of it at the end of "read 1".
+// 16-bit is bound by the matrix cores and the clock that they leave (1.7 GHz at
+// 8192^3 in bf16, 735 to 780 us, 1.4 to 1.5 PFLOP/s, busy 0.76 of the time); 16 groups of 1024 columns 8192 x 16384 x 4096 in
+// 830 us (A is read once for each group) and ragged ones in 980. fp4's k-tiles
+// have as many bytes and as many MFMA cycles as the 16-bit ones, but the matrix
+// cores are busy for 0.38 of the time (16-bit: 0.76; 4096 columns times 8192 x
+// 8192 165 us, 8192^3 302 us, 3.6 PFLOP/s).
+// What differs is that each k-tile waits for all its copies two slots after their
+// issue, the scale reads, whose banks conflict, and registers that are spilled;
+// which of them costs most has not been measured.
 template <class E, bool AMC, bool BMC, bool RK>
 struct TurnKernel {
   static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
@@ -1594,9 +1599,10 @@ inline double small_time(int T, TileCost c, double tiles, double k, double c_siz
   const double store = T * T * c_size / 17.6e3, depth = k / 1024;
   return c.first * depth + store + (tiles > 1 ? tiles - 1 : 0) * (c.next * depth + store);
 }
-// 256 x 256 tiles: whole rounds, then the rest as launch_rounds has it (cut
-// along k, a piece more than fills its share: 60 quarters at k = 4096 in 16
-// bits 30 us and 8 for the sums).
+// 256 x 256 tiles: whole rounds (fewer tiles than CUs are one, however few: 512
+// x 256 x 8192 in bf16 138 us, on 64 x 64 tiles 58), then the rest as
+// launch_rounds has it (cut along k, a piece more than fills its share: 60
+// quarters at k = 4096 in 16 bits 30 us and 8 for the sums).
 inline double rounds_time(TileCost c256, TileCost c128, double tiles, double k, double c_size, int most) {
   const double store = 256 * 256 * c_size / 17.6e3, round = c256.first * (k / 1024) + store;
   const double whole = (double)(int64_t)tiles, rest = tiles - whole;
