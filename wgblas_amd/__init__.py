@@ -17,6 +17,8 @@ from .native import (  # noqa: F401
     NO_TRANS,
     NON_UNIT,
     RIGHT,
+    SIGMOID,
+    SOFTMAX,
     TRANS,
     UNIT,
     UPPER,

@@ -21,7 +21,7 @@ LIBDIR = os.path.join(HERE, "lib")
 INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["runtime.hip", "reduce.hip", "gemm.hip", "level3.hip", "level2.hip", "noalloc.hip",
-               "grouped.hip", "mxfp4.hip"]
+               "grouped.hip", "mxfp4.hip", "fp8.hip", "route.hip"]
 LIB_NAME = "libwgblas_hip.so"
 ADDON_NAME = "wgblas_hip.node"
 ARCH = os.environ.get("WGBLAS_OFFLOAD_ARCH", "gfx950")

@@ -18,9 +18,11 @@ constexpr int TB = 128;
 
 // Chunk keys of the row-contiguous layout, for k-row r of a tile whose rows
 // have `chunks` chunks: 16-bit transposing reads touch k-rows 8 g .. 8 g + 3
-// (32 bytes of each), fp32 reads k-rows 4 g (64 bytes of each).
+// (32 bytes of each), fp32 reads k-rows 4 g (64 bytes of each), 8-bit ones
+// k-rows 16 g .. 16 g + 7 (16 bytes of each).
 template <int BITS, int CHUNKS>
 __host__ __device__ __forceinline__ int mc_key(int r) {
+  if (BITS == 8) return ((r & 7) | (((r >> 4) & 1) << 3)) & (CHUNKS - 1);
   const int key = BITS == 16 ? ((r & 3) << 1) | (((r >> 3) & 1) << 3) : ((r >> 2) & 3) << 2;
   return key & (CHUNKS - 1);
 }
@@ -76,9 +78,9 @@ struct CopyPlan {
   // a last chunk that the end of the rows cuts reads on into the k-rows after
   // it, one where they are 16 bytes apart or more, up to EPC - 1 of them where
   // they are closer (a matrix of 1 to 3 rows). The last k-rows do not have
-  // those.
+  // those. 8-bit columns are whole runs of 128 elements: none is cut.
   __host__ __device__ __forceinline__ int whole_tiles() const {
-    const bool cut = MC && rows_left < BT;
+    const bool cut = MC && BITS != 8 && rows_left < BT;
     const int after = !cut ? 0 : ld < 16 ? EPC - 1 : 1;
     return (int)((K > after ? K - after : 0) / BK);
   }
@@ -91,7 +93,7 @@ struct CopyPlan {
   // (tail_mask). Not where a cut chunk could reach past the matrix: at its
   // last row (k-contiguous), or with cut rows (row-contiguous).
   __host__ __device__ __forceinline__ bool soft_tail() const {
-    return MC ? rows_left >= BT : K % EPC == 0 || (rows_left > BT && K >= EPC);
+    return BITS == 8 ? MC : MC ? rows_left >= BT : K % EPC == 0 || (rows_left > BT && K >= EPC);
   }
   __host__ __device__ __forceinline__ uint32_t tail_voff(int r) const {
     const int left = (int)(K % BK);

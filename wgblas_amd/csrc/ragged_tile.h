@@ -134,8 +134,14 @@ struct Args {
   int round;
   int pieces;     // of k that a tile of that rest is cut into at most, each a block's; their sums go to
   float *parts;   // this array, 128 x 128 a block
+  // fp8: scales of blocks of 128 of k. A's of row r and block b at a_row (r /
+  // block_a) + a_k b, the groups' a_group apart; B's of column j at j + b_k b
+  const float *block_scale_a, *block_scale_b;
+  int64_t a_row, a_k, a_group, b_k;
+  int block_a;
+  int64_t a_rows;  // fp8, row-contiguous A: rows rounded up to whole runs of 128
   int stream;  // C's columns start at 64-byte boundaries: large results bypass the caches
-  int c_f32;   // C holds fp32 (else the operands' type; fp4: bf16, or f16 with c_f16)
+  int c_f32;   // C holds fp32 (else the operands' type; fp4 and fp8: bf16, or f16 with c_f16)
   int c_f16;
 };
 
@@ -776,7 +782,7 @@ __device__ __forceinline__ void store_tile(const Args &p, int64_t at, const f4 (
                                            int64_t cols, int lane) {
   if (E::kBits == 32 || p.c_f32) {
     epilogue<float, MB, NB, STEP, STREAM>(p, (float *)p.C + at, acc, row0, p.m, col0, cols, lane);
-  } else if constexpr (E::kBits == 4) {
+  } else if constexpr (E::kBits <= 8) {
     if (p.c_f16)
       epilogue<_Float16, MB, NB, STEP, STREAM>(p, (_Float16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
     else

@@ -1,0 +1,938 @@
+// Routing tokens to experts: the choice of each token's experts and their
+// weights (wgb_route), its gradient (wgb_route_grad), the order of the pairs
+// (token, expert) by expert (wgb_route_order), and the tokens' way to the
+// experts' columns and back (wgb_route_gather, wgb_route_combine,
+// wgb_route_combine_grad).
+//
+// wgblas has no counterpart. These are what stands before and behind the
+// grouped products (grouped.hip, mxfp4.hip, fp8.hip): their boundaries and
+// the order of their columns are this file's results, and stay on the GPU.
+#include "common.h"
+
+#include <type_traits>
+
+namespace {
+
+using wgb::fail;
+
+constexpr int kMaxExperts = 1024, kMaxTopk = 64, kMaxGroups = 64;
+
+// ---- reductions over the lanes of a token ------------------------------------
+
+// All lanes of each run of LPT (16 or 64) lanes get op over the run. The 16
+// lanes of a DPP row are rotated onto each other; rows meet by shuffles.
+template <int ROR>
+__device__ __forceinline__ float ror(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + ROR, 0xf, 0xf, true));
+}
+template <int ROR>
+__device__ __forceinline__ double ror(double x) {
+  typedef int i2 __attribute__((ext_vector_type(2)));
+  i2 v = __builtin_bit_cast(i2, x);
+  v[0] = __builtin_amdgcn_mov_dpp(v[0], 0x120 + ROR, 0xf, 0xf, true);
+  v[1] = __builtin_amdgcn_mov_dpp(v[1], 0x120 + ROR, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, v);
+}
+template <int LPT, class T, class Op>
+__device__ __forceinline__ T over_lanes(T x, Op op) {
+  x = op(x, ror<8>(x));
+  x = op(x, ror<4>(x));
+  x = op(x, ror<2>(x));
+  x = op(x, ror<1>(x));
+  if constexpr (LPT == 64) {
+    x = op(x, __shfl_xor(x, 16));
+    x = op(x, __shfl_xor(x, 32));
+  }
+  return x;
+}
+struct Max {
+  template <class T>
+  __device__ T operator()(T a, T b) const {
+    return a > b ? a : b;
+  }
+};
+struct Sum {
+  template <class T>
+  __device__ T operator()(T a, T b) const {
+    return a + b;
+  }
+};
+// The lowest lane of this token's run for which `hit` holds, counted in the
+// run; LPT where none.
+template <int LPT>
+__device__ __forceinline__ int first_lane(bool hit, int lane) {
+  uint64_t b = __ballot(hit);
+  if constexpr (LPT == 64) return b ? __builtin_ctzll(b) : LPT;
+  const uint32_t mine = (uint32_t)(b >> (lane & 48)) & 0xffffu;
+  return mine ? __builtin_ctz(mine) : LPT;
+}
+
+// ---- the choice ----------------------------------------------------------------
+
+struct RouteArgs {
+  const void *logits;
+  int64_t ldl, n;
+  const float *bias;
+  int experts, topk, groups, top_groups, best, per;
+  uint32_t magic;  // e / per = e * magic >> 20 for e < 1024
+  int sigmoid, renorm;
+  float scale;
+  int32_t *ids;
+  float *weights;
+};
+
+template <class F>
+struct Limits;
+template <>
+struct Limits<float> {
+  static __device__ float none() { return -__builtin_inff(); }
+  static __device__ float nan() { return -1e38f; }  // below what is a number; two of them can be added
+};
+template <>
+struct Limits<double> {
+  static __device__ double none() { return -__builtin_inf(); }
+  static __device__ double nan() { return -1e300; }
+};
+
+// LPT lanes a token, PER consecutive experts a lane. A token's choice values
+// stay in its lanes' registers; each round takes the largest, the lowest
+// expert of equal ones.
+//
+// F: what is compared. Scores grow with the logits, so without a bias and
+// with groups by their best expert the logits themselves decide (float,
+// exact). Otherwise values next to each other decide, score + bias, and are
+// held in 64 bits: in 32 the choice would depend on the exponential's last
+// bits.
+template <class T, class F, int LPT, int PER>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
+  constexpr bool kWide = std::is_same<F, double>::value;
+  constexpr int TOKENS = 256 / LPT;
+  __shared__ int chosen[TOKENS][kMaxTopk];
+  extern __shared__ __align__(16) char route_smem[];  // with groups: values, groups' scores and which are kept
+  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
+  const bool here = token < p.n;
+  const T *x = (const T *)p.logits + (here ? token : p.n - 1) * p.ldl;
+  const int e0 = lane * PER;
+
+  float l[PER];
+  if (e0 + PER <= p.experts) {
+    struct __attribute__((packed, aligned(sizeof(T)))) V {
+      T v[PER];
+    };
+    const V v = *reinterpret_cast<const V *>(x + e0);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) l[j] = (float)v.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) l[j] = e0 + j < p.experts ? (float)x[e0 + j] : -__builtin_inff();
+  }
+
+  // softmax: the largest logit and the sum of exponentials
+  float top = 0.0f, total = 1.0f;
+  if (!p.sigmoid) {
+    top = l[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) top = fmaxf(top, l[j]);
+    top = over_lanes<LPT>(top, Max());
+    if (top == -__builtin_inff()) top = 0.0f;  // no expert at all: scores of zero
+    total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) total += expf(l[j] - top);
+    total = over_lanes<LPT>(total, Sum());
+    if (total == 0.0f) total = 1.0f;
+  }
+
+  F v[PER];
+  if constexpr (kWide) {
+    double sum = 1.0;
+    double s[PER];
+    if (p.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
+    } else {
+      sum = 0.0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        s[j] = exp((double)l[j] - (double)top);
+        sum += s[j];
+      }
+      sum = over_lanes<LPT>(sum, Sum());
+      if (sum == 0.0) sum = 1.0;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const float b = p.bias && e0 + j < p.experts ? p.bias[e0 + j] : 0.0f;
+      v[j] = l[j] == -__builtin_inff() ? -__builtin_inf() : s[j] / sum + (double)b;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = l[j];
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (v[j] != v[j]) v[j] = Limits<F>::nan();
+
+  if (p.groups > 1) {
+    const int room = (p.experts + 1) & ~1;
+    F *values = reinterpret_cast<F *>(route_smem) + slot * (room + p.groups);
+    F *score = values + room;
+    uint8_t *kept = reinterpret_cast<uint8_t *>(reinterpret_cast<F *>(route_smem) + TOKENS * (room + p.groups)) + slot * kMaxGroups;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (e0 + j < p.experts) values[e0 + j] = v[j];
+    __syncthreads();
+    for (int g = lane; g < p.groups; g += LPT) {
+      F a = Limits<F>::none(), b = a;
+      for (int i = 0; i < p.per; ++i) {
+        const F w = values[g * p.per + i];
+        if (w > a) {
+          b = a;
+          a = w;
+        } else if (w > b) {
+          b = w;
+        }
+      }
+      score[g] = p.best == 2 && p.per > 1 ? a + b : a;
+    }
+    __syncthreads();
+    for (int g = lane; g < p.groups; g += LPT) {
+      const F mine = score[g];
+      int before = 0;
+      for (int o = 0; o < p.groups; ++o) before += score[o] > mine || (score[o] == mine && o < g);
+      kept[g] = before < p.top_groups;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (e0 + j < p.experts && !kept[((uint32_t)(e0 + j) * p.magic) >> 20]) v[j] = Limits<F>::none();
+  }
+
+  const int wave_lane = threadIdx.x & 63;
+  for (int s = 0; s < p.topk; ++s) {
+    F best = v[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) best = v[j] > best ? v[j] : best;
+    const F most = over_lanes<LPT>(best, Max());
+    const bool any = most > Limits<F>::none();
+    const bool mine = any && first_lane<LPT>(best == most, wave_lane) == lane;
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (mine && at < 0 && v[j] == most) {
+        at = j;
+        v[j] = Limits<F>::none();
+      }
+    if (any ? mine : lane == 0) chosen[slot][s] = any ? e0 + at : -1;
+  }
+  __syncthreads();
+
+  // the weights, a lane a choice
+  float w[kMaxTopk / LPT], sum = 0.0f;
+#pragma unroll
+  for (int r = 0; r < kMaxTopk / LPT; ++r) {
+    const int s = lane + r * LPT;
+    w[r] = 0.0f;
+    if (s < p.topk && chosen[slot][s] >= 0) {
+      const float c = (float)x[chosen[slot][s]];
+      w[r] = p.sigmoid ? 1.0f / (1.0f + expf(-c)) : expf(c - top) / total;
+    }
+    sum += w[r];
+  }
+  if (p.renorm) {
+    sum = over_lanes<LPT>(sum, Sum());
+    if (sum == 0.0f) sum = 1.0f;
+  } else {
+    sum = 1.0f;
+  }
+#pragma unroll
+  for (int r = 0; r < kMaxTopk / LPT; ++r) {
+    const int s = lane + r * LPT;
+    if (here && s < p.topk) {
+      p.ids[token * p.topk + s] = chosen[slot][s];
+      p.weights[token * p.topk + s] = w[r] / sum * p.scale;
+    }
+  }
+}
+
+template <class T, class F, int LPT, int PER>
+int launch_route(wgb_ctx *ctx, const RouteArgs &p) {
+  constexpr int TOKENS = 256 / LPT;
+  const size_t lds = p.groups > 1 ? TOKENS * (sizeof(F) * (((p.experts + 1) & ~1) + p.groups) + kMaxGroups) : 0;
+  route_kernel<T, F, LPT, PER><<<(unsigned)((p.n + TOKENS - 1) / TOKENS), 256, lds, ctx->stream>>>(p);
+  WGB_CHECK_LAUNCH("route_kernel");
+  return WGB_OK;
+}
+
+template <class T, class F>
+int route_sizes(wgb_ctx *ctx, const RouteArgs &p) {
+  if (p.experts <= 16) return launch_route<T, F, 16, 1>(ctx, p);
+  if (p.experts <= 32) return launch_route<T, F, 16, 2>(ctx, p);
+  if (p.experts <= 64) return launch_route<T, F, 16, 4>(ctx, p);
+  if (p.experts <= 128) return launch_route<T, F, 16, 8>(ctx, p);
+  if (p.experts <= 256) return launch_route<T, F, 16, 16>(ctx, p);
+  if (p.experts <= 512) return launch_route<T, F, 64, 8>(ctx, p);
+  return launch_route<T, F, 64, 16>(ctx, p);
+}
+
+template <class T>
+int route(wgb_ctx *ctx, const RouteArgs &p) {
+  const bool wide = p.bias || (p.groups > 1 && p.best == 2);
+  return wide ? route_sizes<T, double>(ctx, p) : route_sizes<T, float>(ctx, p);
+}
+
+// ---- its gradient -----------------------------------------------------------------
+
+struct GradArgs {
+  const void *logits;
+  int64_t ldl, n;
+  const int32_t *ids;
+  const float *dweights;
+  void *dlogits;
+  int64_t ldd;
+  int experts, topk, sigmoid, renorm;
+  float scale;
+};
+
+// With p the scores, S the sum of the chosen ones and d_s what came back for
+// weight s (times scale): the chosen scores' gradients are q_s = d_s, or with
+// renormalised weights (d_s - sum_r d_r p_r / S) / S. Sigmoid: the chosen
+// logits get q p (1 - p), the others 0; softmax: every logit p (q - sum_r q_r
+// p_r). An expert that is there twice gets the sum, in the slots' order.
+template <class T, int LPT, int PER>
+__global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
+  constexpr int TOKENS = 256 / LPT, SLOTS = kMaxTopk / LPT;
+  __shared__ float q[TOKENS][kMaxTopk];
+  __shared__ int at[TOKENS][kMaxTopk];
+  __shared__ float back[TOKENS][LPT * PER];
+  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
+  const bool here = token < p.n;
+  const int64_t row = here ? token : p.n - 1;
+  const T *x = (const T *)p.logits + row * p.ldl;
+  const int e0 = lane * PER;
+  float l[PER];
+  if (e0 + PER <= p.experts) {
+    struct __attribute__((packed, aligned(sizeof(T)))) V {
+      T v[PER];
+    };
+    const V v = *reinterpret_cast<const V *>(x + e0);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) l[j] = (float)v.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) l[j] = e0 + j < p.experts ? (float)x[e0 + j] : -__builtin_inff();
+  }
+  // scores, and for sigmoid p (1 - p)
+  float s[PER], slope[PER], top = 0.0f, total = 1.0f;
+  if (p.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const float t = expf(-fabsf(l[j])), r = 1.0f / (1.0f + t);
+      s[j] = l[j] < 0.0f ? t * r : r;
+      slope[j] = t * r * r;
+    }
+  } else {
+    top = l[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) top = fmaxf(top, l[j]);
+    top = over_lanes<LPT>(top, Max());
+    if (top == -__builtin_inff()) top = 0.0f;
+    total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) total += s[j] = expf(l[j] - top);
+    total = over_lanes<LPT>(total, Sum());
+    if (total == 0.0f) total = 1.0f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) s[j] /= total;
+  }
+  // the chosen scores: a lane a slot
+  float w[SLOTS], d[SLOTS], sum = 0.0f, dot = 0.0f;
+#pragma unroll
+  for (int r = 0; r < SLOTS; ++r) {
+    const int i = lane + r * LPT;
+    w[r] = d[r] = 0.0f;
+    int id = -1;
+    if (i < p.topk) {
+      id = p.ids[row * p.topk + i];
+      if (id >= p.experts) id = -1;
+      if (id >= 0) {
+        const float c = (float)x[id];
+        w[r] = p.sigmoid ? 1.0f / (1.0f + expf(-c)) : expf(c - top) / total;
+        d[r] = p.dweights[row * p.topk + i] * p.scale;
+      }
+      at[slot][i] = id;
+    }
+    sum += w[r];
+    dot += d[r] * w[r];
+  }
+  sum = over_lanes<LPT>(sum, Sum());
+  dot = over_lanes<LPT>(dot, Sum());
+  if (sum == 0.0f) sum = 1.0f;
+  float inner = 0.0f;  // sum of q p, of the softmax
+#pragma unroll
+  for (int r = 0; r < SLOTS; ++r) {
+    const int i = lane + r * LPT;
+    if (i < p.topk) {
+      const float g = p.renorm ? (d[r] - dot / sum) / sum : d[r];
+      q[slot][i] = g;
+      if (at[slot][i] >= 0) inner += g * w[r];
+    }
+  }
+  inner = over_lanes<LPT>(inner, Sum());
+#pragma unroll
+  for (int j = 0; j < PER; ++j) back[slot][e0 + j] = 0.0f;
+  __syncthreads();
+  for (int i = 0; i < p.topk; ++i) {  // each expert's lane adds its own
+    const int id = at[slot][i];
+    if (id >= e0 && id < e0 + PER) back[slot][id] += q[slot][i];
+  }
+  if (!here) return;
+  T out[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const float g = back[slot][e0 + j];
+    out[j] = (T)(p.sigmoid ? g * slope[j] : s[j] * (g - inner));
+  }
+  T *y = (T *)p.dlogits + token * p.ldd;
+  if (e0 + PER <= p.experts) {
+    struct __attribute__((packed, aligned(sizeof(T)))) V {
+      T v[PER];
+    };
+    V v;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v.v[j] = out[j];
+    *reinterpret_cast<V *>(y + e0) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (e0 + j < p.experts) y[e0 + j] = out[j];
+  }
+}
+
+template <class T, int LPT, int PER>
+int launch_grad(wgb_ctx *ctx, const GradArgs &p) {
+  constexpr int TOKENS = 256 / LPT;
+  route_grad_kernel<T, LPT, PER><<<(unsigned)((p.n + TOKENS - 1) / TOKENS), 256, 0, ctx->stream>>>(p);
+  WGB_CHECK_LAUNCH("route_grad_kernel");
+  return WGB_OK;
+}
+
+template <class T>
+int grad(wgb_ctx *ctx, const GradArgs &p) {
+  if (p.experts <= 16) return launch_grad<T, 16, 1>(ctx, p);
+  if (p.experts <= 32) return launch_grad<T, 16, 2>(ctx, p);
+  if (p.experts <= 64) return launch_grad<T, 16, 4>(ctx, p);
+  if (p.experts <= 128) return launch_grad<T, 16, 8>(ctx, p);
+  if (p.experts <= 256) return launch_grad<T, 16, 16>(ctx, p);
+  if (p.experts <= 512) return launch_grad<T, 64, 8>(ctx, p);
+  return launch_grad<T, 64, 16>(ctx, p);
+}
+
+// ---- the order by expert ------------------------------------------------------------
+
+// A stable counting sort of the pairs. Each block has a run of `chunk` pairs:
+// their counts go to counts[block][expert] (order_count_kernel), then every
+// block adds up the counts before its own and of all, and places its pairs
+// (order_place_kernel). A single block counts for itself: one launch.
+__device__ __forceinline__ int expert_of(const int32_t *ids, int64_t p, int64_t end, int experts) {
+  const int e = p < end ? ids[p] : -1;
+  return e < experts ? e : -1;
+}
+
+__global__ __launch_bounds__(1024) void order_count_kernel(const int32_t *ids, int64_t pairs, int64_t chunk, int experts,
+                                                           int32_t *counts) {
+  __shared__ int32_t count[kMaxExperts];
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) count[e] = 0;
+  __syncthreads();
+  const int64_t begin = blockIdx.x * chunk, end = begin + chunk < pairs ? begin + chunk : pairs;
+  for (int64_t p = begin + threadIdx.x; p < end; p += blockDim.x) {
+    const int e = expert_of(ids, p, end, experts);
+    if (e >= 0) atomicAdd(&count[e], 1);  // whole numbers: any order gives the same
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[(int64_t)blockIdx.x * experts + e] = count[e];
+}
+
+__global__ __launch_bounds__(1024) void order_place_kernel(const int32_t *ids, int64_t pairs, int64_t chunk, int experts,
+                                                           int bits, const int32_t *counts, int blocks, int64_t *offsets,
+                                                           int32_t *places, int32_t *sorted) {
+  // next[e]: where the block's next pair of expert e goes; in a round, of[w][e] pairs of wave w's
+  __shared__ int32_t next[kMaxExperts], all[kMaxExperts], sums[16];
+  __shared__ uint16_t of[16][kMaxExperts];
+  const int t = threadIdx.x, threads = blockDim.x, lane = t & 63, wave = t >> 6, waves = threads >> 6;
+  const int64_t begin = blockIdx.x * chunk, end = begin + chunk < pairs ? begin + chunk : pairs;
+  for (int e = t; e < experts; e += threads) next[e] = all[e] = 0;
+  __syncthreads();
+  if (blocks == 1) {
+    for (int64_t p = t; p < end; p += threads) {
+      const int e = expert_of(ids, p, end, experts);
+      if (e >= 0) atomicAdd(&all[e], 1);
+    }
+  } else {
+    // threads / width rows of counts at once
+    const int width = 1 << bits, step = threads >> bits;
+    const int e = t & (width - 1);
+    if (e < experts) {
+      int before = 0, sum = 0;
+      for (int b = t >> bits; b < blocks; b += step) {
+        const int c = counts[(int64_t)b * experts + e];
+        sum += c;
+        before += b < (int)blockIdx.x ? c : 0;
+      }
+      atomicAdd(&all[e], sum);
+      atomicAdd(&next[e], before);
+    }
+  }
+  __syncthreads();
+  // exclusive sums of all[] over the experts, a thread each (experts <= threads)
+  int mine = t < experts ? all[t] : 0, scan = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(scan, d);
+    if (lane >= d) scan += up;
+  }
+  if (lane == 63) sums[wave] = scan;
+  __syncthreads();
+  int ahead = 0, total = 0;
+  for (int w = 0; w < waves; ++w) {
+    if (w < wave) ahead += sums[w];
+    total += sums[w];
+  }
+  if (t < experts) {
+    next[t] += ahead + scan - mine;
+    if (blockIdx.x == 0) offsets[t] = ahead + scan - mine;
+  }
+  if (t == 0 && blockIdx.x == 0) offsets[experts] = total;
+
+  for (int64_t p0 = begin; p0 < end; p0 += threads) {
+    const int64_t p = p0 + t;
+    const int e = expert_of(ids, p, end, experts);
+    for (int i = t; i < waves * experts; i += threads) of[i / experts][i % experts] = 0;
+    // lanes with the same expert
+    uint64_t same = __ballot(e >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((e >> b) & 1);
+      same &= (e >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+    __syncthreads();
+    if (e >= 0 && rank == 0) of[wave][e] = (uint16_t)__popcll(same);
+    __syncthreads();
+    int place = -1;
+    if (e >= 0) {
+      place = next[e] + rank;
+      for (int w = 0; w < wave; ++w) place += of[w][e];
+      sorted[place] = (int32_t)p;
+    }
+    if (p < end) {
+      places[p] = place;
+      if (p >= total) sorted[p] = -1;  // behind the last group
+    }
+    __syncthreads();
+    for (int x = t; x < experts; x += threads)
+      for (int w = 0; w < waves; ++w) next[x] += of[w][x];
+    __syncthreads();
+  }
+}
+
+// ---- moving rows -----------------------------------------------------------------------
+
+struct RowsArgs {
+  int64_t d, n;
+  int topk;
+  const void *X, *Y;
+  int64_t ldx, ldy;
+  const int32_t *places;
+  const float *weights;
+  float beta;
+  void *out;
+  int64_t ldo;
+  float *dweights;
+  int shift;  // 2^shift threads a token
+};
+
+template <class T>
+struct Lanes {
+  static constexpr int V = 16 / sizeof(T);  // elements of a 16-byte access
+  struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+    T v[V];
+  };
+  // up to `left` elements at x, as floats
+  static __device__ __forceinline__ void load(const T *x, int64_t left, float (&f)[V]) {
+    if (left >= V) {
+      const Vec v = *reinterpret_cast<const Vec *>(x);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = (float)v.v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = i < left ? (float)x[i] : 0.0f;
+    }
+  }
+  static __device__ __forceinline__ void store(T *x, int64_t left, const float (&f)[V]) {
+    if (left >= V) {
+      Vec v;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v.v[i] = (T)f[i];
+      *reinterpret_cast<Vec *>(x) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < left) x[i] = (T)f[i];
+    }
+  }
+};
+
+// Y(:, places[s, t]) = w X(:, t): a token's row is read once and stored topk
+// times. Bound by those stores.
+template <class T>
+__global__ __launch_bounds__(256) void gather_kernel(RowsArgs p) {
+  typedef Lanes<T> L;
+  const int lanes = 1 << p.shift, lane = threadIdx.x & (lanes - 1);
+  const int64_t token = (int64_t)blockIdx.x * (256 >> p.shift) + (threadIdx.x >> p.shift);
+  if (token >= p.n) return;
+  const int64_t columns = p.n * p.topk;
+  const int32_t *places = p.places + token * p.topk;
+  const T *x = (const T *)p.X + token * p.ldx;
+  for (int64_t at = ((int64_t)blockIdx.y * lanes + lane) * L::V; at < p.d; at += (int64_t)gridDim.y * lanes * L::V) {
+    float f[L::V];
+    L::load(x + at, p.d - at, f);
+    for (int s = 0; s < p.topk; ++s) {
+      const int64_t place = places[s];
+      if (place < 0 || place >= columns) continue;
+      float g[L::V];
+      const float w = p.weights ? p.weights[token * p.topk + s] : 1.0f;
+#pragma unroll
+      for (int i = 0; i < L::V; ++i) g[i] = w * f[i];
+      L::store((T *)p.out + place * p.ldo + at, p.d - at, g);
+    }
+  }
+}
+
+// C(:, t) = sum over s of w Y(:, places[s, t]) + beta C(:, t), in the slots'
+// order, in fp32. Bound by reading Y.
+template <class T, class C>
+__global__ __launch_bounds__(256) void combine_kernel(RowsArgs p) {
+  typedef Lanes<T> L;
+  const int lanes = 1 << p.shift, lane = threadIdx.x & (lanes - 1);
+  const int64_t token = (int64_t)blockIdx.x * (256 >> p.shift) + (threadIdx.x >> p.shift);
+  if (token >= p.n) return;
+  const int64_t columns = p.n * p.topk;
+  const int32_t *places = p.places + token * p.topk;
+  C *c = (C *)p.out + token * p.ldo;
+  for (int64_t at = ((int64_t)blockIdx.y * lanes + lane) * L::V; at < p.d; at += (int64_t)gridDim.y * lanes * L::V) {
+    float sum[L::V];
+#pragma unroll
+    for (int i = 0; i < L::V; ++i) sum[i] = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < p.topk; ++s) {
+      const int64_t place = places[s];
+      if (place < 0 || place >= columns) continue;
+      float f[L::V];
+      L::load((const T *)p.Y + place * p.ldy + at, p.d - at, f);
+      const float w = p.weights ? p.weights[token * p.topk + s] : 1.0f;
+#pragma unroll
+      for (int i = 0; i < L::V; ++i) sum[i] = fmaf(w, f[i], sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < L::V; ++i)
+      if (at + i < p.d) c[at + i] = (C)(p.beta != 0.0f ? fmaf(p.beta, (float)c[at + i], sum[i]) : sum[i]);
+  }
+}
+
+// dY(:, places[s, t]) = w dC(:, t) and dw[s, t] = <Y(:, places[s, t]), dC(:,
+// t)>: 256 threads a token, eight slots at a time; their sums are folded in a
+// fixed order.
+template <class T>
+__global__ __launch_bounds__(256) void combine_grad_kernel(RowsArgs p) {
+  typedef Lanes<T> L;
+  constexpr int S = 8;
+  __shared__ float sums[4][S];
+  const int64_t token = blockIdx.x, columns = p.n * p.topk;
+  const int t = threadIdx.x;
+  const int32_t *places = p.places + token * p.topk;
+  const T *dc = (const T *)p.X + token * p.ldx;
+  for (int s0 = 0; s0 < p.topk; s0 += S) {
+    float dot[S], w[S];
+    int64_t place[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      dot[s] = 0.0f;
+      place[s] = s0 + s < p.topk ? places[s0 + s] : -1;
+      if (place[s] >= columns) place[s] = -1;
+      w[s] = place[s] >= 0 ? p.weights[token * p.topk + s0 + s] : 0.0f;
+    }
+    for (int64_t at = (int64_t)t * L::V; at < p.d; at += 256 * L::V) {
+      float f[L::V];
+      L::load(dc + at, p.d - at, f);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (place[s] < 0) continue;
+        float y[L::V], g[L::V];
+        L::load((const T *)p.Y + place[s] * p.ldy + at, p.d - at, y);
+#pragma unroll
+        for (int i = 0; i < L::V; ++i) {
+          dot[s] = fmaf(y[i], f[i], dot[s]);
+          g[i] = w[s] * f[i];
+        }
+        L::store((T *)p.out + place[s] * p.ldo + at, p.d - at, g);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float x = over_lanes<64>(dot[s], Sum());
+      if ((t & 63) == 0) sums[t >> 6][s] = x;
+    }
+    __syncthreads();
+    if (t < S && s0 + t < p.topk) p.dweights[token * p.topk + s0 + t] = (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
+    __syncthreads();
+  }
+}
+
+// Threads a token (2^shift, at most 256) and blocks along d for rows of d elements of `size` bytes.
+void row_shape(int64_t d, int64_t n, int size, int &shift, dim3 &grid) {
+  const int64_t vectors = (d * size + 15) / 16;
+  shift = 0;
+  while (shift < 8 && ((int64_t)1 << shift) < vectors) ++shift;
+  const int64_t along = (vectors + 255) / 256;
+  grid = dim3((unsigned)((n + (256 >> shift) - 1) / (256 >> shift)), (unsigned)(along < 65535 ? along : 65535));
+}
+
+// ---- checks ----------------------------------------------------------------------------
+
+int check_type(int type) {
+  if (type != WGB_F32 && type != WGB_F16 && type != WGB_BF16)
+    return fail(WGB_ERR_INVALID_VALUE, "type must be WGB_F32, WGB_F16 or WGB_BF16");
+  return WGB_OK;
+}
+
+int check_pairs(int64_t n, int64_t topk) {
+  if (n < 0) return fail(WGB_ERR_INVALID_VALUE, "n must be non-negative");
+  if (topk < 1 || topk > kMaxTopk) return fail(WGB_ERR_INVALID_VALUE, "topk must be between 1 and 64");
+  if (n > INT32_MAX / topk) return fail(WGB_ERR_INVALID_VALUE, "n * topk must be below 2^31");
+  return WGB_OK;
+}
+
+int check_choice(int64_t experts, int64_t n, int64_t topk) {
+  const int st = check_pairs(n, topk);
+  if (st) return st;
+  if (experts < 1 || experts > kMaxExperts) return fail(WGB_ERR_INVALID_VALUE, "experts must be between 1 and 1024");
+  if (topk > experts) return fail(WGB_ERR_INVALID_VALUE, "topk must be at most experts");
+  return WGB_OK;
+}
+
+int check_scoring(int scoring) {
+  if (scoring != WGB_SOFTMAX && scoring != WGB_SIGMOID)
+    return fail(WGB_ERR_INVALID_VALUE, "scoring must be WGB_SOFTMAX or WGB_SIGMOID");
+  return WGB_OK;
+}
+
+int check_rows(int type, int64_t d, int64_t n, int64_t topk) {
+  int st = check_type(type);
+  if (!st) st = check_pairs(n, topk);
+  if (st) return st;
+  if (d < 0 || d > INT32_MAX) return fail(WGB_ERR_INVALID_VALUE, "d must be non-negative and below 2^31");
+  return WGB_OK;
+}
+
+int check_ld(int64_t ld, int64_t rows, const char *what) {
+  if (ld < (rows > 1 ? rows : 1))
+    return fail(WGB_ERR_INVALID_VALUE, std::string(what) + " must be at least the column's length and 1");
+  return WGB_OK;
+}
+
+}  // namespace
+
+extern "C" int wgb_route(wgb_ctx *ctx, int type, int scoring, int64_t experts, int64_t n, int64_t topk,
+                         const void *logits, int64_t ldl, const float *bias, int64_t groups, int64_t top_groups, int best,
+                         int renorm, float scale, int32_t *ids, float *weights) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_type(type)) || (st = check_scoring(scoring)) || (st = check_choice(experts, n, topk)) ||
+      (st = check_ld(ldl, experts, "ldl")))
+    return st;
+  if (groups < 1 || groups > kMaxGroups || experts % groups != 0)
+    return fail(WGB_ERR_INVALID_VALUE, "groups must be between 1 and 64 and divide experts");
+  if (top_groups < 1 || top_groups > groups)
+    return fail(WGB_ERR_INVALID_VALUE, "top_groups must be between 1 and groups");
+  if (best != 1 && best != 2) return fail(WGB_ERR_INVALID_VALUE, "best must be 1 or 2");
+  if (topk > experts / groups * top_groups)
+    return fail(WGB_ERR_INVALID_VALUE, "topk must be at most the experts of top_groups groups");
+  if (n == 0) return WGB_OK;
+  if (!logits || !ids || !weights) return fail(WGB_ERR_INVALID_VALUE, "logits, ids or weights is null");
+  RouteArgs p = {};
+  p.logits = logits;
+  p.ldl = ldl;
+  p.n = n;
+  p.bias = bias;
+  p.experts = (int)experts;
+  p.topk = (int)topk;
+  p.groups = top_groups == groups ? 1 : (int)groups;  // all kept: as none
+  p.top_groups = (int)top_groups;
+  p.best = best;
+  p.per = (int)(experts / groups);
+  p.magic = ((1u << 20) + p.per - 1) / p.per;
+  p.sigmoid = scoring == WGB_SIGMOID;
+  p.renorm = renorm != 0;
+  p.scale = scale;
+  p.ids = ids;
+  p.weights = weights;
+  wgb::timing_begin(ctx);
+  st = type == WGB_F32 ? route<float>(ctx, p) : type == WGB_F16 ? route<_Float16>(ctx, p) : route<__bf16>(ctx, p);
+  wgb::timing_end(ctx);
+  return st;
+}
+
+extern "C" int wgb_route_grad(wgb_ctx *ctx, int type, int scoring, int64_t experts, int64_t n, int64_t topk,
+                              const void *logits, int64_t ldl, const int32_t *ids, int renorm, float scale,
+                              const float *dweights, void *dlogits, int64_t ldd) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_type(type)) || (st = check_scoring(scoring)) || (st = check_choice(experts, n, topk)) ||
+      (st = check_ld(ldl, experts, "ldl")) || (st = check_ld(ldd, experts, "ldd")))
+    return st;
+  if (n == 0) return WGB_OK;
+  if (!logits || !ids || !dweights || !dlogits)
+    return fail(WGB_ERR_INVALID_VALUE, "logits, ids, dweights or dlogits is null");
+  GradArgs p = {logits, ldl, n, ids, dweights, dlogits, ldd, (int)experts, (int)topk, scoring == WGB_SIGMOID, renorm != 0,
+                scale};
+  wgb::timing_begin(ctx);
+  st = type == WGB_F32 ? grad<float>(ctx, p) : type == WGB_F16 ? grad<_Float16>(ctx, p) : grad<__bf16>(ctx, p);
+  wgb::timing_end(ctx);
+  return st;
+}
+
+extern "C" int wgb_route_order(wgb_ctx *ctx, int64_t experts, int64_t n, int64_t topk, const int32_t *ids,
+                               int64_t *d_offsets, int32_t *places, int32_t *pairs) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_choice(experts, n, topk))) return st;
+  if (!d_offsets) return fail(WGB_ERR_INVALID_VALUE, "d_offsets is null");
+  if (n > 0 && (!ids || !places || !pairs)) return fail(WGB_ERR_INVALID_VALUE, "ids, places or pairs is null");
+  const int64_t count = n * topk;
+  int bits = 0;
+  while ((1 << bits) < experts) ++bits;
+  // at most 256 blocks, each of whole rounds of 1024 pairs
+  int64_t chunk = (count + 255) / 256;
+  chunk = (chunk + 1023) / 1024 * 1024;
+  const int blocks = count > 1024 ? (int)((count + chunk - 1) / chunk) : 1;
+  int threads = 1024;
+  while (blocks == 1 && threads > 64 && threads / 2 >= count && threads / 2 >= experts) threads /= 2;
+  if (blocks == 1) chunk = count;
+  if (blocks > 1 && (st = wgb::ensure_op_workspace(ctx, (size_t)blocks * experts * 4))) return st;
+  wgb::timing_begin(ctx);
+  if (blocks > 1) {
+    order_count_kernel<<<blocks, 1024, 0, ctx->stream>>>(ids, count, chunk, (int)experts, (int32_t *)ctx->op_ws);
+  }
+  order_place_kernel<<<blocks, threads, 0, ctx->stream>>>(ids, count, chunk, (int)experts, bits, (const int32_t *)ctx->op_ws,
+                                                          blocks, d_offsets, places, pairs);
+  wgb::timing_end(ctx);
+  WGB_CHECK_LAUNCH("order_place_kernel");
+  return WGB_OK;
+}
+
+extern "C" int wgb_route_gather(wgb_ctx *ctx, int type, int64_t d, int64_t n, int64_t topk, const void *X, int64_t ldx,
+                                const int32_t *places, const float *weights, void *Y, int64_t ldy) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_rows(type, d, n, topk)) || (st = check_ld(ldx, d, "ldx")) || (st = check_ld(ldy, d, "ldy"))) return st;
+  if (n == 0 || d == 0) return WGB_OK;
+  if (!X || !places || !Y) return fail(WGB_ERR_INVALID_VALUE, "X, places or Y is null");
+  RowsArgs p = {};
+  p.d = d;
+  p.n = n;
+  p.topk = (int)topk;
+  p.X = X;
+  p.ldx = ldx;
+  p.places = places;
+  p.weights = weights;
+  p.out = Y;
+  p.ldo = ldy;
+  dim3 grid;
+  row_shape(d, n, type == WGB_F32 ? 4 : 2, p.shift, grid);
+  wgb::timing_begin(ctx);
+  if (type == WGB_F32)
+    gather_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
+  else if (type == WGB_F16)
+    gather_kernel<_Float16><<<grid, 256, 0, ctx->stream>>>(p);
+  else
+    gather_kernel<__bf16><<<grid, 256, 0, ctx->stream>>>(p);
+  wgb::timing_end(ctx);
+  WGB_CHECK_LAUNCH("gather_kernel");
+  return WGB_OK;
+}
+
+extern "C" int wgb_route_combine(wgb_ctx *ctx, int type, int64_t d, int64_t n, int64_t topk, const void *Y, int64_t ldy,
+                                 const int32_t *places, const float *weights, float beta, void *C, int64_t ldc,
+                                 int ctype) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_rows(type, d, n, topk)) || (st = check_ld(ldy, d, "ldy")) || (st = check_ld(ldc, d, "ldc"))) return st;
+  if (ctype != type && ctype != WGB_F32)
+    return fail(WGB_ERR_INVALID_VALUE, "the type of C must be Y's type or WGB_F32");
+  if (n == 0 || d == 0) return WGB_OK;
+  if (!Y || !places || !C) return fail(WGB_ERR_INVALID_VALUE, "Y, places or C is null");
+  RowsArgs p = {};
+  p.d = d;
+  p.n = n;
+  p.topk = (int)topk;
+  p.Y = Y;
+  p.ldy = ldy;
+  p.places = places;
+  p.weights = weights;
+  p.beta = beta;
+  p.out = C;
+  p.ldo = ldc;
+  dim3 grid;
+  row_shape(d, n, type == WGB_F32 ? 4 : 2, p.shift, grid);
+  wgb::timing_begin(ctx);
+  if (type == WGB_F32)
+    combine_kernel<float, float><<<grid, 256, 0, ctx->stream>>>(p);
+  else if (type == WGB_F16 && ctype == WGB_F16)
+    combine_kernel<_Float16, _Float16><<<grid, 256, 0, ctx->stream>>>(p);
+  else if (type == WGB_F16)
+    combine_kernel<_Float16, float><<<grid, 256, 0, ctx->stream>>>(p);
+  else if (ctype == WGB_BF16)
+    combine_kernel<__bf16, __bf16><<<grid, 256, 0, ctx->stream>>>(p);
+  else
+    combine_kernel<__bf16, float><<<grid, 256, 0, ctx->stream>>>(p);
+  wgb::timing_end(ctx);
+  WGB_CHECK_LAUNCH("combine_kernel");
+  return WGB_OK;
+}
+
+extern "C" int wgb_route_combine_grad(wgb_ctx *ctx, int type, int64_t d, int64_t n, int64_t topk, const void *dC,
+                                      int64_t lddc, const void *Y, int64_t ldy, const int32_t *places,
+                                      const float *weights, void *dY, int64_t lddy, float *dweights) {
+  int st = wgb::enter(ctx);
+  if (st) return st;
+  if ((st = check_rows(type, d, n, topk)) || (st = check_ld(lddc, d, "lddc")) || (st = check_ld(ldy, d, "ldy")) ||
+      (st = check_ld(lddy, d, "lddy")))
+    return st;
+  if (n == 0) return WGB_OK;
+  if (!places || !weights || !dweights) return fail(WGB_ERR_INVALID_VALUE, "places, weights or dweights is null");
+  if (d > 0 && (!dC || !Y || !dY)) return fail(WGB_ERR_INVALID_VALUE, "dC, Y or dY is null");
+  RowsArgs p = {};
+  p.d = d;
+  p.n = n;
+  p.topk = (int)topk;
+  p.X = dC;
+  p.ldx = lddc;
+  p.Y = Y;
+  p.ldy = ldy;
+  p.places = places;
+  p.weights = weights;
+  p.out = dY;
+  p.ldo = lddy;
+  p.dweights = dweights;
+  wgb::timing_begin(ctx);
+  if (type == WGB_F32)
+    combine_grad_kernel<float><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
+  else if (type == WGB_F16)
+    combine_grad_kernel<_Float16><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
+  else
+    combine_grad_kernel<__bf16><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
+  wgb::timing_end(ctx);
+  WGB_CHECK_LAUNCH("combine_grad_kernel");
+  return WGB_OK;
+}

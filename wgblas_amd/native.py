@@ -19,6 +19,7 @@ LOWER, UPPER = 1, 2
 LEFT, RIGHT = 1, 2
 NON_UNIT, UNIT = 0, 1
 F32, F16, BF16 = 0, 1, 2
+SOFTMAX, SIGMOID = 0, 1
 
 _i64 = C.c_int64
 _ptr = C.c_void_p
@@ -82,6 +83,19 @@ _SIGNATURES = {
                        _i64, C.c_int],
     "wgb_mxfp4_gemm_grouped": [_ptr, _i64, _i64, _i64, _i64, C.c_float, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64,
                                _ptr, C.c_float, _ptr, _i64, C.c_int],
+    "wgb_fp8_quantize": [_ptr, C.c_int, C.c_int, C.c_int, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64],
+    "wgb_fp8_dequantize": [_ptr, C.c_int, C.c_int, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64],
+    "wgb_fp8_gemm": [_ptr, C.c_int, _i64, _i64, _i64, C.c_float, _ptr, _i64, C.c_int, _ptr, _i64, _ptr, _i64, _ptr,
+                     _i64, C.c_float, _ptr, _i64, C.c_int],
+    "wgb_fp8_gemm_grouped": [_ptr, C.c_int, _i64, _i64, _i64, _i64, C.c_float, _ptr, _i64, _i64, C.c_int, _ptr, _i64,
+                             _i64, _ptr, _i64, _ptr, _i64, _ptr, C.c_float, _ptr, _i64, C.c_int],
+    "wgb_route": [_ptr, C.c_int, C.c_int, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, C.c_int, C.c_int, C.c_float,
+                  _ptr, _ptr],
+    "wgb_route_grad": [_ptr, C.c_int, C.c_int, _i64, _i64, _i64, _ptr, _i64, _ptr, C.c_int, C.c_float, _ptr, _ptr, _i64],
+    "wgb_route_order": [_ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr],
+    "wgb_route_gather": [_ptr, C.c_int, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64],
+    "wgb_route_combine": [_ptr, C.c_int, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, C.c_float, _ptr, _i64, C.c_int],
+    "wgb_route_combine_grad": [_ptr, C.c_int, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _ptr],
     "wgb_sgemv": [_ptr, C.c_int, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, C.c_float, _ptr,
                   _i64],
     "wgb_sger": [_ptr, _i64, _i64, C.c_float, _ptr, _i64, _ptr, _i64, _ptr, _i64],
@@ -381,6 +395,61 @@ class Context:
         _check(self.lib.wgb_mxfp4_gemm_grouped(self.handle, groups, m, n, k, alpha, _p(A), _p(scaleA), lda, strideA,
                                                _p(B), _p(scaleB), ldb, _p(offsets), beta, _p(C_), ldc, ctype),
                "wgb_mxfp4_gemm_grouped")
+
+    # ---- FP8 (ld in codes, a multiple of 128; the scale of rows 128 b .. and columns block * c .. at scales[b * lds + c]) ----
+    def fp8_quantize(self, type, trans, block, k, n, X, ldx, codes, ld, scales, lds):
+        """X (k x n, or n x k with trans) to 8-bit codes with a scale for each 128 x block values."""
+        _check(self.lib.wgb_fp8_quantize(self.handle, type, trans, block, k, n, _p(X), ldx, _p(codes), ld, _p(scales), lds),
+               "wgb_fp8_quantize")
+
+    def fp8_dequantize(self, type, block, k, n, codes, ld, scales, lds, X, ldx):
+        """The k x n values that codes and scales stand for."""
+        _check(self.lib.wgb_fp8_dequantize(self.handle, type, block, k, n, _p(codes), ld, _p(scales), lds, _p(X), ldx),
+               "wgb_fp8_dequantize")
+
+    def fp8_gemm(self, transA, m, n, k, alpha, A, lda, blockA, scaleA, ldsa, B, ldb, scaleB, ldsb, beta, C_, ldc, ctype):
+        """C = alpha op(A) B + beta C, A (k x m with TRANS, else m x k) and B (k x n) in FP8."""
+        _check(self.lib.wgb_fp8_gemm(self.handle, transA, m, n, k, alpha, _p(A), lda, blockA, _p(scaleA), ldsa, _p(B), ldb,
+                                     _p(scaleB), ldsb, beta, _p(C_), ldc, ctype), "wgb_fp8_gemm")
+
+    def fp8_gemm_grouped(self, transA, groups, m, n, k, alpha, A, lda, strideA, blockA, scaleA, ldsa, strideScaleA, B, ldb,
+                         scaleB, ldsb, offsets, beta, C_, ldc, ctype):
+        """C(:, j) = alpha op(A_g) B(:, j) + beta C(:, j) for the columns j of each group g, A_g and B in FP8."""
+        _check(self.lib.wgb_fp8_gemm_grouped(self.handle, transA, groups, m, n, k, alpha, _p(A), lda, strideA, blockA,
+                                             _p(scaleA), ldsa, strideScaleA, _p(B), ldb, _p(scaleB), ldsb, _p(offsets),
+                                             beta, _p(C_), ldc, ctype), "wgb_fp8_gemm_grouped")
+
+    # ---- routing (ids, weights, places: topk values a token) ----
+    def route(self, type, scoring, experts, n, topk, logits, ldl, bias, groups, top_groups, best, renorm, scale, ids,
+              weights):
+        """Each token's experts and their weights from the router's logits (experts x n)."""
+        _check(self.lib.wgb_route(self.handle, type, scoring, experts, n, topk, _p(logits), ldl, _p(bias), groups,
+                                  top_groups, best, renorm, scale, _p(ids), _p(weights)), "wgb_route")
+
+    def route_grad(self, type, scoring, experts, n, topk, logits, ldl, ids, renorm, scale, dweights, dlogits, ldd):
+        """The logits' gradient from the weights'."""
+        _check(self.lib.wgb_route_grad(self.handle, type, scoring, experts, n, topk, _p(logits), ldl, _p(ids), renorm,
+                                       scale, _p(dweights), _p(dlogits), ldd), "wgb_route_grad")
+
+    def route_order(self, experts, n, topk, ids, offsets, places, pairs):
+        """The order of the pairs (token, expert) by expert: boundaries, each pair's column, each column's pair."""
+        _check(self.lib.wgb_route_order(self.handle, experts, n, topk, _p(ids), _p(offsets), _p(places), _p(pairs)),
+               "wgb_route_order")
+
+    def route_gather(self, type, d, n, topk, X, ldx, places, weights, Y, ldy):
+        """Y(:, places[s, t]) = w X(:, t)."""
+        _check(self.lib.wgb_route_gather(self.handle, type, d, n, topk, _p(X), ldx, _p(places), _p(weights), _p(Y), ldy),
+               "wgb_route_gather")
+
+    def route_combine(self, type, d, n, topk, Y, ldy, places, weights, beta, C_, ldc, ctype=None):
+        """C(:, t) = sum over s of w Y(:, places[s, t]) + beta C(:, t)."""
+        _check(self.lib.wgb_route_combine(self.handle, type, d, n, topk, _p(Y), ldy, _p(places), _p(weights), beta, _p(C_),
+                                          ldc, type if ctype is None else ctype), "wgb_route_combine")
+
+    def route_combine_grad(self, type, d, n, topk, dC, lddc, Y, ldy, places, weights, dY, lddy, dweights):
+        """dY(:, places[s, t]) = w dC(:, t) and dw[s, t] = <Y(:, places[s, t]), dC(:, t)>."""
+        _check(self.lib.wgb_route_combine_grad(self.handle, type, d, n, topk, _p(dC), lddc, _p(Y), ldy, _p(places),
+                                               _p(weights), _p(dY), lddy, _p(dweights)), "wgb_route_combine_grad")
 
     # ---- level 2 ----
     def sgemv(self, trans, m, n, alpha, A, lda, x, incx, beta, y, incy):
