@@ -293,6 +293,8 @@ int product(wgb_ctx *ctx, Args &p) {
   const int64_t mean = p.n / p.groups;
   if (mean <= 32) return launch_columns<Fp8Kernel<128, 32, 4, 1, AMC, ROWS, EXACT, 4>>(ctx, p);
   const int64_t tiles = (p.m + 127) / 128 * ((p.n + 127) / 128);
+  if (tiles >= 4 * ctx->num_cus)
+    return launch_columns_rounds<Fp8Large<AMC, ROWS, EXACT>, Fp8Kernel<128, 128, 2, 2, AMC, ROWS, EXACT, 2>>(ctx, p);
   if (tiles >= ctx->num_cus) return launch_columns<Fp8Kernel<128, 128, 2, 2, AMC, ROWS, EXACT, 2>>(ctx, p);
   return launch_columns<Fp8Kernel<64, 64, 2, 2, AMC, ROWS, EXACT, 2>>(ctx, p);
 }
@@ -331,7 +333,8 @@ int run_product(wgb_ctx *ctx, int transA, int64_t groups, int64_t m, int64_t n, 
   Args p = {};
   p.m = m;
   p.n = n;
-  p.k = k;
+  p.k = blocks128(k) * 128;
+  p.a_depth = k;
   p.A = (const char *)A;
   p.B = (const char *)B;
   p.lda = lda;
@@ -344,7 +347,7 @@ int run_product(wgb_ctx *ctx, int transA, int64_t groups, int64_t m, int64_t n, 
   p.a_k = amc ? 1 : ldsa;
   p.a_group = strideScaleA;
   p.b_k = ldsb;
-  p.block_a = blockA;
+  p.a_shift = blockA == 128 ? 7 : 0;
   p.off = grouped ? d_offsets : nullptr;
   p.groups = (int)groups;
   p.C = C;

@@ -68,6 +68,14 @@ struct Codes<true> {
   }
 };
 
+// 8 bytes of k of this lane's row. A pointer of its own, as far as the compiler
+// is told: it would wait for all copies to LDS that are under way otherwise,
+// and those are waited for where their k-tiles are due.
+typedef int v2i __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ v2i read_transposed(const char *__restrict__ at) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i *)at);
+}
+
 // The MFMA operands of a k-tile for MB blocks of 16 rows, `STEP` rows apart,
 // from row `wrow`; only the first `used` blocks.
 template <int BT, bool MC, int MB, int STEP = 16>
@@ -83,8 +91,6 @@ __device__ __forceinline__ void fetch_codes(const char *stage, int wrow, int lan
         out[b] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       }
   } else {
-    typedef int v2i __attribute__((ext_vector_type(2)));
-    typedef __attribute__((address_space(3))) v2i *LdsV2;
     const int kr = 16 * g + (i16 >> 1);
     int at = kr * BT + ((wrow ^ (mc_key<8, BT / 16>(kr) << 4)) + (i16 & 1) * 8);
     asm volatile("" : "+v"(at));  // one register, not one for every block
@@ -93,7 +99,7 @@ __device__ __forceinline__ void fetch_codes(const char *stage, int wrow, int lan
       if (b > 0 && __builtin_expect(b >= used, 0)) break;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsV2)(stage + (at ^ (STEP * b)) + (64 * (q >> 1) + 8 * (q & 1)) * BT));
+        const v2i x = read_transposed(stage + (at ^ (STEP * b)) + (64 * (q >> 1) + 8 * (q & 1)) * BT);
         out[b][2 * q] = x[0];
         out[b][2 * q + 1] = x[1];
       }
@@ -129,9 +135,9 @@ struct BlockScaleStager {
         if (row >= p.m) row = p.m - 1;
         src[r] = p.block_scale_a + g * p.a_group;
         step[r] = p.a_k;
-        const int64_t first_row = m0 / p.block_a;
+        const int64_t first_row = m0 >> p.a_shift;
         src[r] += first_row * p.a_row;
-        voff[r] = (uint32_t)((row / p.block_a - first_row) * p.a_row * 4);
+        voff[r] = (uint32_t)(((row >> p.a_shift) - first_row) * p.a_row * 4);
       } else {
         int64_t col = c * 64 - BM + lane;
         if (col >= n_left) col = n_left - 1;
@@ -148,25 +154,41 @@ struct BlockScaleStager {
   }
 };
 
-// Products of a lane's blocks added to the sums. ROWS: A has a scale for each
-// row (sa[i]: of the lane's four rows of block i), else one for all (sa[0][0]).
-template <bool EXACT, bool ROWS, int MB, int NB>
-__device__ __forceinline__ void multiply_codes(const v8i (&a)[MB], const v8i (&b)[NB], f4 (&acc)[MB][NB], const f4 (&sa)[ROWS ? MB : 1],
-                                               const float (&sb)[NB]) {
+// The products of some row blocks with all column blocks, added to the sums.
+// sb: the columns' scales; ROWS: A has a scale for each row (sa[i]: of the
+// lane's four rows of block i), else the one for all is in sb. A block's products are scaled while the next
+// ones are multiplied: the scheduler, left to itself, puts the v_fma right
+// behind its MFMA and waits for it. FULL: all column blocks are used.
+template <bool EXACT, bool ROWS, int MB, int NB, int FIRST, int COUNT, bool FULL = true>
+__device__ __forceinline__ void multiply_codes(const v8i (&a)[COUNT], const typename Codes<EXACT>::wide (&b)[NB],
+                                               f4 (&acc)[MB][NB], const f4 (&sa)[ROWS ? COUNT : 1], const float (&sb)[NB],
+                                               int used = NB) {
   typedef Codes<EXACT> X;
-  typename X::wide wa[MB];
+  constexpr int LAG = EXACT ? 1 : 2;
+  f4 late[LAG + 1];
+  auto add = [&](int i, int j, const f4 &x) {
 #pragma unroll
-  for (int i = 0; i < MB; ++i) wa[i] = X::widen(a[i]);
+    for (int q = 0; q < 4; ++q) acc[FIRST + i][j][q] = fmaf(x[q], ROWS ? sa[i][q] * sb[j] : sb[j], acc[FIRST + i][j][q]);
+  };
+  if constexpr (FULL) {
+    typename X::wide w;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const typename X::wide wb = X::widen(b[j]);
-    const float s = sa[0][0] * sb[j];
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const f4 x = X::dot(wa[i], wb);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(x[q], ROWS ? sa[i][q] * sb[j] : s, acc[i][j][q]);
+    for (int n = 0; n < COUNT * NB + LAG; ++n) {
+      if (n < COUNT * NB) {
+        if (n % NB == 0) w = X::widen(a[n / NB]);
+        late[n % (LAG + 1)] = X::dot(w, b[n % NB]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const int m = n - LAG;
+      if (m >= 0) add(m / NB, m % NB, late[m % (LAG + 1)]);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (j == 0 || j < used)
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) add(i, j, X::dot(X::widen(a[i]), b[j]));
   }
 }
 
@@ -210,7 +232,7 @@ struct Fp8Kernel {
       for (int j = 0; j < NB; ++j) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
     // alpha == 0 reads neither operand
-    int nt = p.alpha == 0.0f ? 0 : (int)((p.k + TB - 1) / TB), first = 0;
+    int nt = p.alpha == 0.0f ? 0 : (int)(p.k / TB), first = 0;
     if (REST && quarter.pieces > 1) {
       const int most = (nt + quarter.pieces - 1) / quarter.pieces;
       first = quarter.piece * most;
@@ -220,10 +242,9 @@ struct Fp8Kernel {
       SA sa;
       SB sb;
       SS ss;
-      // columns of 8-bit matrices are whole runs of 128; only A's k-rows (MC) end at k itself
-      const int64_t depth = p.k - (int64_t)first * TB;
-      sa.init(p.A + (int64_t)tile.g * p.stride_a, p.lda, m0, AMC ? p.a_rows : p.m, AMC ? depth : (int64_t)TB * nt, t);
-      sb.init(p.B + tile.lo * p.ldb, p.ldb, n0, cols, (int64_t)TB * nt, t);
+      const int64_t depth = (AMC ? p.a_depth : p.k) - (int64_t)first * TB;
+      sa.init(p.A + (int64_t)tile.g * p.stride_a, p.lda, m0, AMC ? p.a_rows : p.m, depth, t);
+      sb.init(p.B + tile.lo * p.ldb, p.ldb, n0, cols, p.k - (int64_t)first * TB, t);
       sa.origin += first * sa.step();
       sb.origin += first * sb.step();
       ss.init(p, tile.g, m0, tile.lo + n0, cols - n0, first, wave, lane);
@@ -248,55 +269,57 @@ struct Fp8Kernel {
         sb.copy(st + SA::BYTES, kt, wave);
         ss.copy(st + SA::BYTES + SB::BYTES, kt);
       };
-      struct Operands {
-        v8i a[MB], b[NB];
-        f4 sa[ROWS ? MB : 1];
-        float sb[NB];
-      };
-      auto fetch = [&](int kt, Operands &o) {
-        const char *st = smem + (kt % S) * STAGE;
-        fetch_codes<BM, AMC, MB>(st, wm, lane, o.a);
-        fetch_codes<BN, false, NB>(st + SA::BYTES, wn, lane, o.b);
+      // the row blocks in PARTS, each read while the one before is multiplied
+      constexpr int PARTS = MB % 2 == 0 ? 2 : 1, PB = MB / PARTS;
+      v8i a[PARTS][PB], b[NB];
+      f4 scale_a[PARTS][ROWS ? PB : 1];
+      float scale_b[NB];
+      auto fetch_a = [&](const char *st, int part) {
+        fetch_codes<BM, AMC, PB>(st, wm + 16 * PB * part, lane, a[part]);
         const float *scales = reinterpret_cast<const float *>(st + SA::BYTES + SB::BYTES);
         if constexpr (ROWS) {
 #pragma unroll
-          for (int i = 0; i < MB; ++i) o.sa[i] = *reinterpret_cast<const f4 *>(scales + wm + 16 * i + 4 * (lane >> 4));
-        } else {
-          o.sa[0][0] = scales[wm];
+          for (int i = 0; i < PB; ++i)
+            scale_a[part][i] = *reinterpret_cast<const f4 *>(scales + wm + 16 * (PB * part + i) + 4 * (lane >> 4));
         }
-#pragma unroll
-        for (int j = 0; j < NB; ++j) o.sb[j] = scales[BM + wn + 16 * j + (lane & 15)];
       };
-      auto multiply = [&](const Operands &o) { multiply_codes<EXACT, ROWS>(o.a, o.b, acc, o.sa, o.sb); };
+      auto fetch_b = [&](const char *st) {
+        fetch_codes<BN, false, NB>(st + SA::BYTES, wn, lane, b);
+        const float *scales = reinterpret_cast<const float *>(st + SA::BYTES + SB::BYTES);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) scale_b[j] = scales[BM + wn + 16 * j + (lane & 15)];
+        if constexpr (!ROWS) {
+          const float rows = scales[wm];
+#pragma unroll
+          for (int j = 0; j < NB; ++j) scale_b[j] *= rows;
+        }
+      };
 
       // Tile kt is read from stage kt % S while the copies of the next S - 1
       // are in flight or landed; its stage takes tile kt + S after the barrier
-      // that ends its reads, and its products run behind that barrier.
+      // that ends its reads.
 #pragma unroll
       for (int i = 0; i < S; ++i)
         if (i < nt) fill(i);
       wait_barrier<0>();
-      Operands x, y;
-      fetch(0, x);
-      int kt = 0;
-      // steady: two tiles a turn while tiles kt + S and kt + 1 + S are whole
-      const int steady = whole - S - 1;
-      for (; kt < steady; kt += 2) {
-        wait_barrier<(S - 2) * PER_TILE>();
-        copy(kt + S);
-        fetch(kt + 1, y);
-        multiply(x);
-        wait_barrier<(S - 2) * PER_TILE>();
-        copy(kt + 1 + S);
-        fetch(kt + 2, x);
-        multiply(y);
-      }
-      for (; kt < nt; ++kt) {
-        wait_barrier<0>();
-        if (kt + S < nt) fill(kt + S);
-        if (kt + 1 < nt) fetch(kt + 1, y);
-        multiply(x);
-        if (kt + 1 < nt) x = y;
+      const int steady = whole - S;  // tile kt + S exists and is whole
+      for (int kt = 0; kt < nt; ++kt) {
+        const char *st = smem + (kt % S) * STAGE;
+        fetch_b(st);
+        fetch_a(st, 0);
+        typename Codes<EXACT>::wide wb[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) wb[j] = Codes<EXACT>::widen(b[j]);
+        if constexpr (PARTS == 2) fetch_a(st, 1);
+        multiply_codes<EXACT, ROWS, MB, NB, 0, PB>(a[0], wb, acc, scale_a[0], scale_b);
+        if (kt < steady) {
+          wait_barrier<(S - 2) * PER_TILE>();
+          copy(kt + S);
+        } else {
+          wait_barrier<0>();
+          if (kt + S < nt) fill(kt + S);
+        }
+        if constexpr (PARTS == 2) multiply_codes<EXACT, ROWS, MB, NB, PB, PB>(a[1], wb, acc, scale_a[1], scale_b);
       }
     }
 
@@ -309,6 +332,263 @@ struct Fp8Kernel {
       return;
     }
     store_tile<Fp8, 16>(p, tile.lo * p.ldc, acc, m0 + wm, n0 + wn, cols, lane);
+  }
+};
+
+// The 256 x 256 tile of the large products: 8 waves of 128 x 64 each, two on
+// every SIMD. Their v_fma and LDS reads fill the time of each other's MFMAs, so
+// nothing orders them but one barrier a k-tile (taking turns, as the 16-bit
+// TurnKernel does, leaves a wave alone with its v_fma: 50 cycles an MFMA, not
+// 32). A k-tile's row blocks are multiplied in PARTS; a part is read while the
+// one before is multiplied. When the last part has been read, the barrier, which
+// also ends the wait for the next k-tile's copies, frees the stage: the next
+// k-tile's columns are read block by block into the registers that the last
+// part's products leave, and the copies of the k-tile after that start. They
+// are issued one by one between MFMAs, A's in the last part, B's in the next
+// k-tile's first one: issued together, 64 KB took all waves 1000 to 1500
+// cycles, at 64 bytes a cycle and CU, with no MFMA running.
+// A block runs through tiles (w, w + blocks, ...). The next tile's first copies
+// are issued before a tile is stored, when its operands' registers are free: in
+// the midst of a tile they would have to be spilled, and each return of one
+// waits for all copies and stores under way.
+template <bool AMC, bool ROWS, bool EXACT>
+struct Fp8Large {
+  static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
+  static constexpr int kBM = BM, kBN = BN;
+  static constexpr int NW = WM * WN, NT = 64 * NW;
+  static constexpr int MB = BM / WM / 16, NB = BN / WN / 16, STEP = 16 * WN;
+  static constexpr int PB = EXACT ? 1 : 2, PARTS = MB / PB;
+  typedef Codes<EXACT> X;
+  typedef Stager<Fp8, BM, AMC, NT> SA;
+  typedef Stager<Fp8, BN, false, NT> SB;
+  typedef BlockScaleStager<BM, BN, NW> SS;
+  typedef TileTable<ColumnOrder> Table;
+  static constexpr int STAGE = SA::BYTES + SB::BYTES + SS::BYTES;
+  static constexpr int LDS = 2 * STAGE;
+  static constexpr int COPIES_B = SB::LOADS + SS::LOADS;
+  static_assert(SB::RPS == STEP, "a load is STEP columns");
+
+  // The copies of a tile's k-tiles: of A, and of B with the scales.
+  struct Copies {
+    SA sa;
+    SB sb;
+    SS ss;
+
+    __device__ __forceinline__ void init(const Args &p, const Tile &tile, int t) {
+      const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * BN, cols = tile.hi - tile.lo;
+      sa.init(p.A + (int64_t)tile.g * p.stride_a, p.lda, m0, AMC ? p.a_rows : p.m, AMC ? p.a_depth : p.k, t);
+      sb.init(p.B + tile.lo * p.ldb, p.ldb, n0, cols, p.k, t);
+      ss.init(p, tile.g, m0, tile.lo + n0, cols - n0, 0, __builtin_amdgcn_readfirstlane(t >> 6), t & 63);
+    }
+    __device__ __forceinline__ char *stage_of(char *smem, int kt) const { return smem + (kt & 1) * STAGE; }
+    __device__ __forceinline__ void a(char *smem, int wave, int kt, int r) const {
+      copy_chunks(sa.origin + kt * sa.step(), sa.voff[r], stage_of(smem, kt) + wave * 1024 + r * NT * 16);
+    }
+    __device__ __forceinline__ void b(char *smem, int wave, int kt, int r) const {
+      char *st = stage_of(smem, kt) + SA::BYTES;
+      if (r < SB::LOADS)
+        copy_chunks(sb.origin + (int64_t)kt * TB, sb.voff[r], st + wave * 1024 + r * NT * 16);
+      else
+        ss.copy(st + SB::BYTES, kt);
+    }
+    // All of A of any k-tile: k-rows past k read the k-tile's first one again, B's codes there are zeros.
+    __device__ __forceinline__ void all_a(char *smem, int wave, int kt) const {
+      const bool cut = AMC && kt >= sa.whole_tiles();
+#pragma unroll
+      for (int r = 0; r < SA::LOADS; ++r)
+        copy_chunks(sa.origin + kt * sa.step(), cut ? sa.tail_voff(r) : sa.voff[r],
+                    stage_of(smem, kt) + wave * 1024 + r * NT * 16);
+    }
+    __device__ __forceinline__ void all_b(char *smem, int wave, int kt) const {
+#pragma unroll
+      for (int r = 0; r < COPIES_B; ++r) b(smem, wave, kt, r);
+    }
+  };
+
+  // What a wave multiplies.
+  struct Operands {
+    v8i a[2][PB];  // the part that is multiplied and the next one
+    f4 rows[2][ROWS ? PB : 1];
+    v8i raw[NB];   // the next k-tile's columns and scales
+    float next_a, next_b[NB];
+
+    template <int P>
+    __device__ __forceinline__ void fetch_a(const char *st, int wm, int lane) {
+      fetch_codes<BM, AMC, PB>(st, wm + 16 * PB * P, lane, a[P & 1]);
+      if constexpr (ROWS) {
+        const float *s = reinterpret_cast<const float *>(st + SA::BYTES + SB::BYTES);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) rows[P & 1][i] = *reinterpret_cast<const f4 *>(s + wm + 16 * (PB * P + i) + 4 * (lane >> 4));
+      }
+    }
+    __device__ __forceinline__ void fetch_b(const char *st, int wn, int lane, int j) {
+      v8i one[1];
+      fetch_codes<BN, false, 1>(st + SA::BYTES, wn + STEP * j, lane, one);
+      raw[j] = one[0];
+    }
+    __device__ __forceinline__ void fetch_scales(const char *st, int wm, int wn, int lane) {
+      const float *s = reinterpret_cast<const float *>(st + SA::BYTES + SB::BYTES);
+      if constexpr (!ROWS) next_a = s[wm];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) next_b[j] = s[BM + wn + STEP * j + (lane & 15)];
+    }
+  };
+
+  static __device__ __forceinline__ void run(const Args &p, char *smem) {
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * 16;
+    const int depth = p.alpha == 0.0f ? 0 : (int)(p.k / TB);  // k-tiles of every tile; alpha == 0 reads neither operand
+    Table table;
+    table.init(p, BN);
+    Copies c;
+    Operands o;
+    f4 acc[MB][NB];
+
+    // k-tile kt, of which the first USED column blocks of the tile exist.
+    // STEADY: k-tiles kt + 1 and kt + 2 exist and are whole.
+    auto k_tile = [&](auto used, auto steady, int kt) {
+      constexpr int USED = decltype(used)::value;
+      constexpr bool STEADY = decltype(steady)::value;
+      const char *st = smem + (kt & 1) * STAGE, *next = smem + (~kt & 1) * STAGE;
+      typename X::wide b[USED];
+      float scale[USED];
+#pragma unroll
+      for (int j = 0; j < USED; ++j) {
+        b[j] = X::widen(o.raw[j]);
+        scale[j] = ROWS ? o.next_b[j] : o.next_a * o.next_b[j];
+      }
+      // part's products; behind(n) is run behind the n-th of PB USED
+      auto multiply = [&](auto part, auto behind) {
+        constexpr int P = decltype(part)::value;
+        typename X::wide w[PB];
+#pragma unroll
+        for (int i = 0; i < PB; ++i) w[i] = X::widen(o.a[P & 1][i]);
+        // a product is scaled behind the LAG next ones: left to itself the
+        // scheduler puts the v_fma right behind its MFMA and waits for it
+        constexpr int LAG = EXACT ? 1 : 2;
+        f4 late[LAG + 1];
+#pragma unroll
+        for (int n = 0; n < PB * USED + LAG; ++n) {
+          if (n < PB * USED) {
+            late[n % (LAG + 1)] = X::dot(w[n % PB], b[n / PB]);
+            __builtin_amdgcn_sched_barrier(0);
+            behind(n);
+          }
+          const int m = n - LAG, i = m % PB, j = m / PB;
+          if (m >= 0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              acc[PB * P + i][j][q] =
+                  fmaf(late[m % (LAG + 1)][q], ROWS ? o.rows[P & 1][i][q] * scale[j] : scale[j], acc[PB * P + i][j][q]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // the sums are made here: past a branch the v_fma would be far from their MFMAs, whose results all wait for them
+#pragma unroll
+        for (int i = 0; i < PB; ++i)
+#pragma unroll
+          for (int j = 0; j < USED; ++j) asm volatile("" : "+v"(acc[PB * P + i][j]));
+      };
+      // of the first part, or of the first two where a part has fewer products than B's k-tile has copies
+      constexpr int AT_ONCE = PB * USED >= COPIES_B ? 1 : (COPIES_B + 2 * PB * USED - 1) / (2 * PB * USED);
+      auto part = [&](auto at) {
+        constexpr int P = decltype(at)::value;
+        o.template fetch_a<P + 1>(st, wm, lane);
+        if constexpr (P == 0 && !STEADY) {
+          if (kt + 1 < depth) c.all_b(smem, wave, kt + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(at, [&](int n) {
+          if (!STEADY || P > 1) return;
+#pragma unroll
+          for (int r = (P * PB * USED + n) * AT_ONCE; r < (P * PB * USED + n + 1) * AT_ONCE; ++r)
+            if (r < COPIES_B) c.b(smem, wave, kt + 1, r);
+        });
+      };
+      part(std::integral_constant<int, 0>());
+      part(std::integral_constant<int, 1>());
+      part(std::integral_constant<int, 2>());
+      if constexpr (PARTS == 8) {
+        part(std::integral_constant<int, 3>());
+        part(std::integral_constant<int, 4>());
+        part(std::integral_constant<int, 5>());
+        part(std::integral_constant<int, 6>());
+      }
+      wait_barrier<0>();
+      if constexpr (!STEADY) {
+        if (kt + 2 < depth) c.all_a(smem, wave, kt + 2);
+      }
+      // (behind the last k-tile: what is read is not used)
+      o.template fetch_a<0>(next, wm, lane);  // PARTS is even: the other registers
+      o.fetch_scales(next, wm, wn, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int A_AT_ONCE = (SA::LOADS + PB * USED - 1) / (PB * USED);
+      multiply(std::integral_constant<int, PARTS - 1>(), [&](int n) {
+        if (n % PB == PB - 1) o.fetch_b(next, wn, lane, n / PB);
+        if (!STEADY) return;
+#pragma unroll
+        for (int r = n * A_AT_ONCE; r < (n + 1) * A_AT_ONCE; ++r)
+          if (r < SA::LOADS) c.a(smem, wave, kt + 2, r);
+      });
+    };
+    auto k_tiles = [&](auto used) {
+      const int whole = AMC ? c.sa.whole_tiles() : depth, steady = (whole < depth ? whole : depth) - 2;
+      int kt = 0;
+      for (; kt < steady; ++kt) k_tile(used, std::true_type(), kt);
+      for (; kt < depth; ++kt) k_tile(used, std::false_type(), kt);
+    };
+    // The first copies of tile i (its k-tile 0, and A of k-tile 1): false if there is none.
+    Tile tile;
+    auto begin = [&](int i) {
+      if (!table.get(i, tile)) return false;
+      if (depth > 0) {
+        c.init(p, tile, t);
+        c.all_a(smem, wave, 0);
+        c.all_b(smem, wave, 0);
+        if (depth > 1) c.all_a(smem, wave, 1);
+      }
+      return true;
+    };
+
+    bool more = begin(0);
+    for (int i = 1; more; ++i) {
+      const int64_t row0 = (int64_t)tile.tm * BM + wm, n0 = (int64_t)tile.tn * BN, cols = tile.hi - tile.lo, at = tile.lo * p.ldc;
+#pragma unroll
+      for (int x = 0; x < MB; ++x)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[x][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (depth > 0) {
+        wait_barrier<0>();
+#pragma unroll
+        for (int j = 0; j < NB; ++j) o.fetch_b(smem, wn, lane, j);
+        o.fetch_scales(smem, wm, wn, lane);
+        o.template fetch_a<0>(smem, wm, lane);
+        // column blocks in use: a group's last tile costs what its columns need
+        if (cols - n0 > STEP * 3)
+          k_tiles(std::integral_constant<int, 4>());
+        else if (cols - n0 > STEP * 2)
+          k_tiles(std::integral_constant<int, 3>());
+        else if (cols - n0 > STEP)
+          k_tiles(std::integral_constant<int, 2>());
+        else
+          k_tiles(std::integral_constant<int, 1>());
+        // all waves have read the last k-tile's operands before its barrier; what they read behind it is not used
+      }
+      more = begin(i);
+      store(p, at, acc, row0, n0 + wn, cols, lane);
+    }
+  }
+
+  // Without guards for rows where there is nothing to guard.
+  static __device__ __forceinline__ void store(const Args &p, int64_t at, const f4 (&acc)[MB][NB], int64_t row0, int64_t col0,
+                                               int64_t cols, int lane) {
+    const bool inside = p.beta == 0.0f && row0 + 16 * MB <= p.m;
+    if (inside && p.stream)
+      store_tile<Fp8, STEP, true, true>(p, at, acc, row0, col0, cols, lane);
+    else if (inside)
+      store_tile<Fp8, STEP, false, true>(p, at, acc, row0, col0, cols, lane);
+    else
+      store_tile<Fp8, STEP, false>(p, at, acc, row0, col0, cols, lane);
   }
 };
 

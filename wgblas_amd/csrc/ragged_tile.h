@@ -138,8 +138,8 @@ struct Args {
   // block_a) + a_k b, the groups' a_group apart; B's of column j at j + b_k b
   const float *block_scale_a, *block_scale_b;
   int64_t a_row, a_k, a_group, b_k;
-  int block_a;
-  int64_t a_rows;  // fp8, row-contiguous A: rows rounded up to whole runs of 128
+  int a_shift;  // block_a = 2^a_shift
+  int64_t a_rows, a_depth;  // fp8: m rounded up to whole runs of 128; k as it is (Args::k is whole runs)
   int stream;  // C's columns start at 64-byte boundaries: large results bypass the caches
   int c_f32;   // C holds fp32 (else the operands' type; fp4 and fp8: bf16, or f16 with c_f16)
   int c_f16;
@@ -668,7 +668,8 @@ __device__ __forceinline__ v4i eight_rows(uint32_t x0, uint32_t x1, uint32_t y0,
 // of 64 bytes, weight gradients of 8 x 4096 x 2048 in fp32 wrote 399 MB for the
 // 268 of C and took 195 us instead of 175, forward products of 16384 columns of
 // 8192 bf16 values 1020 instead of 983.
-template <typename T, int MB, int NB, int STEP, bool STREAM>
+// INSIDE: the caller knows that all rows exist and beta is 0.
+template <typename T, int MB, int NB, int STEP, bool STREAM, bool INSIDE = false>
 __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB][NB], int64_t row0, int64_t rows,
                                          int64_t col0, int64_t cols, int lane) {
   typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -686,7 +687,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
       f4 x = acc[i][j];
 #pragma unroll
       for (int q = 0; q < 4; ++q) x[q] *= p.alpha;
-      if (p.beta != 0.0f && in) {
+      if (!INSIDE && p.beta != 0.0f && in) {
         if (row + 4 <= rows) {
           const V4 c = *reinterpret_cast<const V4 *>(cp + row);
 #pragma unroll
@@ -734,7 +735,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
           if (to >= cols) continue;
           T *at = C + to * p.ldc + row;
           const Run v = __builtin_bit_cast(Run, y[h]);
-          if (row + ROWS <= rows) {
+          if (INSIDE || row + ROWS <= rows) {
             __builtin_nontemporal_store(v, reinterpret_cast<Run *>(at));
           } else {
 #pragma unroll
@@ -751,7 +752,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
         const u2 x = __builtin_bit_cast(u2, value(i)), y = __builtin_bit_cast(u2, value(i + 1));
         const V8 v = __builtin_bit_cast(V8, eight_rows(x[0], x[1], y[0], y[1]));
         const int64_t row = row0 + 16 * (i + (g & 1)) + 8 * (g >> 1);
-        if (row + 8 <= rows) {
+        if (INSIDE || row + 8 <= rows) {
           *reinterpret_cast<V8 *>(cp + row) = v;
         } else {
 #pragma unroll
@@ -764,7 +765,7 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
       for (int i = 0; i < MB; ++i) {
         const V4 v = value(i);
         const int64_t row = row0 + 16 * i + 4 * g;
-        if (row + 4 <= rows) {
+        if (INSIDE || row + 4 <= rows) {
           *reinterpret_cast<V4 *>(cp + row) = v;
         } else {
 #pragma unroll
@@ -777,18 +778,18 @@ __device__ __forceinline__ void epilogue(const Args &p, T *C, const f4 (&acc)[MB
 }
 
 // The epilogue in C's type; `at`: element of C where the group's part starts.
-template <class E, int STEP, bool STREAM = false, int MB, int NB>
+template <class E, int STEP, bool STREAM = false, bool INSIDE = false, int MB, int NB>
 __device__ __forceinline__ void store_tile(const Args &p, int64_t at, const f4 (&acc)[MB][NB], int64_t row0, int64_t col0,
                                            int64_t cols, int lane) {
   if (E::kBits == 32 || p.c_f32) {
-    epilogue<float, MB, NB, STEP, STREAM>(p, (float *)p.C + at, acc, row0, p.m, col0, cols, lane);
+    epilogue<float, MB, NB, STEP, STREAM, INSIDE>(p, (float *)p.C + at, acc, row0, p.m, col0, cols, lane);
   } else if constexpr (E::kBits <= 8) {
     if (p.c_f16)
-      epilogue<_Float16, MB, NB, STEP, STREAM>(p, (_Float16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
+      epilogue<_Float16, MB, NB, STEP, STREAM, INSIDE>(p, (_Float16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
     else
-      epilogue<__bf16, MB, NB, STEP, STREAM>(p, (__bf16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
+      epilogue<__bf16, MB, NB, STEP, STREAM, INSIDE>(p, (__bf16 *)p.C + at, acc, row0, p.m, col0, cols, lane);
   } else if constexpr (E::kBits == 16) {
-    epilogue<typename E::store, MB, NB, STEP, STREAM>(p, (typename E::store *)p.C + at, acc, row0, p.m, col0, cols, lane);
+    epilogue<typename E::store, MB, NB, STEP, STREAM, INSIDE>(p, (typename E::store *)p.C + at, acc, row0, p.m, col0, cols, lane);
   }
 }
 
