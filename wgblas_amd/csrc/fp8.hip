@@ -288,14 +288,47 @@ int check_convert(int type, int block, int64_t k, int64_t n) {
   return WGB_OK;
 }
 
+// Estimated times of tiles (ragged_tile.h) at k = 1024: first and each further
+// one on a CU. Measured from 1024 x 1024 x 4096 (64 x 64 tiles: 15.5 us into
+// bf16, 19.5 into fp32), 2048 x 2048 x 8192 (128 x 128: 57 and 86) and 8192 x
+// 4096 x 4096 (128 x 128: 147 and 245, 256 x 256: 122 and 218).
+template <bool ROWS, bool EXACT>
+constexpr TileCost cost(int T) {
+  if (!EXACT) {
+    return T == 64 ? TileCost{3.0, 1.5}
+           : ROWS  ? (T == 128 ? TileCost{6.6, 4.3} : TileCost{14.5, 14.5})
+                   : (T == 128 ? TileCost{6.4, 3.7} : TileCost{12.0, 12.0});
+  }
+  return T == 64  ? (ROWS ? TileCost{4.2, 2.3} : TileCost{3.7, 2.1})
+         : T == 128 ? (ROWS ? TileCost{10.3, 7.4} : TileCost{9.4, 6.8})
+                    : TileCost{22.0, 22.0};
+}
+
 template <bool AMC, bool ROWS, bool EXACT>
 int product(wgb_ctx *ctx, Args &p) {
+  typedef Fp8Kernel<128, 128, 2, 2, AMC, ROWS, EXACT, 2> K128;
   const int64_t mean = p.n / p.groups;
-  if (mean <= 32) return launch_columns<Fp8Kernel<128, 32, 4, 1, AMC, ROWS, EXACT, 4>>(ctx, p);
-  const int64_t tiles = (p.m + 127) / 128 * ((p.n + 127) / 128);
-  if (tiles >= 4 * ctx->num_cus)
-    return launch_columns_rounds<Fp8Large<AMC, ROWS, EXACT>, Fp8Kernel<128, 128, 2, 2, AMC, ROWS, EXACT, 2>>(ctx, p);
-  if (tiles >= ctx->num_cus) return launch_columns<Fp8Kernel<128, 128, 2, 2, AMC, ROWS, EXACT, 2>>(ctx, p);
+  if (mean <= 32) {
+    // Few columns: reading A counts, streamed through LDS, or with too few
+    // blocks for the CUs straight into registers, the waves sharing k.
+    const int64_t blocks = (p.m + 127) / 128 * (p.n < p.groups ? p.n : p.groups);
+    if constexpr (!AMC) {
+      if (blocks < ctx->num_cus)
+        return mean <= 16 ? launch_columns<Fp8Skinny<2, 1, ROWS, EXACT>>(ctx, p) : launch_columns<Fp8Skinny<2, 2, ROWS, EXACT>>(ctx, p);
+    }
+    return launch_columns<Fp8Kernel<128, 32, 4, 1, AMC, ROWS, EXACT, 4>>(ctx, p);
+  }
+  const double k = (double)p.k, size = p.c_f32 ? 4 : 2;
+  const TileCost c64 = cost<ROWS, EXACT>(64), c128 = cost<ROWS, EXACT>(128), c256 = cost<ROWS, EXACT>(256);
+  const double t64 = small_time(64, c64, per_cu(ctx, p, 64, expected_columns(p, 64)), k, size);
+  const double t128 = small_time(128, c128, per_cu(ctx, p, 128, expected_columns(p, 128)), k, size);
+  // with a scale for each row and exact sums v_fma and the conversions bound
+  // it, and 256 x 256 tiles win nothing (8192 x 4096 x 4096: 261 us on 128 x 128 tiles, 256)
+  if constexpr (!ROWS || !EXACT) {
+    const double t256 = rounds_time(c256, c128, per_cu(ctx, p, 256, expected_columns(p, 256)), k, size, most_pieces(p.k, 128));
+    if (t256 <= t128 && t256 <= t64) return launch_columns_rounds<Fp8Large<AMC, ROWS, EXACT>, K128>(ctx, p);
+  }
+  if (t128 <= t64) return launch_columns<K128>(ctx, p);
   return launch_columns<Fp8Kernel<64, 64, 2, 2, AMC, ROWS, EXACT, 2>>(ctx, p);
 }
 

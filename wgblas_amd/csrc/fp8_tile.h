@@ -592,4 +592,120 @@ struct Fp8Large {
   }
 };
 
+// Few columns a group (single tokens): bound by reading A once. A block has R
+// row blocks and CB column blocks of 16; its eight waves share k in k-tiles,
+// load both operands straight into MFMA operand registers, the next k-tile ahead
+// of the present one's MFMAs, and add their sums in LDS in the waves' order. A
+// k-contiguous only.
+template <int R, int CB, bool ROWS, bool EXACT>
+struct Fp8Skinny {
+  static constexpr int kBM = 16 * R, kBN = 16 * CB;
+  static constexpr int NW = 8, NT = 64 * NW;
+  static constexpr int LDS = NW * R * CB * 1024;
+  typedef Codes<EXACT> X;
+
+  struct Operands {
+    v8i a[R], b[CB];
+    f4 sa[R];  // of the lane's four rows, or [0][0] for all
+    float sb[CB];
+  };
+
+  static __device__ __forceinline__ v8i load(const char *row) {
+    const v4i x = *reinterpret_cast<const v4i *>(row), y = *reinterpret_cast<const v4i *>(row + 64);
+    return v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  }
+
+  static __device__ __forceinline__ void run(const Args &p, char *smem) {
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int i16 = lane & 15, g = lane >> 4;
+    Tile tile;
+    ColumnOrder order;
+    order.init(p, kBN);
+    if (!order.find(p, blockIdx.x, tile)) return;
+    const int64_t m0 = (int64_t)tile.tm * kBM, n0 = tile.lo + (int64_t)tile.tn * kBN;
+    const int nt = p.alpha == 0.0f ? 0 : (int)(p.k / TB);  // alpha == 0 reads neither operand
+
+    // this lane's chunks and scales; past the end the last row or column is
+    // read again (what it gives is never stored)
+    const char *pa[R], *pb[CB];
+    const float *sa[R][ROWS ? 4 : 1], *sb[CB];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = m0 + 16 * r + i16, last = p.m - 1;
+      pa[r] = p.A + (int64_t)tile.g * p.stride_a + (row < last ? row : last) * p.lda + 16 * g;
+#pragma unroll
+      for (int q = 0; q < (ROWS ? 4 : 1); ++q) {
+        const int64_t of = ROWS ? m0 + 16 * r + 4 * g + q : m0;  // a block's rows share a scale
+        sa[r][q] = p.block_scale_a + tile.g * p.a_group + ((of < last ? of : last) >> p.a_shift) * p.a_row;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      int64_t col = n0 + 16 * c + i16;
+      if (col >= tile.hi) col = tile.hi - 1;
+      pb[c] = p.B + col * p.ldb + 16 * g;
+      sb[c] = p.block_scale_b + col;
+    }
+    auto fetch = [&](int kt, Operands &o) {
+      const int64_t at = (int64_t)kt * TB;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        o.a[r] = load(pa[r] + at);
+        if (ROWS || r == 0)
+#pragma unroll
+          for (int q = 0; q < (ROWS ? 4 : 1); ++q) o.sa[r][q] = sa[r][q][kt * p.a_k];
+      }
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        o.b[c] = load(pb[c] + at);
+        o.sb[c] = sb[c][kt * p.b_k];
+      }
+    };
+    f4 acc[R][CB];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < CB; ++c) acc[r][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const Operands &o) {
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        const typename X::wide b = X::widen(o.b[c]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const f4 x = X::dot(X::widen(o.a[r]), b);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[r][c][q] = fmaf(x[q], (ROWS ? o.sa[r][q] : o.sa[0][0]) * o.sb[c], acc[r][c][q]);
+        }
+      }
+    };
+    Operands x, y;
+    int kt = wave;
+    if (kt < nt) fetch(kt, x);
+    while (kt < nt) {
+      if (kt + NW < nt) fetch(kt + NW, y);
+      multiply(x);
+      kt += NW;
+      if (kt >= nt) break;
+      if (kt + NW < nt) fetch(kt + NW, x);
+      multiply(y);
+      kt += NW;
+    }
+
+    // the waves' sums, one block (r, c) after the other: lane's f4 as it is
+    f4 *sums = reinterpret_cast<f4 *>(smem);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < CB; ++c) sums[(wave * R * CB + r * CB + c) * 64 + lane] = acc[r][c];
+    __syncthreads();
+    const int64_t cols = tile.hi - n0;
+    if (wave >= R * CB) return;
+    static_assert(R * CB <= NW, "a wave a block");
+    f4 total[1][1] = {{sums[wave * 64 + lane]}};
+#pragma unroll
+    for (int v = 1; v < NW; ++v) total[0][0] += sums[(v * R * CB + wave) * 64 + lane];
+    store_tile<Fp8, 16>(p, n0 * p.ldc, total, m0 + 16 * (wave / CB), 16 * (wave % CB), cols, lane);
+  }
+};
+
 }  // namespace wgb_ragged

@@ -1537,6 +1537,11 @@ inline int most_pieces(int64_t k, int bk) {
 // Bytes of Args::parts: what the rest's blocks that run at once (two a CU) may hold.
 inline size_t parts_bytes(const wgb_ctx *ctx) { return (size_t)ctx->num_cus * 2 * 128 * 128 * 4; }
 
+// Whether C's columns start at 64-byte boundaries (Args::stream).
+inline int stores_lines(const Args &p) {
+  return ((uintptr_t)p.C & 63) == 0 && p.ldc * (p.c_f32 ? 4 : 2) % 64 == 0 && p.stride_c * (p.c_f32 ? 4 : 2) % 64 == 0;
+}
+
 // `Turn` on at most `tiles` 256 x 256 tiles, a block a CU (more where one
 // could not keep its tiles), then `Rest` (128 x 128 tiles, a quarter of one
 // each) on what that leaves, and if that may be cut along k, their sums. Which
@@ -1544,7 +1549,7 @@ inline size_t parts_bytes(const wgb_ctx *ctx) { return (size_t)ctx->num_cus * 2 
 // expect.
 template <class Turn, class Rest>
 int launch_rounds(wgb_ctx *ctx, Args &p, int64_t tiles, bool exact, int64_t k) {
-  p.stream = ((uintptr_t)p.C & 63) == 0 && p.ldc * (p.c_f32 ? 4 : 2) % 64 == 0 && p.stride_c * (p.c_f32 ? 4 : 2) % 64 == 0;
+  p.stream = stores_lines(p);
   int64_t blocks = tiles;
   if (tiles > ctx->num_cus) {
     blocks = (tiles + kTilesPerBlock - 1) / kTilesPerBlock;
