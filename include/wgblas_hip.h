@@ -457,7 +457,9 @@ int wgb_fp8_gemm_grouped(wgb_ctx *ctx, int transA, int64_t groups, int64_t m,
  * column-major at ldl, of `type`). An expert's score is the softmax over all
  * experts' logits (WGB_SOFTMAX) or the logistic function of its own
  * (WGB_SIGMOID); its choice value is the score plus bias[e] (fp32; null: none;
- * used for the choice alone, to balance the experts' load). With groups > 1
+ * used for the choice alone, to balance the experts' load); without a bias, and
+ * with groups by their best one, the logits themselves, whose order is the
+ * scores', are compared. With groups > 1
  * the experts come in groups of experts/groups neighbours: only those
  * top_groups groups stay whose best choice value (best 1), or the sum of whose
  * two best (best 2), is largest. ids gets the topk experts of the largest
@@ -485,7 +487,7 @@ int wgb_route_grad(wgb_ctx *ctx, int type, int scoring, int64_t experts,
  * take them, places[p] pair p's column in that order, pairs[c] the pair that
  * column c belongs to (its token is pairs[c] / topk). A pair whose id is
  * outside the experts has place -1; columns behind the last expert's get pair
- * -1. More than 1024 pairs use the context's workspace (at most 1 MiB), as the
+ * -1. More than 1024 pairs use the context's workspace (at most 256 KiB), as the
  * grouped products do. */
 int wgb_route_order(wgb_ctx *ctx, int64_t experts, int64_t n, int64_t topk,
                     const int32_t *ids, int64_t *d_offsets, int32_t *places,

@@ -26,6 +26,10 @@ __device__ __forceinline__ float ror(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + ROR, 0xf, 0xf, true));
 }
 template <int ROR>
+__device__ __forceinline__ int ror(int x) {
+  return __builtin_amdgcn_mov_dpp(x, 0x120 + ROR, 0xf, 0xf, true);
+}
+template <int ROR>
 __device__ __forceinline__ double ror(double x) {
   typedef int i2 __attribute__((ext_vector_type(2)));
   i2 v = __builtin_bit_cast(i2, x);
@@ -81,42 +85,200 @@ struct RouteArgs {
   float *weights;
 };
 
+// A token's lanes are in one wave: what one has stored in LDS the others read
+// behind this.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// What is compared: whole numbers in the order of fp32 values (zeros of either
+// sign are equal, NaN comes after all numbers), or fp64 values themselves.
 template <class F>
-struct Limits;
+struct Keys;
 template <>
-struct Limits<float> {
-  static __device__ float none() { return -__builtin_inff(); }
-  static __device__ float nan() { return -1e38f; }  // below what is a number; two of them can be added
+struct Keys<float> {
+  typedef int key;
+  static constexpr int kNone = (int)0x80000000;  // not there
+  static constexpr int kNan = kNone + 1;
+  static __device__ __forceinline__ int of(float x) {
+    const int b = __float_as_int(x + 0.0f);
+    return x != x ? kNan : x == -__builtin_inff() ? kNone : b ^ ((b >> 31) & 0x7fffffff);
+  }
+  static __device__ __forceinline__ float value(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+  // of a group: the sum of its two best; scores that are NaN come after all numbers there, too
+  static __device__ __forceinline__ int sum(int a, int b) {
+    if (a == kNone || b == kNone) return kNone;
+    if (b == kNan) return a == kNan ? kNan : of(value(a) - 1e30f);
+    return of(value(a) + value(b));
+  }
 };
 template <>
-struct Limits<double> {
-  static __device__ double none() { return -__builtin_inf(); }
-  static __device__ double nan() { return -1e300; }
+struct Keys<double> {
+  typedef double key;
+  static constexpr double kNone = -__builtin_inf(), kNan = -1e300;
+  static __device__ __forceinline__ double of(double x) { return x != x ? kNan : x; }
+  static __device__ __forceinline__ double sum(double a, double b) {
+    if (a == kNone || b == kNone) return kNone;
+    if (b == kNan) return a == kNan ? kNan : a - 1e30;
+    return a + b;
+  }
 };
 
-// LPT lanes a token, PER consecutive experts a lane. A token's choice values
-// stay in its lanes' registers; each round takes the largest, the lowest
-// expert of equal ones.
-//
-// F: what is compared. Scores grow with the logits, so without a bias and
-// with groups by their best expert the logits themselves decide (float,
-// exact). Otherwise values next to each other decide, score + bias, and are
-// held in 64 bits: in 32 the choice would depend on the exponential's last
-// bits.
-template <class T, class F, int LPT, int PER>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
-  constexpr bool kWide = std::is_same<F, double>::value;
-  constexpr int TOKENS = 256 / LPT;
-  __shared__ int chosen[TOKENS][kMaxTopk];
-  extern __shared__ __align__(16) char route_smem[];  // with groups: values, groups' scores and which are kept
-  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT;
-  const int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
-  const bool here = token < p.n;
-  const T *x = (const T *)p.logits + (here ? token : p.n - 1) * p.ldl;
-  const int e0 = lane * PER;
+// Room of a token in LDS: its values, and its groups' scores.
+template <class F>
+struct Room {
+  static __host__ __device__ int values(int experts) { return (experts + 3) & ~3; }
+  static __host__ __device__ size_t bytes(int experts, int groups) {
+    return (values(experts) + ((groups + 3) & ~3)) * sizeof(F);
+  }
+};
 
-  float l[PER];
-  if (e0 + PER <= p.experts) {
+// How far two choice values have to be apart so that fp32 tells which is the
+// larger: a score is off by at most 4 units of 2^-24 (sigmoid: the exponential
+// by |x| 2^-23 of itself, which p (1 - p) |x| < 0.3 makes 0.6 units, the
+// reciprocal by 2; softmax: 26 with the sum's), the value by half a unit more,
+// and twice that is doubled.
+__device__ __forceinline__ float unsure(float value, int sigmoid) {
+  return ((sigmoid ? 4.0f : 32.0f) + fabsf(value)) * 0x1p-22f;
+}
+
+// The two best of a run of values, a >= b.
+template <class K>
+__device__ __forceinline__ void best_two(K &a, K &b, K x, K y) {
+  const K low = a < x ? a : x;
+  a = a < x ? x : a;
+  b = b < y ? y : b;
+  b = b < low ? low : b;
+}
+
+// What a lane knows of its values: bit j of value j.
+struct Groups {
+  uint32_t kept;   // in one of the top_groups best groups
+  uint32_t best;   // may be one of its group's best
+  bool close;      // a kept group and one that is not are too near to tell (fp32)
+};
+
+template <class F, int LPT, int PER>
+__device__ __forceinline__ Groups keep_groups(const RouteArgs &p, char *room, int lane, const typename Keys<F>::key (&v)[PER]) {
+  typedef typename Keys<F>::key K;
+  K *values = reinterpret_cast<K *>(room), *score = values + Room<K>::values(p.experts);
+  const int e0 = lane * PER, lanes = p.per / PER;  // of a group, where groups are whole lanes
+  auto scored = [&](K a, K b) { return p.best == 2 && p.per > 1 ? Keys<F>::sum(a, b) : a; };
+  Groups g = {0, (1u << PER) - 1, false};
+  const bool whole = lanes * PER == p.per && (lanes & (lanes - 1)) == 0;
+  if (whole) {
+    K a = v[0], b = Keys<F>::kNone;
+#pragma unroll
+    for (int j = 1; j < PER; ++j) best_two(a, b, v[j], Keys<F>::kNone);
+    for (int d = 1; d < lanes; d <<= 1) best_two(a, b, (K)__shfl_xor(a, d), (K)__shfl_xor(b, d));
+    if ((lane & (lanes - 1)) == 0 && e0 < p.experts) score[e0 / p.per] = scored(a, b);
+    if constexpr (std::is_same<F, float>::value) {
+      if (b > Keys<F>::kNan) {
+        const K least = Keys<F>::of(Keys<F>::value(b) - unsure(Keys<F>::value(b), p.sigmoid));
+        g.best = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) g.best |= v[j] >= least ? 1u << j : 0u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (e0 + j < p.experts) values[e0 + j] = v[j];
+    wave_sync();
+    for (int i = lane; i < p.groups; i += LPT) {
+      K a = Keys<F>::kNone, b = a;
+      for (int j = 0; j < p.per; ++j) best_two(a, b, values[i * p.per + j], Keys<F>::kNone);
+      score[i] = scored(a, b);
+    }
+  }
+  wave_sync();
+  // whether group i is kept; one that is compares itself with those that are not
+  auto kept = [&](int i) {
+    const K mine = score[i];
+    int before = 0;
+    for (int o = 0; o < p.groups; ++o) before += score[o] > mine || (score[o] == mine && o < i);
+    const bool in = before < p.top_groups;
+    if constexpr (std::is_same<F, float>::value) {
+      // the group behind the last kept one: the last one asks for it
+      if (before == p.top_groups - 1 && mine > Keys<F>::kNan) {
+        K next = Keys<F>::kNone;
+        for (int o = 0; o < p.groups; ++o) {
+          const K s = score[o];
+          if (s > next && (s < mine || (s == mine && o > i))) next = s;
+        }
+        const float least = Keys<F>::value(mine);
+        if (next > Keys<F>::kNan) g.close |= least - Keys<F>::value(next) <= 2.0f * unsure(least, p.sigmoid);
+      }
+    }
+    return in;
+  };
+  if (whole) {
+    if (e0 < p.experts && kept(e0 / p.per)) g.kept = (1u << PER) - 1;
+  } else {
+    int of = -1;
+    bool in = false;
+#pragma nounroll
+    for (int j = 0; j < PER && e0 + j < p.experts; ++j) {
+      const int i = (int)(((uint32_t)(e0 + j) * p.magic) >> 20);
+      if (i != of) in = kept(of = i);
+      g.kept |= in ? 1u << j : 0u;
+    }
+  }
+  wave_sync();
+  return g;
+}
+
+// The topk largest, one a round, the lowest expert of equal ones, into
+// chosen[]. fp32 values that are not exact: `may` gets a lane's values that may
+// be among them, and the result is whether two of them, or the last one and the
+// next, are too near to tell.
+template <class F, int LPT, int PER>
+__device__ __forceinline__ bool choose(const RouteArgs &p, int lane, int wave_lane, typename Keys<F>::key (&v)[PER],
+                                       int *chosen, uint32_t &may) {
+  typedef typename Keys<F>::key K;
+  bool close = false;
+  K last = Keys<F>::kNone;
+  may = 0;
+  for (int s = 0; s <= p.topk; ++s) {
+    K best = v[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) best = v[j] > best ? v[j] : best;
+    const K most = over_lanes<LPT>(best, Max());
+    const bool any = most != Keys<F>::kNone;
+    if constexpr (std::is_same<F, float>::value) {
+      if (s > 0 && any) close |= Keys<F>::value(last) - Keys<F>::value(most) <= unsure(Keys<F>::value(most), p.sigmoid);
+      if (s == p.topk && close) {
+        const K least = Keys<F>::of(Keys<F>::value(last) - unsure(Keys<F>::value(last), p.sigmoid));
+#pragma unroll
+        for (int j = 0; j < PER; ++j) may |= v[j] != Keys<F>::kNone && (last <= Keys<F>::kNan || v[j] >= least) ? 1u << j : 0u;
+      }
+    }
+    last = any ? most : last;
+    if (s == p.topk) break;
+    const bool mine = any && first_lane<LPT>(best == most, wave_lane) == lane;
+    // the lowest of the lane's that is the largest, as masks of lanes
+    uint64_t open = __ballot(mine);
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t hit = __ballot(v[j] == most) & open;
+      open &= ~hit;
+      const bool here = __builtin_amdgcn_inverse_ballot_w64(hit);
+      v[j] = here ? Keys<F>::kNone : v[j];
+      at = here ? j : at;
+    }
+    if (mine) may |= 1u << at;
+    if (any ? mine : lane == 0) chosen[s] = any ? lane * PER + at : -1;
+  }
+  return close;
+}
+
+// PER values of a row from e0, `none` past its end; any alignment.
+template <class T, int PER>
+__device__ __forceinline__ void load_row(const T *x, int e0, int experts, float none, float (&l)[PER]) {
+  if (e0 + PER <= experts) {
     struct __attribute__((packed, aligned(sizeof(T)))) V {
       T v[PER];
     };
@@ -125,8 +287,36 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
     for (int j = 0; j < PER; ++j) l[j] = (float)v.v[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) l[j] = e0 + j < p.experts ? (float)x[e0 + j] : -__builtin_inff();
+    for (int j = 0; j < PER; ++j) l[j] = e0 + j < experts ? (float)x[e0 + j] : none;
   }
+}
+
+// LPT lanes a token, PER consecutive experts a lane. A token's choice values
+// stay in its lanes' registers; each round takes the largest.
+//
+// Scores grow with the logits, so without a bias and with groups by their best
+// expert the logits themselves decide, exactly. Otherwise (WIDE) score + bias
+// do, or sums of two scores, and values next to each other are told apart in 64
+// bits: fp32 ones first, and where two that matter are within what those may be
+// off (0.1% of tokens with 256 experts, all with equal ones), fp64 ones of the
+// values that may be chosen, one at a time: few, and the code short, for it is
+// seldom run and comes from beyond the instruction cache (fp64 values of all 256
+// experts of such tokens alone: 10 us, for 16384 tokens that otherwise take 16).
+template <class T, bool WIDE, int LPT, int PER>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
+  constexpr int TOKENS = 256 / LPT;
+  typedef typename std::conditional<WIDE, double, int>::type Widest;
+  __shared__ int chosen[TOKENS][kMaxTopk];
+  extern __shared__ __align__(16) char route_smem[];  // WIDE or with groups: a Room for each token
+  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT, wave_lane = threadIdx.x & 63;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + slot;
+  const bool here = token < p.n;
+  const T *x = (const T *)p.logits + (here ? token : p.n - 1) * p.ldl;
+  const int e0 = lane * PER;
+  char *room = route_smem + slot * Room<Widest>::bytes(p.experts, p.groups);
+
+  float l[PER];
+  load_row<T, PER>(x, e0, p.experts, -__builtin_inff(), l);
 
   // softmax: the largest logit and the sum of exponentials
   float top = 0.0f, total = 1.0f;
@@ -138,94 +328,80 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
     if (top == -__builtin_inff()) top = 0.0f;  // no expert at all: scores of zero
     total = 0.0f;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) total += expf(l[j] - top);
+    for (int j = 0; j < PER; ++j) total += __expf(l[j] - top);
     total = over_lanes<LPT>(total, Sum());
     if (total == 0.0f) total = 1.0f;
   }
 
-  F v[PER];
-  if constexpr (kWide) {
-    double sum = 1.0;
-    double s[PER];
-    if (p.sigmoid) {
+  int v[PER];
+  uint32_t may;
+  if constexpr (!WIDE) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
-    } else {
-      sum = 0.0;
+    for (int j = 0; j < PER; ++j) v[j] = Keys<float>::of(l[j]);
+    if (p.groups > 1) {
+      const Groups g = keep_groups<float, LPT, PER>(p, room, lane, v);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        s[j] = exp((double)l[j] - (double)top);
-        sum += s[j];
-      }
-      sum = over_lanes<LPT>(sum, Sum());
-      if (sum == 0.0) sum = 1.0;
+      for (int j = 0; j < PER; ++j) v[j] = g.kept >> j & 1 ? v[j] : Keys<float>::kNone;
     }
+    choose<float, LPT, PER>(p, lane, wave_lane, v, chosen[slot], may);
+  } else {
+    float b[PER];
+    if (p.bias) {
+      load_row<float, PER>(p.bias, e0, p.experts, 0.0f, b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) b[j] = 0.0f;
+    }
+    const float inverse = __builtin_amdgcn_rcpf(total);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const float b = p.bias && e0 + j < p.experts ? p.bias[e0 + j] : 0.0f;
-      v[j] = l[j] == -__builtin_inff() ? -__builtin_inf() : s[j] / sum + (double)b;
+      const float s = p.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __expf(-l[j])) : __expf(l[j] - top) * inverse;
+      v[j] = l[j] == -__builtin_inff() ? Keys<float>::kNone : Keys<float>::of(s + b[j]);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) v[j] = l[j];
-  }
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (v[j] != v[j]) v[j] = Limits<F>::nan();
-
-  if (p.groups > 1) {
-    const int room = (p.experts + 1) & ~1;
-    F *values = reinterpret_cast<F *>(route_smem) + slot * (room + p.groups);
-    F *score = values + room;
-    uint8_t *kept = reinterpret_cast<uint8_t *>(reinterpret_cast<F *>(route_smem) + TOKENS * (room + p.groups)) + slot * kMaxGroups;
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (e0 + j < p.experts) values[e0 + j] = v[j];
-    __syncthreads();
-    for (int g = lane; g < p.groups; g += LPT) {
-      F a = Limits<F>::none(), b = a;
-      for (int i = 0; i < p.per; ++i) {
-        const F w = values[g * p.per + i];
-        if (w > a) {
-          b = a;
-          a = w;
-        } else if (w > b) {
-          b = w;
-        }
+    // the fp64 values of those of `which`, the others none
+    double w[PER];
+    auto exact = [&](uint32_t which) {
+      auto score = [&](float y) { return p.sigmoid ? 1.0 / (1.0 + exp(-(double)y)) : exp((double)y - (double)top); };
+      double *values = reinterpret_cast<double *>(room), sum = 1.0;
+      if (!p.sigmoid) {
+        sum = 0.0;
+#pragma nounroll
+        for (int j = 0; j < PER && e0 + j < p.experts; ++j) sum += score((float)x[e0 + j]);
+        sum = over_lanes<LPT>(sum, Sum());
+        if (sum == 0.0) sum = 1.0;
       }
-      score[g] = p.best == 2 && p.per > 1 ? a + b : a;
-    }
-    __syncthreads();
-    for (int g = lane; g < p.groups; g += LPT) {
-      const F mine = score[g];
-      int before = 0;
-      for (int o = 0; o < p.groups; ++o) before += score[o] > mine || (score[o] == mine && o < g);
-      kept[g] = before < p.top_groups;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (e0 + j < p.experts && !kept[((uint32_t)(e0 + j) * p.magic) >> 20]) v[j] = Limits<F>::none();
-  }
-
-  const int wave_lane = threadIdx.x & 63;
-  for (int s = 0; s < p.topk; ++s) {
-    F best = v[0];
-#pragma unroll
-    for (int j = 1; j < PER; ++j) best = v[j] > best ? v[j] : best;
-    const F most = over_lanes<LPT>(best, Max());
-    const bool any = most > Limits<F>::none();
-    const bool mine = any && first_lane<LPT>(best == most, wave_lane) == lane;
-    int at = -1;
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (mine && at < 0 && v[j] == most) {
-        at = j;
-        v[j] = Limits<F>::none();
+#pragma nounroll
+      for (uint32_t left = e0 < p.experts ? which : 0; left; left &= left - 1) {
+        const int e = e0 + __builtin_ctz(left);
+        if (e < p.experts) values[e] = score((float)x[e]) / sum + (p.bias ? (double)p.bias[e] : 0.0);
       }
-    if (any ? mine : lane == 0) chosen[slot][s] = any ? e0 + at : -1;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        w[j] = (which >> j & 1) && l[j] != -__builtin_inff() ? Keys<double>::of(values[e0 + j]) : Keys<double>::kNone;
+      wave_sync();
+    };
+    uint32_t kept = (1u << PER) - 1;
+    if (p.groups > 1) {
+      const Groups g = keep_groups<float, LPT, PER>(p, room, lane, v);
+      kept = g.kept;
+      if (__ballot(g.close)) {
+        exact(g.best);
+        kept = keep_groups<double, LPT, PER>(p, room, lane, w).kept;
+      }
+    }
+    // without a bias the logits decide in the groups that stay, among scores that are numbers
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (!p.bias && v[j] > Keys<float>::kNan) v[j] = Keys<float>::of(l[j]);
+      v[j] = kept >> j & 1 ? v[j] : Keys<float>::kNone;
+    }
+    const bool close = choose<float, LPT, PER>(p, lane, wave_lane, v, chosen[slot], may);
+    if (p.bias && __ballot(close)) {
+      exact(may);
+      choose<double, LPT, PER>(p, lane, wave_lane, w, chosen[slot], may);
+    }
   }
-  __syncthreads();
+  wave_sync();
 
   // the weights, a lane a choice
   float w[kMaxTopk / LPT], sum = 0.0f;
@@ -255,30 +431,30 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
   }
 }
 
-template <class T, class F, int LPT, int PER>
+template <class T, bool WIDE, int LPT, int PER>
 int launch_route(wgb_ctx *ctx, const RouteArgs &p) {
   constexpr int TOKENS = 256 / LPT;
-  const size_t lds = p.groups > 1 ? TOKENS * (sizeof(F) * (((p.experts + 1) & ~1) + p.groups) + kMaxGroups) : 0;
-  route_kernel<T, F, LPT, PER><<<(unsigned)((p.n + TOKENS - 1) / TOKENS), 256, lds, ctx->stream>>>(p);
+  const size_t room = WIDE ? Room<double>::bytes(p.experts, p.groups) : p.groups > 1 ? Room<int>::bytes(p.experts, p.groups) : 0;
+  route_kernel<T, WIDE, LPT, PER><<<(unsigned)((p.n + TOKENS - 1) / TOKENS), 256, TOKENS * room, ctx->stream>>>(p);
   WGB_CHECK_LAUNCH("route_kernel");
   return WGB_OK;
 }
 
-template <class T, class F>
+template <class T, bool WIDE>
 int route_sizes(wgb_ctx *ctx, const RouteArgs &p) {
-  if (p.experts <= 16) return launch_route<T, F, 16, 1>(ctx, p);
-  if (p.experts <= 32) return launch_route<T, F, 16, 2>(ctx, p);
-  if (p.experts <= 64) return launch_route<T, F, 16, 4>(ctx, p);
-  if (p.experts <= 128) return launch_route<T, F, 16, 8>(ctx, p);
-  if (p.experts <= 256) return launch_route<T, F, 16, 16>(ctx, p);
-  if (p.experts <= 512) return launch_route<T, F, 64, 8>(ctx, p);
-  return launch_route<T, F, 64, 16>(ctx, p);
+  if (p.experts <= 16) return launch_route<T, WIDE, 16, 1>(ctx, p);
+  if (p.experts <= 32) return launch_route<T, WIDE, 16, 2>(ctx, p);
+  if (p.experts <= 64) return launch_route<T, WIDE, 16, 4>(ctx, p);
+  if (p.experts <= 128) return launch_route<T, WIDE, 16, 8>(ctx, p);
+  if (p.experts <= 256) return launch_route<T, WIDE, 16, 16>(ctx, p);
+  if (p.experts <= 512) return launch_route<T, WIDE, 64, 8>(ctx, p);
+  return launch_route<T, WIDE, 64, 16>(ctx, p);
 }
 
 template <class T>
 int route(wgb_ctx *ctx, const RouteArgs &p) {
   const bool wide = p.bias || (p.groups > 1 && p.best == 2);
-  return wide ? route_sizes<T, double>(ctx, p) : route_sizes<T, float>(ctx, p);
+  return wide ? route_sizes<T, true>(ctx, p) : route_sizes<T, false>(ctx, p);
 }
 
 // ---- its gradient -----------------------------------------------------------------
@@ -457,31 +633,35 @@ __global__ __launch_bounds__(1024) void order_count_kernel(const int32_t *ids, i
 __global__ __launch_bounds__(1024) void order_place_kernel(const int32_t *ids, int64_t pairs, int64_t chunk, int experts,
                                                            int bits, const int32_t *counts, int blocks, int64_t *offsets,
                                                            int32_t *places, int32_t *sorted) {
-  // next[e]: where the block's next pair of expert e goes; in a round, of[w][e] pairs of wave w's
+  // next[e]: where the block's next pair of expert e goes; in a round, of[w * experts + e] pairs of wave w's
   __shared__ int32_t next[kMaxExperts], all[kMaxExperts], sums[16];
-  __shared__ uint16_t of[16][kMaxExperts];
+  __shared__ __align__(16) uint16_t of[16 * kMaxExperts];
   const int t = threadIdx.x, threads = blockDim.x, lane = t & 63, wave = t >> 6, waves = threads >> 6;
   const int64_t begin = blockIdx.x * chunk, end = begin + chunk < pairs ? begin + chunk : pairs;
-  for (int e = t; e < experts; e += threads) next[e] = all[e] = 0;
+  int e = expert_of(ids, begin + t, end, experts);  // of the round's pair
+  for (int i = t; i < experts; i += threads) next[i] = all[i] = 0;
+  typedef int v4i __attribute__((ext_vector_type(4)));
+  const int clear = (waves * experts * 2 + 15) / 16;
+  for (int i = t; i < clear; i += threads) reinterpret_cast<v4i *>(of)[i] = v4i{0, 0, 0, 0};
   __syncthreads();
   if (blocks == 1) {
     for (int64_t p = t; p < end; p += threads) {
-      const int e = expert_of(ids, p, end, experts);
-      if (e >= 0) atomicAdd(&all[e], 1);
+      const int x = expert_of(ids, p, end, experts);
+      if (x >= 0) atomicAdd(&all[x], 1);
     }
   } else {
-    // threads / width rows of counts at once
-    const int width = 1 << bits, step = threads >> bits;
-    const int e = t & (width - 1);
-    if (e < experts) {
+    // threads / width rows of counts at once, all of a thread's loads under way together
+    const int width = 1 << bits, step = threads >> bits, x = t & (width - 1), b0 = t >> bits;
+    if (x < experts) {
       int before = 0, sum = 0;
-      for (int b = t >> bits; b < blocks; b += step) {
-        const int c = counts[(int64_t)b * experts + e];
+#pragma unroll 16
+      for (int b = b0; b < blocks; b += step) {
+        const int c = counts[(int64_t)b * experts + x];
         sum += c;
         before += b < (int)blockIdx.x ? c : 0;
       }
-      atomicAdd(&all[e], sum);
-      atomicAdd(&next[e], before);
+      atomicAdd(&all[x], sum);
+      atomicAdd(&next[x], before);
     }
   }
   __syncthreads();
@@ -507,8 +687,6 @@ __global__ __launch_bounds__(1024) void order_place_kernel(const int32_t *ids, i
 
   for (int64_t p0 = begin; p0 < end; p0 += threads) {
     const int64_t p = p0 + t;
-    const int e = expert_of(ids, p, end, experts);
-    for (int i = t; i < waves * experts; i += threads) of[i / experts][i % experts] = 0;
     // lanes with the same expert
     uint64_t same = __ballot(e >= 0);
     for (int b = 0; b < bits; ++b) {
@@ -516,22 +694,29 @@ __global__ __launch_bounds__(1024) void order_place_kernel(const int32_t *ids, i
       same &= (e >> b) & 1 ? set : ~set;
     }
     const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
-    __syncthreads();
-    if (e >= 0 && rank == 0) of[wave][e] = (uint16_t)__popcll(same);
+    if (e >= 0 && rank == 0) of[wave * experts + e] = (uint16_t)__popcll(same);
     __syncthreads();
     int place = -1;
     if (e >= 0) {
       place = next[e] + rank;
-      for (int w = 0; w < wave; ++w) place += of[w][e];
+      for (int w = 0; w < wave; ++w) place += of[w * experts + e];
       sorted[place] = (int32_t)p;
     }
     if (p < end) {
       places[p] = place;
       if (p >= total) sorted[p] = -1;  // behind the last group
     }
+    if (p0 + threads >= end) break;
+    e = expert_of(ids, p + threads, end, experts);
     __syncthreads();
-    for (int x = t; x < experts; x += threads)
-      for (int w = 0; w < waves; ++w) next[x] += of[w][x];
+    for (int x = t; x < experts; x += threads) {
+      int here = 0;
+      for (int w = 0; w < waves; ++w) {
+        here += of[w * experts + x];
+        of[w * experts + x] = 0;
+      }
+      next[x] += here;
+    }
     __syncthreads();
   }
 }
@@ -812,8 +997,8 @@ extern "C" int wgb_route_order(wgb_ctx *ctx, int64_t experts, int64_t n, int64_t
   const int64_t count = n * topk;
   int bits = 0;
   while ((1 << bits) < experts) ++bits;
-  // at most 256 blocks, each of whole rounds of 1024 pairs
-  int64_t chunk = (count + 255) / 256;
+  // at most 64 blocks, each of whole rounds of 1024 pairs: every block reads all counts
+  int64_t chunk = (count + 63) / 64;
   chunk = (chunk + 1023) / 1024 * 1024;
   const int blocks = count > 1024 ? (int)((count + chunk - 1) / chunk) : 1;
   int threads = 1024;
