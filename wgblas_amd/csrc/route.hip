@@ -737,18 +737,42 @@ struct RowsArgs {
   int shift;  // 2^shift threads a token
 };
 
-template <class T>
+// STREAM: non-temporal accesses, where the rows are more than the L2 caches
+// hold. With 49152 rows of 2048 bf16 values (201 MB), read in any order, their
+// sums take 44 us instead of 63, the gradients 87 instead of 110.
+// Only for rows at whole dwords: at halves they are slower than plain ones.
+template <class T, bool STREAM>
 struct Lanes {
   static constexpr int V = 16 / sizeof(T);  // elements of a 16-byte access
+  typedef int Raw __attribute__((ext_vector_type(4), aligned(4)));
+  typedef int Any __attribute__((ext_vector_type(4), aligned(2)));
   struct __attribute__((packed, aligned(sizeof(T)))) Vec {
     T v[V];
   };
+  // As dwords: made values of at the load they would be waited for there.
+  static __device__ __forceinline__ Raw get(const T *x) {
+    if constexpr (STREAM)
+      return __builtin_nontemporal_load(reinterpret_cast<const Raw *>(x));
+    else
+      return *reinterpret_cast<const Any *>(x);
+  }
+  static __device__ __forceinline__ void put(T *x, const Vec &v) {
+    if constexpr (STREAM) {
+      const Raw raw = __builtin_bit_cast(Raw, v);
+      __builtin_nontemporal_store(raw, reinterpret_cast<Raw *>(x));
+    } else {
+      *reinterpret_cast<Vec *>(x) = v;
+    }
+  }
+  static __device__ __forceinline__ void widen(const Raw &raw, float (&f)[V]) {
+    const Vec v = __builtin_bit_cast(Vec, raw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = (float)v.v[i];
+  }
   // up to `left` elements at x, as floats
   static __device__ __forceinline__ void load(const T *x, int64_t left, float (&f)[V]) {
     if (left >= V) {
-      const Vec v = *reinterpret_cast<const Vec *>(x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = (float)v.v[i];
+      widen(get(x), f);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] = i < left ? (float)x[i] : 0.0f;
@@ -759,7 +783,7 @@ struct Lanes {
       Vec v;
 #pragma unroll
       for (int i = 0; i < V; ++i) v.v[i] = (T)f[i];
-      *reinterpret_cast<Vec *>(x) = v;
+      put(x, v);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i)
@@ -768,119 +792,214 @@ struct Lanes {
   }
 };
 
+// Up to S of a token's slots from s0 on: their columns (-1: none, or outside)
+// and weights. A thread's loads of them and of their rows are under way together.
+template <int S>
+struct Slots {
+  int64_t place[S];
+  float w[S];
+  __device__ __forceinline__ void load(const RowsArgs &p, int64_t token, int s0) {
+    const int64_t columns = p.n * p.topk, at = token * p.topk + s0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const bool there = s0 + s < p.topk;
+      place[s] = there ? p.places[at + s] : -1;
+      w[s] = there && p.weights ? p.weights[at + s] : 1.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (place[s] >= columns) place[s] = -1;
+  }
+};
+constexpr int kSlots = 8;
+
 // Y(:, places[s, t]) = w X(:, t): a token's row is read once and stored topk
 // times. Bound by those stores.
-template <class T>
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void gather_kernel(RowsArgs p) {
-  typedef Lanes<T> L;
+  typedef Lanes<T, STREAM> L;
   const int lanes = 1 << p.shift, lane = threadIdx.x & (lanes - 1);
-  const int64_t token = (int64_t)blockIdx.x * (256 >> p.shift) + (threadIdx.x >> p.shift);
+  const int64_t token = (int64_t)blockIdx.x * (blockDim.x >> p.shift) + (threadIdx.x >> p.shift);
   if (token >= p.n) return;
-  const int64_t columns = p.n * p.topk;
-  const int32_t *places = p.places + token * p.topk;
   const T *x = (const T *)p.X + token * p.ldx;
   for (int64_t at = ((int64_t)blockIdx.y * lanes + lane) * L::V; at < p.d; at += (int64_t)gridDim.y * lanes * L::V) {
     float f[L::V];
-    L::load(x + at, p.d - at, f);
-    for (int s = 0; s < p.topk; ++s) {
-      const int64_t place = places[s];
-      if (place < 0 || place >= columns) continue;
-      float g[L::V];
-      const float w = p.weights ? p.weights[token * p.topk + s] : 1.0f;
+    Lanes<T, false>::load(x + at, p.d - at, f);
+    for (int s0 = 0; s0 < p.topk; s0 += kSlots) {
+      Slots<kSlots> slots;
+      slots.load(p, token, s0);
 #pragma unroll
-      for (int i = 0; i < L::V; ++i) g[i] = w * f[i];
-      L::store((T *)p.out + place * p.ldo + at, p.d - at, g);
+      for (int s = 0; s < kSlots; ++s) {
+        if (slots.place[s] < 0) continue;
+        float g[L::V];
+#pragma unroll
+        for (int i = 0; i < L::V; ++i) g[i] = slots.w[s] * f[i];
+        L::store((T *)p.out + slots.place[s] * p.ldo + at, p.d - at, g);
+      }
     }
   }
 }
 
 // C(:, t) = sum over s of w Y(:, places[s, t]) + beta C(:, t), in the slots'
 // order, in fp32. Bound by reading Y.
-template <class T, class C>
+template <class T, class C, bool STREAM>
 __global__ __launch_bounds__(256) void combine_kernel(RowsArgs p) {
-  typedef Lanes<T> L;
+  typedef Lanes<T, STREAM> L;
   const int lanes = 1 << p.shift, lane = threadIdx.x & (lanes - 1);
-  const int64_t token = (int64_t)blockIdx.x * (256 >> p.shift) + (threadIdx.x >> p.shift);
+  const int64_t token = (int64_t)blockIdx.x * (blockDim.x >> p.shift) + (threadIdx.x >> p.shift);
   if (token >= p.n) return;
-  const int64_t columns = p.n * p.topk;
-  const int32_t *places = p.places + token * p.topk;
   C *c = (C *)p.out + token * p.ldo;
   for (int64_t at = ((int64_t)blockIdx.y * lanes + lane) * L::V; at < p.d; at += (int64_t)gridDim.y * lanes * L::V) {
     float sum[L::V];
 #pragma unroll
     for (int i = 0; i < L::V; ++i) sum[i] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < p.topk; ++s) {
-      const int64_t place = places[s];
-      if (place < 0 || place >= columns) continue;
-      float f[L::V];
-      L::load((const T *)p.Y + place * p.ldy + at, p.d - at, f);
-      const float w = p.weights ? p.weights[token * p.topk + s] : 1.0f;
+    const bool whole = p.d - at >= L::V;
+    for (int s0 = 0; s0 < p.topk; s0 += kSlots) {
+      Slots<kSlots> slots;
+      slots.load(p, token, s0);
+      if (whole) {
+        typename L::Raw y[kSlots];
 #pragma unroll
-      for (int i = 0; i < L::V; ++i) sum[i] = fmaf(w, f[i], sum[i]);
+        for (int s = 0; s < kSlots; ++s)
+          if (slots.place[s] >= 0) y[s] = L::get((const T *)p.Y + slots.place[s] * p.ldy + at);
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s) {
+          if (slots.place[s] < 0) continue;
+          float f[L::V];
+          L::widen(y[s], f);
+#pragma unroll
+          for (int i = 0; i < L::V; ++i) sum[i] = fmaf(slots.w[s], f[i], sum[i]);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s) {
+          if (slots.place[s] < 0) continue;
+          float f[L::V];
+          L::load((const T *)p.Y + slots.place[s] * p.ldy + at, p.d - at, f);
+#pragma unroll
+          for (int i = 0; i < L::V; ++i) sum[i] = fmaf(slots.w[s], f[i], sum[i]);
+        }
+      }
     }
+    if (p.beta != 0.0f) {
 #pragma unroll
-    for (int i = 0; i < L::V; ++i)
-      if (at + i < p.d) c[at + i] = (C)(p.beta != 0.0f ? fmaf(p.beta, (float)c[at + i], sum[i]) : sum[i]);
+      for (int i = 0; i < L::V; ++i)
+        if (at + i < p.d) sum[i] = fmaf(p.beta, (float)c[at + i], sum[i]);
+    }
+    if (whole) {
+      struct __attribute__((packed, aligned(sizeof(C)))) Out {
+        C v[L::V];
+      } out;
+#pragma unroll
+      for (int i = 0; i < L::V; ++i) out.v[i] = (C)sum[i];
+      *reinterpret_cast<Out *>(c + at) = out;
+    } else {
+#pragma unroll
+      for (int i = 0; i < L::V; ++i)
+        if (at + i < p.d) c[at + i] = (C)sum[i];
+    }
   }
 }
 
 // dY(:, places[s, t]) = w dC(:, t) and dw[s, t] = <Y(:, places[s, t]), dC(:,
-// t)>: 256 threads a token, eight slots at a time; their sums are folded in a
-// fixed order.
-template <class T>
+// t)>: eight slots at a time, their rows' loads under way together; the threads'
+// sums are folded in a fixed order.
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void combine_grad_kernel(RowsArgs p) {
-  typedef Lanes<T> L;
-  constexpr int S = 8;
-  __shared__ float sums[4][S];
-  const int64_t token = blockIdx.x, columns = p.n * p.topk;
+  typedef Lanes<T, STREAM> L;
+  __shared__ float sums[4][kSlots];
+  const int64_t token = blockIdx.x;
   const int t = threadIdx.x;
-  const int32_t *places = p.places + token * p.topk;
   const T *dc = (const T *)p.X + token * p.ldx;
-  for (int s0 = 0; s0 < p.topk; s0 += S) {
-    float dot[S], w[S];
-    int64_t place[S];
+  for (int s0 = 0; s0 < p.topk; s0 += kSlots) {
+    Slots<kSlots> slots;
+    slots.load(p, token, s0);
+    float dot[kSlots];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      dot[s] = 0.0f;
-      place[s] = s0 + s < p.topk ? places[s0 + s] : -1;
-      if (place[s] >= columns) place[s] = -1;
-      w[s] = place[s] >= 0 ? p.weights[token * p.topk + s0 + s] : 0.0f;
-    }
-    for (int64_t at = (int64_t)t * L::V; at < p.d; at += 256 * L::V) {
+    for (int s = 0; s < kSlots; ++s) dot[s] = 0.0f;
+    for (int64_t at = (int64_t)t * L::V; at < p.d; at += (int64_t)blockDim.x * L::V) {
       float f[L::V];
-      L::load(dc + at, p.d - at, f);
+      if (p.d - at >= L::V) {
+        const auto own = Lanes<T, false>::get(dc + at);
+        typename L::Raw y[kSlots];
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (place[s] < 0) continue;
-        float y[L::V], g[L::V];
-        L::load((const T *)p.Y + place[s] * p.ldy + at, p.d - at, y);
+        for (int s = 0; s < kSlots; ++s)
+          if (slots.place[s] >= 0) y[s] = L::get((const T *)p.Y + slots.place[s] * p.ldy + at);
+        L::widen(own, f);
 #pragma unroll
-        for (int i = 0; i < L::V; ++i) {
-          dot[s] = fmaf(y[i], f[i], dot[s]);
-          g[i] = w[s] * f[i];
+        for (int s = 0; s < kSlots; ++s) {
+          if (slots.place[s] < 0) continue;
+          float v[L::V], g[L::V];
+          L::widen(y[s], v);
+#pragma unroll
+          for (int i = 0; i < L::V; ++i) {
+            dot[s] = fmaf(v[i], f[i], dot[s]);
+            g[i] = slots.w[s] * f[i];
+          }
+          L::store((T *)p.out + slots.place[s] * p.ldo + at, L::V, g);
         }
-        L::store((T *)p.out + place[s] * p.ldo + at, p.d - at, g);
+      } else {
+        Lanes<T, false>::load(dc + at, p.d - at, f);
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s) {
+          if (slots.place[s] < 0) continue;
+          float y[L::V], g[L::V];
+          L::load((const T *)p.Y + slots.place[s] * p.ldy + at, p.d - at, y);
+#pragma unroll
+          for (int i = 0; i < L::V; ++i) {
+            dot[s] = fmaf(y[i], f[i], dot[s]);
+            g[i] = slots.w[s] * f[i];
+          }
+          L::store((T *)p.out + slots.place[s] * p.ldo + at, p.d - at, g);
+        }
       }
     }
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < kSlots; ++s) {
       const float x = over_lanes<64>(dot[s], Sum());
       if ((t & 63) == 0) sums[t >> 6][s] = x;
     }
     __syncthreads();
-    if (t < S && s0 + t < p.topk) p.dweights[token * p.topk + s0 + t] = (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
+    if (t < kSlots && s0 + t < p.topk) {
+      float x = sums[0][t];
+      for (int w = 1; w < (int)blockDim.x >> 6; ++w) x += sums[w][t];
+      p.dweights[token * p.topk + s0 + t] = x;
+    }
     __syncthreads();
   }
 }
 
-// Threads a token (2^shift, at most 256) and blocks along d for rows of d elements of `size` bytes.
-void row_shape(int64_t d, int64_t n, int size, int &shift, dim3 &grid) {
+// Threads of a block and of a token (2^shift), and blocks along d, for rows of
+// d elements of `size` bytes: 256 threads a block, or 64 where that leaves CUs
+// idle (32 tokens of 4096 bf16 values).
+int row_shape(const wgb_ctx *ctx, int64_t d, int64_t n, int size, int &shift, dim3 &grid) {
   const int64_t vectors = (d * size + 15) / 16;
+  const int threads = n * vectors < (int64_t)ctx->num_cus * 512 ? 64 : 256, most = threads == 64 ? 6 : 8;
   shift = 0;
-  while (shift < 8 && ((int64_t)1 << shift) < vectors) ++shift;
-  const int64_t along = (vectors + 255) / 256;
-  grid = dim3((unsigned)((n + (256 >> shift) - 1) / (256 >> shift)), (unsigned)(along < 65535 ? along : 65535));
+  while (shift < most && ((int64_t)1 << shift) < vectors) ++shift;
+  const int64_t along = (vectors + ((int64_t)1 << shift) - 1) >> shift, per = threads >> shift;
+  grid = dim3((unsigned)((n + per - 1) / per), (unsigned)(along < 65535 ? along : 65535));
+  return threads;
+}
+
+// Whether the rows of all pairs are more than the L2 caches hold (8 of 4 MB),
+// and at whole dwords: `parts`, their addresses and leading dimensions in bytes
+// or'ed together.
+bool streams(int type, int64_t d, int64_t n, int64_t topk, uint64_t parts) {
+  return d * n * topk * (type == WGB_F32 ? 4 : 2) > (int64_t)32 << 20 && (parts & 3) == 0;
+}
+uint64_t part(int type, const void *p, int64_t ld) { return (uint64_t)(uintptr_t)p | (uint64_t)ld * (type == WGB_F32 ? 4 : 2); }
+
+// f(a value of the type, std::true_type or std::false_type)
+template <class F>
+void with_type(int type, bool flag, F f) {
+  auto call = [&](auto t) { flag ? f(t, std::true_type()) : f(t, std::false_type()); };
+  if (type == WGB_F32)
+    call(0.0f);
+  else if (type == WGB_F16)
+    call((_Float16)0.0f);
+  else
+    call((__bf16)0.0f);
 }
 
 // ---- checks ----------------------------------------------------------------------------
@@ -1034,14 +1153,11 @@ extern "C" int wgb_route_gather(wgb_ctx *ctx, int type, int64_t d, int64_t n, in
   p.out = Y;
   p.ldo = ldy;
   dim3 grid;
-  row_shape(d, n, type == WGB_F32 ? 4 : 2, p.shift, grid);
+  const int threads = row_shape(ctx, d, n, type == WGB_F32 ? 4 : 2, p.shift, grid);
   wgb::timing_begin(ctx);
-  if (type == WGB_F32)
-    gather_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
-  else if (type == WGB_F16)
-    gather_kernel<_Float16><<<grid, 256, 0, ctx->stream>>>(p);
-  else
-    gather_kernel<__bf16><<<grid, 256, 0, ctx->stream>>>(p);
+  with_type(type, streams(type, d, n, topk, part(type, X, ldx) | part(type, Y, ldy)), [&](auto t, auto stream) {
+    gather_kernel<decltype(t), decltype(stream)::value><<<grid, threads, 0, ctx->stream>>>(p);
+  });
   wgb::timing_end(ctx);
   WGB_CHECK_LAUNCH("gather_kernel");
   return WGB_OK;
@@ -1069,18 +1185,15 @@ extern "C" int wgb_route_combine(wgb_ctx *ctx, int type, int64_t d, int64_t n, i
   p.out = C;
   p.ldo = ldc;
   dim3 grid;
-  row_shape(d, n, type == WGB_F32 ? 4 : 2, p.shift, grid);
+  const int threads = row_shape(ctx, d, n, type == WGB_F32 ? 4 : 2, p.shift, grid);
   wgb::timing_begin(ctx);
-  if (type == WGB_F32)
-    combine_kernel<float, float><<<grid, 256, 0, ctx->stream>>>(p);
-  else if (type == WGB_F16 && ctype == WGB_F16)
-    combine_kernel<_Float16, _Float16><<<grid, 256, 0, ctx->stream>>>(p);
-  else if (type == WGB_F16)
-    combine_kernel<_Float16, float><<<grid, 256, 0, ctx->stream>>>(p);
-  else if (ctype == WGB_BF16)
-    combine_kernel<__bf16, __bf16><<<grid, 256, 0, ctx->stream>>>(p);
-  else
-    combine_kernel<__bf16, float><<<grid, 256, 0, ctx->stream>>>(p);
+  with_type(type, streams(type, d, n, topk, part(type, Y, ldy)), [&](auto t, auto stream) {
+    typedef decltype(t) T;
+    if (ctype == type)
+      combine_kernel<T, T, decltype(stream)::value><<<grid, threads, 0, ctx->stream>>>(p);
+    else
+      combine_kernel<T, float, decltype(stream)::value><<<grid, threads, 0, ctx->stream>>>(p);
+  });
   wgb::timing_end(ctx);
   WGB_CHECK_LAUNCH("combine_kernel");
   return WGB_OK;
@@ -1111,12 +1224,9 @@ extern "C" int wgb_route_combine_grad(wgb_ctx *ctx, int type, int64_t d, int64_t
   p.ldo = lddy;
   p.dweights = dweights;
   wgb::timing_begin(ctx);
-  if (type == WGB_F32)
-    combine_grad_kernel<float><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
-  else if (type == WGB_F16)
-    combine_grad_kernel<_Float16><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
-  else
-    combine_grad_kernel<__bf16><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
+  with_type(type, streams(type, d, n, topk, part(type, dC, lddc) | part(type, Y, ldy) | part(type, dY, lddy)), [&](auto t, auto stream) {
+    combine_grad_kernel<decltype(t), decltype(stream)::value><<<(unsigned)n, 256, 0, ctx->stream>>>(p);
+  });
   wgb::timing_end(ctx);
   WGB_CHECK_LAUNCH("combine_grad_kernel");
   return WGB_OK;
