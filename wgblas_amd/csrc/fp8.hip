@@ -53,6 +53,16 @@ __device__ __forceinline__ void load8(const T *x, int64_t left, float (&f)[8]) {
   }
 }
 
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+// Past the caches, if STREAM.
+template <bool STREAM, class V>
+__device__ __forceinline__ void put(uint8_t *to, V codes) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(codes, reinterpret_cast<V *>(to));
+  else
+    *reinterpret_cast<V *>(to) = codes;
+}
+
 template <int ROR>
 __device__ __forceinline__ uint32_t max_ror(uint32_t x) {
   const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x120 + ROR, 0xf, 0xf, true);
@@ -62,8 +72,10 @@ __device__ __forceinline__ uint32_t max_ror(uint32_t x) {
 __device__ __forceinline__ uint32_t row_max(uint32_t x) { return max_ror<1>(max_ror<2>(max_ror<4>(max_ror<8>(x)))); }
 
 // Blocks of one column, along the contiguous axis: 16 lanes have a block, 8
-// values each. Bound by memory.
-template <class T>
+// values each. Bound by memory. STREAM, here and below: the values are more than
+// the caches hold, and codes are stored past them (bf16 8192 x 4096: 17.8 us,
+// 5.6 TB/s, and 22.4 us through them).
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void quantize_kernel(const T *X, int64_t ldx, int64_t k, int64_t n, uint8_t *codes,
                                                        int64_t ld, float *scales, int64_t lds) {
   const int lane = threadIdx.x & 63;
@@ -75,13 +87,13 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T *X, int64_t ldx, 
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = top_of(top, f[i]);
   const uint32_t scale = scale_bits(row_max(top));
-  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-  *reinterpret_cast<u2 *>(codes + j * ld + k0) = u2{codes4(f, scale), codes4(f + 4, scale)};
+  put<STREAM>(codes + j * ld + k0, u2{codes4(f, scale), codes4(f + 4, scale)});
   if ((lane & 15) == 0) scales[k0 / 128 * lds + j] = __uint_as_float(scale);
 }
 
-// 128 x 128 values a block: 32 columns at a time, 16 lanes a column.
-template <class T>
+// 128 x 128 values a block: 32 columns at a time, 16 lanes a column (f32
+// 8192 x 4096: 29.4 us, 5.7 TB/s).
+template <class T, bool STREAM>
 __global__ __launch_bounds__(512) void quantize_square_kernel(const T *X, int64_t ldx, int64_t k, int64_t n, uint8_t *codes,
                                                               int64_t ld, float *scales, int64_t lds, int blocks_k) {
   __shared__ uint32_t tops[8];
@@ -114,150 +126,202 @@ __global__ __launch_bounds__(512) void quantize_square_kernel(const T *X, int64_
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int64_t j = jb * 128 + q * 32 + (t >> 4);
-    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    if (j < n) *reinterpret_cast<u2 *>(codes + j * ld + k0) = u2{codes4(f[q], scale), codes4(f[q] + 4, scale)};
+    if (j < n) put<STREAM>(codes + j * ld + k0, u2{codes4(f[q], scale), codes4(f[q] + 4, scale)});
   }
   if (t == 0) scales[kb * lds + jb] = __uint_as_float(scale);
 }
 
-// Blocks along the strided axis, 128 x 128 values a block of threads: a lane
-// has two neighbouring columns, a wave 16 rows of k. The codes go through LDS
-// (16-byte chunks at chunk ^ column, no two lanes of a quarter wave in the
-// same banks) and out as 128-byte lines.
-template <class T, bool SQUARE>
+// Blocks along the strided axis, 128 x 128 values a block of threads: a wave has
+// 16 rows of k, a lane 16 bytes of neighbouring columns in some of them, so that
+// loads are as wide as those along the contiguous axis (two columns a lane and
+// 16 rows: 2.9 TB/s). A lane's codes of a column, RG rows of k, go through LDS
+// (four dwords more after every lane's columns: two lanes in a bank) and out as
+// 128-byte lines. STREAM loads past the caches (bf16 16384 x 4096: 43 us,
+// 4.7 TB/s, and 50 us through them; stores past them too: 45 us).
+template <class T, bool SQUARE, bool STREAM>
 __global__ __launch_bounds__(512) void quantize_strided_kernel(const T *X, int64_t ldx, int64_t k, int64_t n,
                                                                uint8_t *codes, int64_t ld, float *scales, int64_t lds,
                                                                int blocks_k) {
-  __shared__ v4i lines[128][8];
+  constexpr int V = 16 / sizeof(T), LR = 128 / V, G = 64 / LR, RG = 16 / G;  // columns, lanes a row, rows at once, a lane's rows
+  __shared__ __attribute__((aligned(16))) uint32_t lines[128 * 32 + 4 * LR];
   __shared__ uint32_t tops[8][128];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, g = lane / LR, c0 = lane % LR * V;
   const int kb = (int)(blockIdx.x % blocks_k);
-  const int64_t j0 = blockIdx.x / blocks_k * 128, j = j0 + 2 * lane, k0 = (int64_t)kb * 128 + wave * 16;
-  struct __attribute__((packed, aligned(sizeof(T)))) Two {
-    T v[2];
+  const int64_t j0 = blockIdx.x / blocks_k * 128, j = j0 + c0, k0 = (int64_t)kb * 128 + wave * 16 + g * RG;
+  typedef int Any __attribute__((ext_vector_type(4), aligned(2)));
+  struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+    T v[V];
   };
   const T *x = X + k0 * ldx + j;
-  float f[2][16];
+  Any raw[RG];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    f[0][r] = f[1][r] = 0.0f;
+  for (int r = 0; r < RG; ++r) {
+    raw[r] = Any{0, 0, 0, 0};
     if (k0 + r >= k) continue;
-    if (j + 1 < n) {
-      const Two v = *reinterpret_cast<const Two *>(x + r * ldx);
-      f[0][r] = (float)v.v[0];
-      f[1][r] = (float)v.v[1];
+    if (j + V <= n) {
+      const Any *from = reinterpret_cast<const Any *>(x + r * ldx);
+      if constexpr (STREAM)
+        raw[r] = __builtin_nontemporal_load(from);
+      else
+        raw[r] = *from;
     } else if (j < n) {
-      f[0][r] = (float)x[r * ldx];
+      Vec v;
+#pragma unroll
+      for (int c = 0; c < V; ++c) v.v[c] = j + c < n ? x[r * ldx + c] : (T)0.0f;
+      raw[r] = __builtin_bit_cast(Any, v);
     }
   }
+  float f[V][RG];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int r = 0; r < RG; ++r) {
+    const Vec v = __builtin_bit_cast(Vec, raw[r]);
+#pragma unroll
+    for (int c = 0; c < V; ++c) f[c][r] = (float)v.v[c];
+  }
+  // the columns' largest: of the lane, of the wave's lanes with the same columns, of the waves
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
     uint32_t top = 0;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = top_of(top, f[c][r]);
-    tops[wave][2 * lane + c] = top;
+    for (int r = 0; r < RG; ++r) top = top_of(top, f[c][r]);
+#pragma unroll
+    for (int d = LR; d < 64; d <<= 1) {
+      const uint32_t other = (uint32_t)__shfl_xor((int)top, d);
+      top = top > other ? top : other;
+    }
+    if (g == 0) tops[wave][c0 + c] = top;
   }
   __syncthreads();
-  uint32_t scale[2];
+  uint32_t scale[V];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t top = 0;
+  for (int c = 0; c < V; ++c) {
+    scale[c] = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) top = top > tops[w][2 * lane + c] ? top : tops[w][2 * lane + c];
-    scale[c] = top;
+    for (int w = 0; w < 8; ++w) scale[c] = scale[c] > tops[w][c0 + c] ? scale[c] : tops[w][c0 + c];
   }
   if constexpr (SQUARE) {
-    uint32_t top = scale[0] > scale[1] ? scale[0] : scale[1];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < V; ++c) top = top > scale[c] ? top : scale[c];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t other = (uint32_t)__shfl_xor((int)top, d);
       top = top > other ? top : other;
     }
-    scale[0] = scale[1] = top;
+#pragma unroll
+    for (int c = 0; c < V; ++c) scale[c] = top;
   }
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < V; ++c) {
     scale[c] = scale_bits(scale[c]);
-    v4i out;
+    uint32_t *line = lines + (c0 + c) * 32 + lane % LR * 4 + wave * 4 + g * (RG / 4);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) out[q] = (int)codes4(f[c] + 4 * q, scale[c]);
-    lines[2 * lane + c][wave ^ (lane & 7)] = out;
+    for (int q = 0; q < RG / 4; ++q) line[q] = codes4(f[c] + 4 * q, scale[c]);
   }
-  if (wave == 0) {
+  if (wave == 0 && g == 0) {
     if constexpr (SQUARE) {
       if (lane == 0) scales[kb * lds + j0 / 128] = __uint_as_float(scale[0]);
     } else {
-      if (j < n) scales[kb * lds + j] = __uint_as_float(scale[0]);
-      if (j + 1 < n) scales[kb * lds + j + 1] = __uint_as_float(scale[1]);
+#pragma unroll
+      for (int c = 0; c < V; ++c)
+        if (j + c < n) scales[kb * lds + j + c] = __uint_as_float(scale[c]);
     }
   }
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int col = (t >> 3) + 64 * q, chunk = t & 7;
-    if (j0 + col < n) *reinterpret_cast<v4i *>(codes + (j0 + col) * ld + kb * 128 + chunk * 16) = lines[col][chunk ^ ((col >> 1) & 7)];
+    if (j0 + col < n)
+      put<false>(codes + (j0 + col) * ld + kb * 128 + chunk * 16, *reinterpret_cast<const v4i *>(lines + col * 32 + (col / V + chunk) * 4));
   }
 }
 
-// A lane has 8 codes of a column: code * scale in fp32, rounded to the
-// output's type. Bound by memory.
-template <class T>
+// A lane has 16 bytes of output: code * scale in fp32, rounded to the output's
+// type. Bound by memory. STREAM: the output is more than the caches hold, and
+// stored past them (bf16 8192 x 4096: 17.0 us, 5.9 TB/s, and 29.7 us through
+// them); at whole dwords only.
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t *codes, int64_t ld, const float *scales, int64_t lds,
                                                          int shift, int64_t k, int64_t n, T *X, int64_t ldx) {
-  const int lane = threadIdx.x & 63;
-  const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), k0 = (int64_t)blockIdx.y * 512 + lane * 8;
+  constexpr int V = 16 / sizeof(T);
+  const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), k0 = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * V;
   if (j >= n || k0 >= k) return;
-  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-  const u2 q = *reinterpret_cast<const u2 *>(codes + j * ld + k0);
+  struct __attribute__((aligned(V))) Dwords {
+    uint32_t d[V / 4];
+  };
+  const Dwords q = *reinterpret_cast<const Dwords *>(codes + j * ld + k0);
   const float scale = scales[k0 / 128 * lds + (j >> shift)];
-  Eight<T> v;
+  struct __attribute__((packed, aligned(sizeof(T)))) Vec {
+    T v[V];
+  } v;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const f2v lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[c], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[c], true);
-    v.v[4 * c] = (T)(lo[0] * scale);
-    v.v[4 * c + 1] = (T)(lo[1] * scale);
-    v.v[4 * c + 2] = (T)(hi[0] * scale);
-    v.v[4 * c + 3] = (T)(hi[1] * scale);
+  for (int h = 0; h < V / 4; ++h) {
+    const f2v lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.d[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.d[h], true);
+    v.v[4 * h] = (T)(lo[0] * scale);
+    v.v[4 * h + 1] = (T)(lo[1] * scale);
+    v.v[4 * h + 2] = (T)(hi[0] * scale);
+    v.v[4 * h + 3] = (T)(hi[1] * scale);
   }
   T *x = X + j * ldx + k0;
-  if (k - k0 >= 8) {
-    *reinterpret_cast<Eight<T> *>(x) = v;
+  if (k - k0 >= V) {
+    typedef int Any __attribute__((ext_vector_type(4), aligned(4)));
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(__builtin_bit_cast(Any, v), reinterpret_cast<Any *>(x));
+    else
+      *reinterpret_cast<Vec *>(x) = v;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < V; ++i)
       if (i < k - k0) x[i] = v.v[i];
   }
 }
 
 int64_t blocks128(int64_t k) { return (k + 127) / 128; }
-
+// More than the caches hold: 8 L2 caches of 4 MB.
 template <class T>
+bool streams(int64_t k, int64_t n) {
+  return k * n * (int64_t)sizeof(T) > (int64_t)32 << 20;
+}
+
+template <class T, bool STREAM>
 int quantize(wgb_ctx *ctx, int trans, int block, int64_t k, int64_t n, const void *X, int64_t ldx, uint8_t *codes,
              int64_t ld, float *scales, int64_t lds) {
   const int blocks_k = (int)blocks128(k);
   const int64_t tiles = blocks_k * blocks128(n);
   if ((trans == WGB_TRANS || block == 128) && tiles > INT32_MAX)
     return fail(WGB_ERR_INVALID_VALUE, "wgb_fp8_quantize: too many blocks");
+  const T *x = (const T *)X;
   if (trans == WGB_TRANS) {
     if (block == 128)
-      quantize_strided_kernel<T, true><<<(unsigned)tiles, 512, 0, ctx->stream>>>((const T *)X, ldx, k, n, codes, ld, scales, lds, blocks_k);
+      quantize_strided_kernel<T, true, STREAM><<<(unsigned)tiles, 512, 0, ctx->stream>>>(x, ldx, k, n, codes, ld, scales, lds, blocks_k);
     else
-      quantize_strided_kernel<T, false><<<(unsigned)tiles, 512, 0, ctx->stream>>>((const T *)X, ldx, k, n, codes, ld, scales, lds, blocks_k);
+      quantize_strided_kernel<T, false, STREAM><<<(unsigned)tiles, 512, 0, ctx->stream>>>(x, ldx, k, n, codes, ld, scales, lds, blocks_k);
   } else if (block == 128) {
-    quantize_square_kernel<T><<<(unsigned)tiles, 512, 0, ctx->stream>>>((const T *)X, ldx, k, n, codes, ld, scales, lds, blocks_k);
+    quantize_square_kernel<T, STREAM><<<(unsigned)tiles, 512, 0, ctx->stream>>>(x, ldx, k, n, codes, ld, scales, lds, blocks_k);
   } else {
     const dim3 grid((unsigned)((n + 3) / 4), (unsigned)((k + 511) / 512));
-    quantize_kernel<T><<<grid, 256, 0, ctx->stream>>>((const T *)X, ldx, k, n, codes, ld, scales, lds);
+    quantize_kernel<T, STREAM><<<grid, 256, 0, ctx->stream>>>(x, ldx, k, n, codes, ld, scales, lds);
   }
   WGB_CHECK_LAUNCH("wgb_fp8_quantize");
   return WGB_OK;
 }
 
 template <class T>
+int quantize_as(wgb_ctx *ctx, int trans, int block, int64_t k, int64_t n, const void *X, int64_t ldx, uint8_t *codes,
+                int64_t ld, float *scales, int64_t lds) {
+  return (streams<T>(k, n) ? quantize<T, true> : quantize<T, false>)(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds);
+}
+
+template <class T>
 int dequantize(wgb_ctx *ctx, int block, int64_t k, int64_t n, const uint8_t *codes, int64_t ld, const float *scales,
                int64_t lds, void *X, int64_t ldx) {
-  const dim3 grid((unsigned)((n + 3) / 4), (unsigned)((k + 511) / 512));
-  dequantize_kernel<T><<<grid, 256, 0, ctx->stream>>>(codes, ld, scales, lds, block == 128 ? 7 : 0, k, n, (T *)X, ldx);
+  const int shift = block == 128 ? 7 : 0, along = (int)((k * sizeof(T) + 1023) / 1024);
+  const bool stream = streams<T>(k, n) && (((uintptr_t)X | ldx * sizeof(T)) & 3) == 0;
+  const dim3 grid((unsigned)((n + 3) / 4), (unsigned)along);
+  if (stream)
+    dequantize_kernel<T, true><<<grid, 256, 0, ctx->stream>>>(codes, ld, scales, lds, shift, k, n, (T *)X, ldx);
+  else
+    dequantize_kernel<T, false><<<grid, 256, 0, ctx->stream>>>(codes, ld, scales, lds, shift, k, n, (T *)X, ldx);
   WGB_CHECK_LAUNCH("wgb_fp8_dequantize");
   return WGB_OK;
 }
@@ -415,9 +479,9 @@ extern "C" int wgb_fp8_quantize(wgb_ctx *ctx, int type, int trans, int block, in
   if (k == 0 || n == 0) return WGB_OK;
   if (!X) return fail(WGB_ERR_INVALID_VALUE, "X is null");
   wgb::timing_begin(ctx);
-  st = type == WGB_F32   ? quantize<float>(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds)
-       : type == WGB_F16 ? quantize<_Float16>(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds)
-                         : quantize<__bf16>(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds);
+  st = type == WGB_F32   ? quantize_as<float>(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds)
+       : type == WGB_F16 ? quantize_as<_Float16>(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds)
+                         : quantize_as<__bf16>(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds);
   wgb::timing_end(ctx);
   return st;
 }
