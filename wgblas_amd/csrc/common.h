@@ -122,6 +122,14 @@ int check_gemm(int uplo, bool want_uplo, int transA, int transB, int64_t m, int6
                const void *A, int64_t lda, const void *B, int64_t ldb, const void *C,
                int64_t ldc);
 
+// x as it is in fp32: keeps a product from being rounded to f16 in one step
+// with its conversion (v_fma_mixlo), which the compiler does at some places of
+// a kernel and not at others, so that a value's bits would hang on where it lies.
+__device__ __forceinline__ float in_fp32(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 }  // namespace wgb
 
 #define WGB_CHECK_HIP(expr)                               \

@@ -257,10 +257,10 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t *codes, i
 #pragma unroll
   for (int h = 0; h < V / 4; ++h) {
     const f2v lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.d[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.d[h], true);
-    v.v[4 * h] = (T)(lo[0] * scale);
-    v.v[4 * h + 1] = (T)(lo[1] * scale);
-    v.v[4 * h + 2] = (T)(hi[0] * scale);
-    v.v[4 * h + 3] = (T)(hi[1] * scale);
+    v.v[4 * h] = (T)wgb::in_fp32(lo[0] * scale);
+    v.v[4 * h + 1] = (T)wgb::in_fp32(lo[1] * scale);
+    v.v[4 * h + 2] = (T)wgb::in_fp32(hi[0] * scale);
+    v.v[4 * h + 3] = (T)wgb::in_fp32(hi[1] * scale);
   }
   T *x = X + j * ldx + k0;
   if (k - k0 >= V) {

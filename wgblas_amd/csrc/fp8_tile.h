@@ -77,26 +77,24 @@ __device__ __forceinline__ v2i read_transposed(const char *__restrict__ at) {
 }
 
 // The MFMA operands of a k-tile for MB blocks of 16 rows, `STEP` rows apart,
-// from row `wrow`; only the first `used` blocks.
+// from row `wrow`.
 template <int BT, bool MC, int MB, int STEP = 16>
-__device__ __forceinline__ void fetch_codes(const char *stage, int wrow, int lane, v8i (&out)[MB], int used = MB) {
+__device__ __forceinline__ void fetch_codes(const char *stage, int wrow, int lane, v8i (&out)[MB]) {
   const int i16 = lane & 15, g = lane >> 4;
   if constexpr (!MC) {
     const int lo = (g ^ (i16 & 7)) * 16, hi = ((4 + g) ^ (i16 & 7)) * 16;
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
-      if (b == 0 || __builtin_expect(b < used, 1)) {
-        const char *row = stage + (wrow + STEP * b + i16) * TB;
-        const v4i x = *reinterpret_cast<const v4i *>(row + lo), y = *reinterpret_cast<const v4i *>(row + hi);
-        out[b] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      }
+    for (int b = 0; b < MB; ++b) {
+      const char *row = stage + (wrow + STEP * b + i16) * TB;
+      const v4i x = *reinterpret_cast<const v4i *>(row + lo), y = *reinterpret_cast<const v4i *>(row + hi);
+      out[b] = v8i{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    }
   } else {
     const int kr = 16 * g + (i16 >> 1);
     int at = kr * BT + ((wrow ^ (mc_key<8, BT / 16>(kr) << 4)) + (i16 & 1) * 8);
     asm volatile("" : "+v"(at));  // one register, not one for every block
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
-      if (b > 0 && __builtin_expect(b >= used, 0)) break;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const v2i x = read_transposed(stage + (at ^ (STEP * b)) + (64 * (q >> 1) + 8 * (q & 1)) * BT);
@@ -156,39 +154,31 @@ struct BlockScaleStager {
 
 // The products of some row blocks with all column blocks, added to the sums.
 // sb: the columns' scales; ROWS: A has a scale for each row (sa[i]: of the
-// lane's four rows of block i), else the one for all is in sb. A block's products are scaled while the next
-// ones are multiplied: the scheduler, left to itself, puts the v_fma right
-// behind its MFMA and waits for it. FULL: all column blocks are used.
-template <bool EXACT, bool ROWS, int MB, int NB, int FIRST, int COUNT, bool FULL = true>
+// lane's four rows of block i), else the one for all is in sb. A block's
+// products are scaled while the next ones are multiplied: the scheduler, left
+// to itself, puts the v_fma right behind its MFMA and waits for it.
+template <bool EXACT, bool ROWS, int MB, int NB, int FIRST, int COUNT>
 __device__ __forceinline__ void multiply_codes(const v8i (&a)[COUNT], const typename Codes<EXACT>::wide (&b)[NB],
-                                               f4 (&acc)[MB][NB], const f4 (&sa)[ROWS ? COUNT : 1], const float (&sb)[NB],
-                                               int used = NB) {
+                                               f4 (&acc)[MB][NB], const f4 (&sa)[ROWS ? COUNT : 1], const float (&sb)[NB]) {
   typedef Codes<EXACT> X;
   constexpr int LAG = EXACT ? 1 : 2;
+  typename X::wide w;
   f4 late[LAG + 1];
-  auto add = [&](int i, int j, const f4 &x) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[FIRST + i][j][q] = fmaf(x[q], ROWS ? sa[i][q] * sb[j] : sb[j], acc[FIRST + i][j][q]);
-  };
-  if constexpr (FULL) {
-    typename X::wide w;
-#pragma unroll
-    for (int n = 0; n < COUNT * NB + LAG; ++n) {
-      if (n < COUNT * NB) {
-        if (n % NB == 0) w = X::widen(a[n / NB]);
-        late[n % (LAG + 1)] = X::dot(w, b[n % NB]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      const int m = n - LAG;
-      if (m >= 0) add(m / NB, m % NB, late[m % (LAG + 1)]);
-      __builtin_amdgcn_sched_barrier(0);
+  for (int n = 0; n < COUNT * NB + LAG; ++n) {
+    if (n < COUNT * NB) {
+      if (n % NB == 0) w = X::widen(a[n / NB]);
+      late[n % (LAG + 1)] = X::dot(w, b[n % NB]);
     }
-  } else {
+    __builtin_amdgcn_sched_barrier(0);
+    const int m = n - LAG;
+    if (m >= 0) {
+      const int i = m / NB, j = m % NB;
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-      if (j == 0 || j < used)
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i) add(i, j, X::dot(X::widen(a[i]), b[j]));
+      for (int q = 0; q < 4; ++q)
+        acc[FIRST + i][j][q] = fmaf(late[m % (LAG + 1)][q], ROWS ? sa[i][q] * sb[j] : sb[j], acc[FIRST + i][j][q]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 

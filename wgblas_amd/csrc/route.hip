@@ -568,7 +568,7 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const float g = back[slot][e0 + j];
-    out[j] = (T)(p.sigmoid ? g * slope[j] : s[j] * (g - inner));
+    out[j] = (T)wgb::in_fp32(p.sigmoid ? g * slope[j] : s[j] * (g - inner));
   }
   T *y = (T *)p.dlogits + token * p.ldd;
   if (e0 + PER <= p.experts) {
@@ -782,12 +782,12 @@ struct Lanes {
     if (left >= V) {
       Vec v;
 #pragma unroll
-      for (int i = 0; i < V; ++i) v.v[i] = (T)f[i];
+      for (int i = 0; i < V; ++i) v.v[i] = (T)wgb::in_fp32(f[i]);
       put(x, v);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (i < left) x[i] = (T)f[i];
+        if (i < left) x[i] = (T)wgb::in_fp32(f[i]);
     }
   }
 };
