@@ -2,8 +2,9 @@
  * wgblas_hip.h — C ABI of libwgblas_hip, the MI355X (gfx950) implementation
  * of wgblas's data-parallel hot path: the GEMM family (sgemm, sgemmtr, ssyrk,
  * dgemm) and the level-1 reductions (sdot, sasum, snrm2, isamax), and of the
- * products of expert layers: grouped products in fp32, fp16 and bf16, and 4-bit
- * (MXFP4) matrices with theirs.
+ * products of expert layers: grouped products in fp32, fp16 and bf16, 4-bit
+ * (MXFP4) and 8-bit (FP8) matrices with theirs, and the routing of tokens to
+ * experts.
  *
  * Every entry point takes plain pointers and sizes. Matrices are
  * COLUMN-MAJOR (element (i, j) of an ld-strided matrix sits at p[i + j*ld]);
@@ -449,8 +450,9 @@ int wgb_fp8_gemm_grouped(wgb_ctx *ctx, int transA, int64_t groups, int64_t m,
  * again, with the gradients of all of it. Everything stays in device memory;
  * no call waits for another. A pair is slot s of token t, at t*topk + s in
  * ids, weights and places (topk-by-n matrices without padding). topk is at
- * most 64, n*topk below 2^31, experts at most 1024. Results are reproducible
- * run to run. No counterpart in the reference, which has no operator of this
+ * most 64, n*topk below 2^31, experts at most 1024. No two pairs have the same
+ * place (wgb_route_order's never do): of columns written for two of them it is
+ * not defined which stays. Results are reproducible run to run. No counterpart in the reference, which has no operator of this
  * kind. */
 
 /* The experts of each of n tokens from the router's logits (experts-by-n
@@ -463,8 +465,8 @@ int wgb_fp8_gemm_grouped(wgb_ctx *ctx, int transA, int64_t groups, int64_t m,
  * the experts come in groups of experts/groups neighbours: only those
  * top_groups groups stay whose best choice value (best 1), or the sum of whose
  * two best (best 2), is largest. ids gets the topk experts of the largest
- * choice values, in their order; among equal ones the lowest expert (or group)
- * goes first. weights gets the chosen scores, divided by their sum if renorm
+ * choice values, in their order (as 64-bit scores have it; weights are fp32
+ * ones); among equal ones the lowest expert (or group) goes first. weights gets the chosen scores, divided by their sum if renorm
  * is not 0, times scale. An expert whose logit or choice value is -Inf is
  * never chosen (a mask): slots that no expert is left for get id -1 and weight
  * 0. A NaN choice value comes after all numbers; NaN scores give NaN weights. */
