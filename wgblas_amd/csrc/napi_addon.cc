@@ -36,12 +36,12 @@ napi_value throw_status(napi_env env, int status, const char *what) {
   } while (0)
 
 struct Args {
-  napi_value v[20];
-  size_t n = 20;
+  napi_value v[24];
+  size_t n = 24;
 };
 
 bool get_args(napi_env env, napi_callback_info info, Args &a, size_t want) {
-  a.n = 20;
+  a.n = 24;
   if (napi_get_cb_info(env, info, &a.n, a.v, nullptr, nullptr) != napi_ok) return false;
   if (a.n < want) {
     napi_throw_type_error(env, nullptr, "wgblas_hip addon: too few arguments");
@@ -730,6 +730,201 @@ napi_value Mxfp4Gemm(napi_env env, napi_callback_info info) {
   return nullptr;
 }
 
+// fp8Quantize(ctx, type, trans, block, matrices, k, n, X, ldx, codes, ld, scales, lds):
+// X, codes and scales hold the matrices one behind another.
+napi_value Fp8Quantize(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 13)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, trans, block;
+  int64_t matrices, k, n, ldx, ld, lds;
+  void *X, *codes, *scales;
+  if (!get_i32(env, a.v[1], &type) || !get_i32(env, a.v[2], &trans) || !get_i32(env, a.v[3], &block) ||
+      !get_i64(env, a.v[4], &matrices) || !get_i64(env, a.v[5], &k) || !get_i64(env, a.v[6], &n) ||
+      !get_ptr(env, a.v[7], &X) || !get_i64(env, a.v[8], &ldx) || !get_ptr(env, a.v[9], &codes) ||
+      !get_i64(env, a.v[10], &ld) || !get_ptr(env, a.v[11], &scales) || !get_i64(env, a.v[12], &lds))
+    return nullptr;
+  const int64_t bytes = type == WGB_F32 ? 4 : 2;
+  for (int64_t i = 0; i < matrices; ++i)
+    WGB_OK_OR_THROW(wgb_fp8_quantize(ctx, type, trans, block, k, n, (char *)X + i * ldx * (trans == WGB_TRANS ? k : n) * bytes, ldx,
+                                     (uint8_t *)codes + i * n * ld, ld, (float *)scales + i * (ld / 128) * lds, lds),
+                    "wgb_fp8_quantize");
+  return nullptr;
+}
+
+// fp8Dequantize(ctx, type, block, matrices, k, n, codes, ld, scales, lds, X, ldx)
+napi_value Fp8Dequantize(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 12)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, block;
+  int64_t matrices, k, n, ldx, ld, lds;
+  void *X, *codes, *scales;
+  if (!get_i32(env, a.v[1], &type) || !get_i32(env, a.v[2], &block) || !get_i64(env, a.v[3], &matrices) ||
+      !get_i64(env, a.v[4], &k) || !get_i64(env, a.v[5], &n) || !get_ptr(env, a.v[6], &codes) ||
+      !get_i64(env, a.v[7], &ld) || !get_ptr(env, a.v[8], &scales) || !get_i64(env, a.v[9], &lds) ||
+      !get_ptr(env, a.v[10], &X) || !get_i64(env, a.v[11], &ldx))
+    return nullptr;
+  const int64_t bytes = type == WGB_F32 ? 4 : 2;
+  for (int64_t i = 0; i < matrices; ++i)
+    WGB_OK_OR_THROW(wgb_fp8_dequantize(ctx, type, block, k, n, (const uint8_t *)codes + i * n * ld, ld,
+                                       (const float *)scales + i * (ld / 128) * lds, lds, (char *)X + i * ldx * n * bytes, ldx),
+                    "wgb_fp8_dequantize");
+  return nullptr;
+}
+
+// fp8Gemm(ctx, transA, groups (-1: one matrix), m, n, k, alpha, A, lda, strideA,
+// blockA, scaleA, ldsa, B, ldb, scaleB, ldsb, offsets, beta, C, ldc, ctype); a
+// group's scales follow the last one's.
+napi_value Fp8Gemm(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 22)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int ta, block, ctype;
+  int64_t groups, m, n, k, lda, strideA, ldsa, ldb, ldsb, ldc;
+  double alpha, beta;
+  void *A, *sA, *B, *sB, *off, *C;
+  if (!get_i32(env, a.v[1], &ta) || !get_i64(env, a.v[2], &groups) || !get_i64(env, a.v[3], &m) ||
+      !get_i64(env, a.v[4], &n) || !get_i64(env, a.v[5], &k) || !get_f64(env, a.v[6], &alpha) ||
+      !get_ptr(env, a.v[7], &A) || !get_i64(env, a.v[8], &lda) || !get_i64(env, a.v[9], &strideA) ||
+      !get_i32(env, a.v[10], &block) || !get_ptr(env, a.v[11], &sA) || !get_i64(env, a.v[12], &ldsa) ||
+      !get_ptr(env, a.v[13], &B) || !get_i64(env, a.v[14], &ldb) || !get_ptr(env, a.v[15], &sB) ||
+      !get_i64(env, a.v[16], &ldsb) || !get_ptr(env, a.v[17], &off) || !get_f64(env, a.v[18], &beta) ||
+      !get_ptr(env, a.v[19], &C) || !get_i64(env, a.v[20], &ldc) || !get_i32(env, a.v[21], &ctype))
+    return nullptr;
+  const uint8_t *a8 = (const uint8_t *)A, *b8 = (const uint8_t *)B;
+  if (groups < 0)
+    WGB_OK_OR_THROW(wgb_fp8_gemm(ctx, ta, m, n, k, (float)alpha, a8, lda, block, (const float *)sA, ldsa, b8, ldb,
+                                 (const float *)sB, ldsb, (float)beta, C, ldc, ctype), "wgb_fp8_gemm");
+  else
+    WGB_OK_OR_THROW(wgb_fp8_gemm_grouped(ctx, ta, groups, m, n, k, (float)alpha, a8, lda, strideA, block, (const float *)sA,
+                                         ldsa, lda / 128 * ldsa, b8, ldb, (const float *)sB, ldsb, (const int64_t *)off,
+                                         (float)beta, C, ldc, ctype), "wgb_fp8_gemm_grouped");
+  return nullptr;
+}
+
+// route(ctx, type, scoring, experts, n, topk, logits, ldl, bias, groups,
+// topGroups, best, renorm, scale, ids, weights)
+napi_value Route(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 16)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, scoring, best, renorm;
+  int64_t experts, n, topk, ldl, groups, top_groups;
+  double scale;
+  void *logits, *bias, *ids, *weights;
+  if (!get_i32(env, a.v[1], &type) || !get_i32(env, a.v[2], &scoring) || !get_i64(env, a.v[3], &experts) ||
+      !get_i64(env, a.v[4], &n) || !get_i64(env, a.v[5], &topk) || !get_ptr(env, a.v[6], &logits) ||
+      !get_i64(env, a.v[7], &ldl) || !get_ptr(env, a.v[8], &bias) || !get_i64(env, a.v[9], &groups) ||
+      !get_i64(env, a.v[10], &top_groups) || !get_i32(env, a.v[11], &best) || !get_i32(env, a.v[12], &renorm) ||
+      !get_f64(env, a.v[13], &scale) || !get_ptr(env, a.v[14], &ids) || !get_ptr(env, a.v[15], &weights))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_route(ctx, type, scoring, experts, n, topk, logits, ldl, (const float *)bias, groups, top_groups, best,
+                            renorm, (float)scale, (int32_t *)ids, (float *)weights), "wgb_route");
+  return nullptr;
+}
+
+// routeGrad(ctx, type, scoring, experts, n, topk, logits, ldl, ids, renorm, scale, dweights, dlogits, ldd)
+napi_value RouteGrad(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 14)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, scoring, renorm;
+  int64_t experts, n, topk, ldl, ldd;
+  double scale;
+  void *logits, *ids, *dweights, *dlogits;
+  if (!get_i32(env, a.v[1], &type) || !get_i32(env, a.v[2], &scoring) || !get_i64(env, a.v[3], &experts) ||
+      !get_i64(env, a.v[4], &n) || !get_i64(env, a.v[5], &topk) || !get_ptr(env, a.v[6], &logits) ||
+      !get_i64(env, a.v[7], &ldl) || !get_ptr(env, a.v[8], &ids) || !get_i32(env, a.v[9], &renorm) ||
+      !get_f64(env, a.v[10], &scale) || !get_ptr(env, a.v[11], &dweights) || !get_ptr(env, a.v[12], &dlogits) ||
+      !get_i64(env, a.v[13], &ldd))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_route_grad(ctx, type, scoring, experts, n, topk, logits, ldl, (const int32_t *)ids, renorm, (float)scale,
+                                 (const float *)dweights, dlogits, ldd), "wgb_route_grad");
+  return nullptr;
+}
+
+// routeOrder(ctx, experts, n, topk, ids, offsets, places, pairs)
+napi_value RouteOrder(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 8)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int64_t experts, n, topk;
+  void *ids, *offsets, *places, *pairs;
+  if (!get_i64(env, a.v[1], &experts) || !get_i64(env, a.v[2], &n) || !get_i64(env, a.v[3], &topk) ||
+      !get_ptr(env, a.v[4], &ids) || !get_ptr(env, a.v[5], &offsets) || !get_ptr(env, a.v[6], &places) ||
+      !get_ptr(env, a.v[7], &pairs))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_route_order(ctx, experts, n, topk, (const int32_t *)ids, (int64_t *)offsets, (int32_t *)places,
+                                  (int32_t *)pairs), "wgb_route_order");
+  return nullptr;
+}
+
+// routeGather(ctx, type, d, n, topk, X, ldx, places, weights, Y, ldy)
+napi_value RouteGather(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 11)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type;
+  int64_t d, n, topk, ldx, ldy;
+  void *X, *places, *weights, *Y;
+  if (!get_i32(env, a.v[1], &type) || !get_i64(env, a.v[2], &d) || !get_i64(env, a.v[3], &n) ||
+      !get_i64(env, a.v[4], &topk) || !get_ptr(env, a.v[5], &X) || !get_i64(env, a.v[6], &ldx) ||
+      !get_ptr(env, a.v[7], &places) || !get_ptr(env, a.v[8], &weights) || !get_ptr(env, a.v[9], &Y) ||
+      !get_i64(env, a.v[10], &ldy))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_route_gather(ctx, type, d, n, topk, X, ldx, (const int32_t *)places, (const float *)weights, Y, ldy),
+                  "wgb_route_gather");
+  return nullptr;
+}
+
+// routeCombine(ctx, type, d, n, topk, Y, ldy, places, weights, beta, C, ldc, ctype)
+napi_value RouteCombine(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 13)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type, ctype;
+  int64_t d, n, topk, ldy, ldc;
+  double beta;
+  void *Y, *places, *weights, *C;
+  if (!get_i32(env, a.v[1], &type) || !get_i64(env, a.v[2], &d) || !get_i64(env, a.v[3], &n) ||
+      !get_i64(env, a.v[4], &topk) || !get_ptr(env, a.v[5], &Y) || !get_i64(env, a.v[6], &ldy) ||
+      !get_ptr(env, a.v[7], &places) || !get_ptr(env, a.v[8], &weights) || !get_f64(env, a.v[9], &beta) ||
+      !get_ptr(env, a.v[10], &C) || !get_i64(env, a.v[11], &ldc) || !get_i32(env, a.v[12], &ctype))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_route_combine(ctx, type, d, n, topk, Y, ldy, (const int32_t *)places, (const float *)weights, (float)beta,
+                                    C, ldc, ctype), "wgb_route_combine");
+  return nullptr;
+}
+
+// routeCombineGrad(ctx, type, d, n, topk, dC, lddc, Y, ldy, places, weights, dY, lddy, dweights)
+napi_value RouteCombineGrad(napi_env env, napi_callback_info info) {
+  Args a;
+  if (!get_args(env, info, a, 14)) return nullptr;
+  wgb_ctx *ctx = ctx_of(env, a.v[0]);
+  if (!ctx) return nullptr;
+  int type;
+  int64_t d, n, topk, lddc, ldy, lddy;
+  void *dC, *Y, *places, *weights, *dY, *dweights;
+  if (!get_i32(env, a.v[1], &type) || !get_i64(env, a.v[2], &d) || !get_i64(env, a.v[3], &n) ||
+      !get_i64(env, a.v[4], &topk) || !get_ptr(env, a.v[5], &dC) || !get_i64(env, a.v[6], &lddc) ||
+      !get_ptr(env, a.v[7], &Y) || !get_i64(env, a.v[8], &ldy) || !get_ptr(env, a.v[9], &places) ||
+      !get_ptr(env, a.v[10], &weights) || !get_ptr(env, a.v[11], &dY) || !get_i64(env, a.v[12], &lddy) ||
+      !get_ptr(env, a.v[13], &dweights))
+    return nullptr;
+  WGB_OK_OR_THROW(wgb_route_combine_grad(ctx, type, d, n, topk, dC, lddc, Y, ldy, (const int32_t *)places,
+                                         (const float *)weights, dY, lddy, (float *)dweights), "wgb_route_combine_grad");
+  return nullptr;
+}
+
 napi_value ModuleInit(napi_env env, napi_value exports) {
   if (wgb_abi_version() != WGB_ABI_VERSION) {
     std::string msg = "wgblas_hip addon: libwgblas_hip implements C ABI version " +
@@ -749,7 +944,10 @@ napi_value ModuleInit(napi_env env, napi_value exports) {
       {"ssyrk", Ssyrk}, {"ssyr2k", Ssyr2k}, {"ssymm", Ssymm},
       {"tri", Tri}, {"sgemv", Sgemv}, {"ger", Ger}, {"syr", Syr}, {"symv", Symv}, {"trmv", Trmv}, {"reduce", Reduce},
       {"gemmGrouped", GemmGrouped}, {"gemmGroupedK", GemmGroupedK}, {"mxfp4Quantize", Mxfp4Quantize},
-      {"mxfp4Dequantize", Mxfp4Dequantize}, {"mxfp4Gemm", Mxfp4Gemm},
+      {"mxfp4Dequantize", Mxfp4Dequantize}, {"mxfp4Gemm", Mxfp4Gemm}, {"fp8Quantize", Fp8Quantize},
+      {"fp8Dequantize", Fp8Dequantize}, {"fp8Gemm", Fp8Gemm}, {"route", Route}, {"routeGrad", RouteGrad},
+      {"routeOrder", RouteOrder}, {"routeGather", RouteGather}, {"routeCombine", RouteCombine},
+      {"routeCombineGrad", RouteCombineGrad},
   };
   for (const Fn &f : fns) {
     napi_value v;

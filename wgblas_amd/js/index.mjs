@@ -1,11 +1,13 @@
 // wgblas's public API for the hot path, on HIP (the routine set of
 // index.mjs in wgblas limited to the GEMM family, the level-3 routines built
 // on it and the level-1 reductions, plus the device, residency and
-// seeded-input helpers), and the grouped and 4-bit products.
+// seeded-input helpers), the grouped, 4-bit and 8-bit
+// products, and routing to experts.
 export { init, cleanup, gpuName, HipDevice } from "./src/init.mjs";
 export { GpuVector } from "./src/classes/GpuVector.mjs";
 export { GpuMatrix } from "./src/classes/GpuMatrix.mjs";
 export { Mxfp4Matrix } from "./src/classes/Mxfp4Matrix.mjs";
+export { Fp8Matrix } from "./src/classes/Fp8Matrix.mjs";
 export { randomFloat32Array, randomFloat64Array, randomTriangularFloat32Array } from "./src/random.mjs";
 export { sgemm } from "./src/sgemm.mjs";
 export { sgemmtr } from "./src/sgemmtr.mjs";
@@ -22,6 +24,8 @@ export { dtrmm } from "./src/dtrmm.mjs";
 export { strsm } from "./src/strsm.mjs";
 export { sgemmGrouped, sgemmGroupedK } from "./src/sgemmGrouped.mjs";
 export { mxfp4Gemm, mxfp4GemmGrouped } from "./src/mxfp4Gemm.mjs";
+export { fp8Gemm, fp8GemmGrouped } from "./src/fp8Gemm.mjs";
+export { route, routeGrad, routeOrder, routeGather, routeCombine, routeCombineGrad } from "./src/routing.mjs";
 export { sgemv } from "./src/sgemv.mjs";
 export { dgemv } from "./src/dgemv.mjs";
 export { sger } from "./src/sger.mjs";
