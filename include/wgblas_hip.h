@@ -400,7 +400,8 @@ int wgb_mxfp4_gemm_grouped(wgb_ctx *ctx, int64_t groups, int64_t m, int64_t n,
  * quantised, for products that sum over X's columns). A block's scale is the
  * least power of two that brings its largest magnitude to 448 or less, at
  * least 2^-126; x/scale goes to the nearest code, ties to the even code. A
- * block with an Inf or a NaN becomes NaN as a whole (scale NaN, codes 0). */
+ * block with an Inf or a NaN becomes NaN as a whole (scale NaN, codes 0).
+ * Quantising and back take fewer than 2^26 columns. */
 int wgb_fp8_quantize(wgb_ctx *ctx, int type, int trans, int block, int64_t k,
                      int64_t n, const void *X, int64_t ldx, uint8_t *codes,
                      int64_t ld, float *scales, int64_t lds);
@@ -450,9 +451,10 @@ int wgb_fp8_gemm_grouped(wgb_ctx *ctx, int transA, int64_t groups, int64_t m,
  * again, with the gradients of all of it. Everything stays in device memory;
  * no call waits for another. A pair is slot s of token t, at t*topk + s in
  * ids, weights and places (topk-by-n matrices without padding). topk is at
- * most 64, n*topk below 2^31, experts at most 1024. No two pairs have the same
- * place (wgb_route_order's never do): of columns written for two of them it is
- * not defined which stays. Results are reproducible run to run. No counterpart in the reference, which has no operator of this
+ * most 64, n*topk below 2^31, n below 2^24 (but for wgb_route_order), experts
+ * at most 1024. No two pairs have the same place (wgb_route_order's never do):
+ * of columns written for two of them it is not defined which stays. Results
+ * are reproducible run to run. No counterpart in the reference, which has no operator of this
  * kind. */
 
 /* The experts of each of n tokens from the router's logits (experts-by-n

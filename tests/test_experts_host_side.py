@@ -70,7 +70,7 @@ def child(tmp_path_factory):
 
 REFUSED = {
     "route": [dict(type=3), dict(scoring=2), dict(experts=0), dict(experts=1025, ldl=2000, groups=1, top_groups=1),
-              dict(n=-1), dict(topk=0), dict(topk=65), dict(topk=17), dict(n=2 ** 31 // 8), dict(ldl=63), dict(groups=0),
+              dict(n=-1), dict(topk=0), dict(topk=65), dict(topk=17), dict(n=2 ** 31 // 8), dict(n=2 ** 24, topk=1), dict(ldl=63), dict(groups=0),
               dict(groups=7), dict(groups=128, experts=128, ldl=128), dict(top_groups=0), dict(top_groups=9), dict(best=0),
               dict(best=3), dict(logits=None), dict(ids=None), dict(weights=None)],
     "route_grad": [dict(type=-1), dict(scoring=-1), dict(experts=7), dict(n=-2), dict(topk=70), dict(ldl=8), dict(ldd=8),
@@ -78,13 +78,14 @@ REFUSED = {
     "route_order": [dict(experts=0), dict(experts=2000), dict(n=-1), dict(topk=0), dict(topk=65), dict(n=2 ** 30),
                     dict(ids=None), dict(offsets=None), dict(places=None), dict(pairs=None)],
     "route_gather": [dict(type=5), dict(d=-1), dict(d=2 ** 31, ldx=2 ** 31, ldy=2 ** 31), dict(n=-1), dict(topk=0),
-                     dict(topk=65), dict(n=2 ** 31), dict(ldx=99), dict(ldy=99), dict(X=None), dict(places=None), dict(Y=None)],
+                     dict(topk=65), dict(n=2 ** 31), dict(n=2 ** 24, topk=1), dict(ldx=99), dict(ldy=99), dict(X=None), dict(places=None), dict(Y=None)],
     "route_combine": [dict(type=5), dict(ctype=2), dict(d=-1), dict(n=-1), dict(topk=0), dict(ldy=99), dict(ldc=99),
                       dict(Y=None), dict(places=None), dict(C=None)],
     "route_combine_grad": [dict(type=5), dict(d=-1), dict(n=-1), dict(topk=65), dict(lddc=99), dict(ldy=99), dict(lddy=99),
                            dict(dC=None), dict(Y=None), dict(places=None), dict(weights=None), dict(dY=None),
                            dict(dweights=None)],
-    "fp8_quantize": [dict(type=3), dict(trans=2), dict(block=64), dict(k=-1), dict(n=-1), dict(n=2 ** 31), dict(ldx=19),
+    "fp8_quantize": [dict(type=3), dict(trans=2), dict(block=64), dict(k=-1), dict(n=-1), dict(n=2 ** 31), dict(n=2 ** 26, lds=2 ** 26),
+                     dict(ldx=19),
                      dict(ld=300), dict(ld=256), dict(ld=2 ** 23 + 128), dict(lds=19), dict(lds=2 ** 29), dict(X=None),
                      dict(codes=None), dict(scales=None), "codes=P + 8", "scales=P + 2"],
     "fp8_dequantize": [dict(type=3), dict(block=0), dict(k=-1), dict(ld=320), dict(lds=1), dict(ldx=299), dict(X=None),

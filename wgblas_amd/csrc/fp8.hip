@@ -348,7 +348,8 @@ int check_convert(int type, int block, int64_t k, int64_t n) {
     return fail(WGB_ERR_INVALID_VALUE, "type must be WGB_F32, WGB_F16 or WGB_BF16");
   if (block != 1 && block != 128) return fail(WGB_ERR_INVALID_VALUE, "block must be 1 or 128");
   if (k < 0 || n < 0) return fail(WGB_ERR_INVALID_VALUE, "k and n must be non-negative");
-  if (n > INT32_MAX) return fail(WGB_ERR_INVALID_VALUE, "n must be below 2^31");
+  // a launch has fewer than 2^32 threads, of which a column has 64
+  if (n >= (int64_t)1 << 26) return fail(WGB_ERR_INVALID_VALUE, "n must be below 2^26");
   return WGB_OK;
 }
 

@@ -1017,6 +1017,12 @@ int check_pairs(int64_t n, int64_t topk) {
   return WGB_OK;
 }
 
+// A launch has fewer than 2^32 threads, of which a token has up to 256.
+int check_tokens(int64_t n) {
+  if (n >= (int64_t)1 << 24) return fail(WGB_ERR_INVALID_VALUE, "n must be below 2^24");
+  return WGB_OK;
+}
+
 int check_choice(int64_t experts, int64_t n, int64_t topk) {
   const int st = check_pairs(n, topk);
   if (st) return st;
@@ -1034,6 +1040,7 @@ int check_scoring(int scoring) {
 int check_rows(int type, int64_t d, int64_t n, int64_t topk) {
   int st = check_type(type);
   if (!st) st = check_pairs(n, topk);
+  if (!st) st = check_tokens(n);
   if (st) return st;
   if (d < 0 || d > INT32_MAX) return fail(WGB_ERR_INVALID_VALUE, "d must be non-negative and below 2^31");
   return WGB_OK;
@@ -1053,7 +1060,7 @@ extern "C" int wgb_route(wgb_ctx *ctx, int type, int scoring, int64_t experts, i
   int st = wgb::enter(ctx);
   if (st) return st;
   if ((st = check_type(type)) || (st = check_scoring(scoring)) || (st = check_choice(experts, n, topk)) ||
-      (st = check_ld(ldl, experts, "ldl")))
+      (st = check_tokens(n)) || (st = check_ld(ldl, experts, "ldl")))
     return st;
   if (groups < 1 || groups > kMaxGroups || experts % groups != 0)
     return fail(WGB_ERR_INVALID_VALUE, "groups must be between 1 and 64 and divide experts");
@@ -1093,7 +1100,7 @@ extern "C" int wgb_route_grad(wgb_ctx *ctx, int type, int scoring, int64_t exper
   int st = wgb::enter(ctx);
   if (st) return st;
   if ((st = check_type(type)) || (st = check_scoring(scoring)) || (st = check_choice(experts, n, topk)) ||
-      (st = check_ld(ldl, experts, "ldl")) || (st = check_ld(ldd, experts, "ldd")))
+      (st = check_tokens(n)) || (st = check_ld(ldl, experts, "ldl")) || (st = check_ld(ldd, experts, "ldd")))
     return st;
   if (n == 0) return WGB_OK;
   if (!logits || !ids || !dweights || !dlogits)
