@@ -182,7 +182,10 @@ __device__ __forceinline__ void multiply_codes(const v8i (&a)[COUNT], const type
   }
 }
 
-// One BM x BN tile of C a block, WM x WN waves, S stages of LDS.
+// One BM x BN tile of C a block, WM x WN waves, S stages of LDS. 128 x 128 with
+// exact sums and rows' own scales is bound by the conversions and v_fma (4096 x
+// 2048 x 16384: 264 us, 1.04 PFLOP/s), 128 x 32 by reading A (49 experts of 4096
+// x 2048 with 96 columns: 78 us, 5.3 TB/s).
 template <int BM, int BN, int WM, int WN, bool AMC, bool ROWS, bool EXACT, int S>
 struct Fp8Kernel {
   typedef Fp8 Element;
@@ -341,6 +344,8 @@ struct Fp8Kernel {
 // are issued before a tile is stored, when its operands' registers are free: in
 // the midst of a tile they would have to be spilled, and each return of one
 // waits for all copies and stores under way.
+// 8192 x 4096 x 8192 into bf16: 215 us, 2.56 PFLOP/s, and 226 with A
+// row-contiguous, bound by power; at k = 2048 1.97, for a tile's start and end.
 template <bool AMC, bool ROWS, bool EXACT>
 struct Fp8Large {
   static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
@@ -586,7 +591,8 @@ struct Fp8Large {
 // row blocks and CB column blocks of 16; its eight waves share k in k-tiles,
 // load both operands straight into MFMA operand registers, the next k-tile ahead
 // of the present one's MFMAs, and add their sums in LDS in the waves' order. A
-// k-contiguous only.
+// k-contiguous only. One column, repeated: 8192 x 8192 12.4 us (5.4 TB/s), 4096 x
+// 4096 6.9; 16 columns, 8192 x 4096 8.6.
 template <int R, int CB, bool ROWS, bool EXACT>
 struct Fp8Skinny {
   static constexpr int kBM = 16 * R, kBN = 16 * CB;
