@@ -100,3 +100,57 @@ def test_conversion_past_the_caches(ctx, t, trans, block):
         back.free()
     for d in (dX, codes, scales):
         d.free()
+
+
+@pytest.mark.parametrize("trans,block", FORMS)
+def test_replays_with_sums_in_the_workspace(trans, block):
+    """A captured product whose rest is cut along k: its partial sums' workspace stays its own when a later call grows it."""
+    import ctypes
+
+    from wgblas_amd import BF16, NO_TRANS, Context
+
+    hip = ctypes.CDLL("libamdhip64.so")
+
+    def check(status):
+        assert status == 0, f"HIP status {status}"
+
+    rng = np.random.default_rng(4)
+    m, n, k = 6144, 2816, 640
+    rows, cols = (k, m) if trans == TRANS else (m, k)
+    with Context(0) as c:
+        W, X = c.empty((cols, rows), np.float32), c.empty((n, k), np.float32)
+        c.fill_normal(W, 1)
+        A, SA = c.empty((cols, rows), np.uint8), c.empty((rows // 128, (cols + block - 1) // block), np.float32)
+        c.fp8_quantize(R.TYPES["f32"], NO_TRANS, block, rows, cols, W, rows, A, rows, SA, SA.shape[1])
+        B, SB, C = c.empty((n, k), np.uint8), c.empty((k // 128, n), np.float32), c.empty((n, m), np.uint16)
+
+        def product():
+            c.fp8_quantize(R.TYPES["f32"], NO_TRANS, 1, k, n, X, k, B, k, SB, n)
+            c.fp8_gemm(trans, m, n, k, 1.0, A, rows, block, SA, SA.shape[1], B, k, SB, n, 0.0, C, m, BF16)
+
+        c.fill_normal(X, 2)
+        product()
+        c.synchronize()
+        stream = ctypes.c_void_p(c.stream)
+        graph, executable = ctypes.c_void_p(), ctypes.c_void_p()
+        check(hip.hipStreamBeginCapture(stream, 1))  # thread-local mode
+        try:
+            product()
+        finally:
+            check(hip.hipStreamEndCapture(stream, ctypes.byref(graph)))
+        check(hip.hipGraphInstantiate(ctypes.byref(executable), graph, None, None, ctypes.c_size_t(0)))
+        for replay in range(4):
+            if replay == 1:  # both operands moved to a workspace of 150 MB
+                big, out = c.upload(R.encode(rng.standard_normal((6001, 6001)), "bf16")), c.empty((6001, 6001), np.float32)
+                one = c.upload(np.array([0, 6001], np.int64))
+                c.gemm_grouped(BF16, TRANS, 1, 6001, 6001, 6001, 1.0, big, 6001, 6001 * 6001, big, 6001, one, 0.0, out, 6001,
+                               R.TYPES["f32"])
+            c.fill_normal(X, 10 + replay)
+            product()
+            eager = C.to_host()
+            c.h2d(C.ptr, np.zeros((n, m), np.uint16))
+            check(hip.hipGraphLaunch(executable, stream))
+            c.synchronize()
+            assert np.array_equal(C.to_host(), eager), replay
+        check(hip.hipGraphExecDestroy(executable))
+        check(hip.hipGraphDestroy(graph))
