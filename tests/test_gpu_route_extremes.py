@@ -1,0 +1,56 @@
+"""Routing where fp32 numbers lose what the definition needs: groups whose two best values nearly cancel. Against float64 by
+the definition (tests/routing.py)."""
+import numpy as np
+import pytest
+
+from tests import routing as Q
+from tests.test_gpu_route import run_route
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- the choice ----------------------------------------------------------------------
+
+
+def group_gaps(choice, groups, top_groups):
+    """How far the last kept group's score (the sum of its two best) is from the next one's."""
+    best = np.sort(np.sort(choice.reshape(len(choice), groups, -1), axis=2)[:, :, -2:].sum(2), axis=1)
+    return best[:, groups - top_groups] - best[:, groups - top_groups - 1]
+
+
+@pytest.mark.parametrize("experts,groups,top_groups", [(16, 8, 4), (24, 8, 3), (64, 4, 1), (256, 8, 4), (528, 33, 10), (1024, 64, 7)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [1e3, 1e4, 1e6])
+def test_groups_whose_two_best_nearly_cancel(ctx, experts, groups, top_groups, scoring, size):
+    """One expert of a group has a bias near `size`, the others one near -size: the sum is of the size of the scores, its
+    terms' roundings are not."""
+    rng = np.random.default_rng(experts)
+    n, per = 64000 // experts, experts // groups
+    x = rng.standard_normal((n, experts)).astype(np.float32)
+    b = (-size + 0.1 * rng.standard_normal(experts)).astype(np.float32)
+    first = np.arange(groups) * per + rng.integers(0, per, groups)
+    b[first] = (size + 0.1 * rng.standard_normal(groups)).astype(np.float32)
+    choice = Q.scores(x, scoring) + b.astype(np.float64)
+    sure = group_gaps(choice, groups, top_groups) > 1e-9  # a float64 value of 1e6 is rounded at 1.2e-10
+    assert sure.mean() > 0.99
+    ids, _ = run_route(ctx, x, "f32", experts, scoring, top_groups, b, groups, top_groups, 2)
+    # the top_groups largest values are the kept groups' first experts: their order is not the question here
+    want, _ = Q.route(x[sure].astype(np.float64), scoring, top_groups, b.astype(np.float64), groups, top_groups, 2)
+    assert np.array_equal(np.sort(ids[sure], axis=1), np.sort(want, axis=1))
+
+
+def test_groups_whose_sums_leave_fp32(ctx):
+    """The two best values' sum is past fp32's largest number, of either sign."""
+    experts, groups = 12, 4
+    b = np.zeros(experts, np.float32)
+    b[[0, 1, 3, 4]] = 3.0e38
+    b[1] = 2.9e38
+    b[[6, 7, 8]] = -3.0e38
+    b[[9, 10, 11]] = -3.1e38
+    x = np.random.default_rng(0).standard_normal((40, experts)).astype(np.float32)
+    for top_groups in (1, 2, 3):
+        topk = 3 * top_groups
+        ids, _ = run_route(ctx, x, "f32", experts, "sigmoid", topk, b, groups, top_groups, 2)
+        want, _ = Q.route(x.astype(np.float64), "sigmoid", topk, b.astype(np.float64), groups, top_groups, 2)
+        # values of 3e38 that differ by a score are one value in float64: the lowest goes first
+        assert np.array_equal(ids, want), top_groups

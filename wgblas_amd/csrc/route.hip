@@ -107,11 +107,11 @@ struct Keys<float> {
     return x != x ? kNan : x == -__builtin_inff() ? kNone : b ^ ((b >> 31) & 0x7fffffff);
   }
   static __device__ __forceinline__ float value(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
-  // of a group: the sum of its two best; scores that are NaN come after all numbers there, too
+  // of a group: half the sum of its two best (the sum may be past fp32); scores that are NaN come after all numbers there, too
   static __device__ __forceinline__ int sum(int a, int b) {
     if (a == kNone || b == kNone) return kNone;
     if (b == kNan) return a == kNan ? kNan : of(value(a) - 1e30f);
-    return of(value(a) + value(b));
+    return of(0.5f * value(a) + 0.5f * value(b));
   }
 };
 template <>
@@ -126,7 +126,7 @@ struct Keys<double> {
   }
 };
 
-// Room of a token in LDS: its values, and its groups' scores.
+// Room of a token in LDS: its values, and its groups' scores (fp64 ones, or fp32 ones and their sizes).
 template <class F>
 struct Room {
   static __host__ __device__ int values(int experts) { return (experts + 3) & ~3; }
@@ -139,7 +139,9 @@ struct Room {
 // larger: a score is off by at most 4 units of 2^-24 (sigmoid: the exponential
 // by |x| 2^-23 of itself, which p (1 - p) |x| < 0.3 makes 0.6 units, the
 // reciprocal by 2; softmax: 26 with the sum's), the value by half a unit more,
-// and twice that is doubled.
+// and twice that is doubled. Half the sum of two values is off by half of what
+// they are, whatever it is itself: `value` is half the sum of their magnitudes
+// there, for large ones of different signs leave a small sum.
 __device__ __forceinline__ float unsure(float value, int sigmoid) {
   return ((sigmoid ? 4.0f : 32.0f) + fabsf(value)) * 0x1p-22f;
 }
@@ -164,8 +166,15 @@ template <class F, int LPT, int PER>
 __device__ __forceinline__ Groups keep_groups(const RouteArgs &p, char *room, int lane, const typename Keys<F>::key (&v)[PER]) {
   typedef typename Keys<F>::key K;
   K *values = reinterpret_cast<K *>(room), *score = values + Room<K>::values(p.experts);
+  float *size = reinterpret_cast<float *>(score + ((p.groups + 3) & ~3));  // fp32: half the two values' magnitudes
   const int e0 = lane * PER, lanes = p.per / PER;  // of a group, where groups are whole lanes
-  auto scored = [&](K a, K b) { return p.best == 2 && p.per > 1 ? Keys<F>::sum(a, b) : a; };
+  const bool two = p.best == 2 && p.per > 1;
+  auto put_score = [&](int i, K a, K b) {
+    score[i] = two ? Keys<F>::sum(a, b) : a;
+    if constexpr (std::is_same<F, float>::value) {
+      if (two) size[i] = 0.5f * fabsf(Keys<F>::value(a)) + 0.5f * fabsf(Keys<F>::value(b));
+    }
+  };
   Groups g = {0, (1u << PER) - 1, false};
   const bool whole = lanes * PER == p.per && (lanes & (lanes - 1)) == 0;
   if (whole) {
@@ -173,7 +182,7 @@ __device__ __forceinline__ Groups keep_groups(const RouteArgs &p, char *room, in
 #pragma unroll
     for (int j = 1; j < PER; ++j) best_two(a, b, v[j], Keys<F>::kNone);
     for (int d = 1; d < lanes; d <<= 1) best_two(a, b, (K)__shfl_xor(a, d), (K)__shfl_xor(b, d));
-    if ((lane & (lanes - 1)) == 0 && e0 < p.experts) score[e0 / p.per] = scored(a, b);
+    if ((lane & (lanes - 1)) == 0 && e0 < p.experts) put_score(e0 / p.per, a, b);
     if constexpr (std::is_same<F, float>::value) {
       if (b > Keys<F>::kNan) {
         const K least = Keys<F>::of(Keys<F>::value(b) - unsure(Keys<F>::value(b), p.sigmoid));
@@ -190,26 +199,25 @@ __device__ __forceinline__ Groups keep_groups(const RouteArgs &p, char *room, in
     for (int i = lane; i < p.groups; i += LPT) {
       K a = Keys<F>::kNone, b = a;
       for (int j = 0; j < p.per; ++j) best_two(a, b, values[i * p.per + j], Keys<F>::kNone);
-      score[i] = scored(a, b);
+      put_score(i, a, b);
     }
   }
   wave_sync();
-  // whether group i is kept; one that is compares itself with those that are not
+  // whether group i is kept; the least that a kept one's score may be, the most that another's may be (a score that is
+  // no number is behind all others, whatever those are off by)
+  float least = __builtin_inff(), next = -__builtin_inff();
   auto kept = [&](int i) {
     const K mine = score[i];
     int before = 0;
     for (int o = 0; o < p.groups; ++o) before += score[o] > mine || (score[o] == mine && o < i);
     const bool in = before < p.top_groups;
     if constexpr (std::is_same<F, float>::value) {
-      // the group behind the last kept one: the last one asks for it
-      if (before == p.top_groups - 1 && mine > Keys<F>::kNan) {
-        K next = Keys<F>::kNone;
-        for (int o = 0; o < p.groups; ++o) {
-          const K s = score[o];
-          if (s > next && (s < mine || (s == mine && o > i))) next = s;
-        }
-        const float least = Keys<F>::value(mine);
-        if (next > Keys<F>::kNan) g.close |= least - Keys<F>::value(next) <= 2.0f * unsure(least, p.sigmoid);
+      if (mine > Keys<F>::kNan) {
+        const float x = Keys<F>::value(mine), off = unsure(two ? size[i] : x, p.sigmoid);
+        if (in)
+          least = fminf(least, x - off);
+        else
+          next = fmaxf(next, x + off);
       }
     }
     return in;
@@ -226,6 +234,7 @@ __device__ __forceinline__ Groups keep_groups(const RouteArgs &p, char *room, in
       g.kept |= in ? 1u << j : 0u;
     }
   }
+  if constexpr (std::is_same<F, float>::value) g.close = -over_lanes<LPT>(-least, Max()) <= over_lanes<LPT>(next, Max());
   wave_sync();
   return g;
 }
