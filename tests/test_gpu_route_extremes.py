@@ -54,3 +54,18 @@ def test_groups_whose_sums_leave_fp32(ctx):
         want, _ = Q.route(x.astype(np.float64), "sigmoid", topk, b.astype(np.float64), groups, top_groups, 2)
         # values of 3e38 that differ by a score are one value in float64: the lowest goes first
         assert np.array_equal(ids, want), top_groups
+
+
+@pytest.mark.parametrize("experts", [8, 12])
+def test_groups_with_nan_come_after_numbers(ctx, experts):
+    """Also after numbers far below zero, and the lowest group of those with a NaN first."""
+    groups, per = 4, experts // 4
+    b = np.full(experts, -1.0e35, np.float32)
+    b[per:2 * per] = [0.0] + [np.nan] * (per - 1)  # its second best is NaN
+    b[2 * per:3 * per] = [1.0] + [np.nan] * (per - 1)
+    b[3 * per:] = -2.0e35
+    x = np.random.default_rng(0).standard_normal((5, experts)).astype(np.float32)
+    for top_groups in (1, 2, 3):
+        ids, _ = run_route(ctx, x, "f32", experts, "sigmoid", per, b, groups, top_groups, 2)
+        want, _ = Q.route(x.astype(np.float64), "sigmoid", per, b.astype(np.float64), groups, top_groups, 2)
+        assert np.array_equal(ids, want), top_groups

@@ -102,6 +102,7 @@ struct Keys<float> {
   typedef int key;
   static constexpr int kNone = (int)0x80000000;  // not there
   static constexpr int kNan = kNone + 1;
+  static constexpr int kPart = kNone + 2;  // of a group: a number and a NaN
   static __device__ __forceinline__ int of(float x) {
     const int b = __float_as_int(x + 0.0f);
     return x != x ? kNan : x == -__builtin_inff() ? kNone : b ^ ((b >> 31) & 0x7fffffff);
@@ -110,18 +111,18 @@ struct Keys<float> {
   // of a group: half the sum of its two best (the sum may be past fp32); scores that are NaN come after all numbers there, too
   static __device__ __forceinline__ int sum(int a, int b) {
     if (a == kNone || b == kNone) return kNone;
-    if (b == kNan) return a == kNan ? kNan : of(value(a) - 1e30f);
+    if (b == kNan) return a == kNan ? kNan : kPart;
     return of(0.5f * value(a) + 0.5f * value(b));
   }
 };
 template <>
 struct Keys<double> {
   typedef double key;
-  static constexpr double kNone = -__builtin_inf(), kNan = -1e300;
+  static constexpr double kNone = -__builtin_inf(), kNan = -1e300, kPart = -1e299;
   static __device__ __forceinline__ double of(double x) { return x != x ? kNan : x; }
   static __device__ __forceinline__ double sum(double a, double b) {
     if (a == kNone || b == kNone) return kNone;
-    if (b == kNan) return a == kNan ? kNan : a - 1e30;
+    if (b == kNan) return a == kNan ? kNan : kPart;
     return a + b;
   }
 };
@@ -212,7 +213,7 @@ __device__ __forceinline__ Groups keep_groups(const RouteArgs &p, char *room, in
     for (int o = 0; o < p.groups; ++o) before += score[o] > mine || (score[o] == mine && o < i);
     const bool in = before < p.top_groups;
     if constexpr (std::is_same<F, float>::value) {
-      if (mine > Keys<F>::kNan) {
+      if (mine > Keys<F>::kPart) {
         const float x = Keys<F>::value(mine), off = unsure(two ? size[i] : x, p.sigmoid);
         if (in)
           least = fminf(least, x - off);
