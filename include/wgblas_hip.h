@@ -468,10 +468,14 @@ int wgb_fp8_gemm_grouped(wgb_ctx *ctx, int transA, int64_t groups, int64_t m,
  * top_groups groups stay whose best choice value (best 1), or the sum of whose
  * two best (best 2), is largest. ids gets the topk experts of the largest
  * choice values, in their order (as 64-bit scores have it; weights are fp32
- * ones); among equal ones the lowest expert (or group) goes first. weights gets the chosen scores, divided by their sum if renorm
- * is not 0, times scale. An expert whose logit or choice value is -Inf is
- * never chosen (a mask): slots that no expert is left for get id -1 and weight
- * 0. A NaN choice value comes after all numbers; NaN scores give NaN weights. */
+ * ones); among equal ones the lowest expert (or group) goes first. weights gets
+ * the chosen scores, divided by their sum if renorm is not 0, times scale; that
+ * sum and what is divided may be far below fp32's range (scores that 64 bits
+ * hold as 0, of logits below -745 or as far below the softmax's largest, are 0:
+ * a mask of the type's lowest value has no weight). An expert whose logit or
+ * choice value is -Inf is never chosen (a mask): slots that no expert is left
+ * for get id -1 and weight 0. A NaN choice value comes after all numbers; NaN
+ * scores give NaN weights. */
 int wgb_route(wgb_ctx *ctx, int type, int scoring, int64_t experts, int64_t n,
               int64_t topk, const void *logits, int64_t ldl, const float *bias,
               int64_t groups, int64_t top_groups, int best, int renorm,

@@ -1,12 +1,16 @@
-"""Routing where fp32 numbers lose what the definition needs: groups whose two best values nearly cancel. Against float64 by
-the definition (tests/routing.py)."""
+"""Routing where fp32 numbers lose what the definition needs: groups whose two best values nearly cancel, scores far below
+fp32's range that are divided by their sum. Against float64 by the definition (tests/routing.py). A weight is off by a
+relative 2 weight_bound (tests/test_gpu_route.py)."""
 import numpy as np
 import pytest
 
+from tests import ragged as R
 from tests import routing as Q
-from tests.test_gpu_route import run_route
+from tests.test_gpu_route import run_route, weight_bound
 
 pytestmark = pytest.mark.gpu
+
+LEAST = 2.0 ** -149  # a step of fp32's subnormals
 
 
 # ---- the choice ----------------------------------------------------------------------
@@ -69,3 +73,61 @@ def test_groups_with_nan_come_after_numbers(ctx, experts):
         ids, _ = run_route(ctx, x, "f32", experts, "sigmoid", per, b, groups, top_groups, 2)
         want, _ = Q.route(x.astype(np.float64), "sigmoid", per, b.astype(np.float64), groups, top_groups, 2)
         assert np.array_equal(ids, want), top_groups
+
+
+# ---- weights and their gradients -------------------------------------------------------
+
+LEVELS = [-60.0, -80.0, -86.5, -88.5, -95.0, -104.0, -120.0, -300.0, -700.0]
+
+
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("experts,topk", [(8, 2), (60, 6), (384, 8), (64, 64)])
+def test_weights_of_small_sigmoids(ctx, level, experts, topk):
+    rng = np.random.default_rng(experts)
+    x = (level + rng.standard_normal((30, experts))).astype(np.float32)
+    x[:4, ::2] = -np.inf
+    for renorm, scale in ((1, 2.5), (0, 1.0)):
+        ids, w = run_route(ctx, x, "f32", experts, "sigmoid", topk, renorm=renorm, scale=scale)
+        want, weights = Q.route(x.astype(np.float64), "sigmoid", topk, renorm=renorm, scale=scale)
+        assert np.array_equal(ids, want)
+        # without the sum's division the scores themselves may be subnormal: an exponential and a quotient of that size
+        assert (np.abs(w - weights) <= weight_bound(x, experts) * 2 * np.abs(weights) + (0.0 if renorm else 4 * LEAST)).all()
+
+
+@pytest.mark.parametrize("ahead", [20.0, 80.0, 87.5, 95.0, 104.0, 150.0, 700.0])
+@pytest.mark.parametrize("experts,topk,groups", [(16, 4, 1), (64, 6, 8), (600, 5, 1)])
+def test_weights_of_experts_far_below_the_largest(ctx, ahead, experts, topk, groups):
+    """A bias keeps the largest logits from being chosen: the others' softmax scores are divided by their own sum."""
+    rng = np.random.default_rng(experts)
+    x = rng.standard_normal((30, experts)).astype(np.float32)
+    b = np.zeros(experts, np.float32)
+    x[:, 1] += ahead
+    b[1] = -100.0
+    b[3:] = rng.permutation(experts - 3) / np.float32(experts)  # so far apart that the small scores do not decide
+    if groups > 1:
+        b[:experts // groups] = -100.0
+    ids, w = run_route(ctx, x, "f32", experts, "softmax", topk, b, groups, max(1, groups // 2), 1, renorm=1)
+    want, weights = Q.route(x.astype(np.float64), "softmax", topk, b.astype(np.float64), groups, max(1, groups // 2), 1, renorm=1)
+    assert np.array_equal(ids, want) and (ids != 1).all()
+    # only differences of the logits and of the largest chosen one enter; the bound counts those from the largest of all
+    assert (np.abs(w - weights) <= weight_bound(x, experts) * 2 * np.abs(weights)).all()
+
+
+def test_scores_that_64_bits_hold_as_zero(ctx):
+    """Masks of the type's lowest value: no weight, as -Inf, where others are left and where none is."""
+    low = np.finfo(np.float32).min
+    x = np.full((3, 8), low, np.float32)
+    x[1, 2], x[2, [0, 5]] = -90.0, [-1.0, -700.0]
+    for t in ("f32", "bf16"):
+        stored = R.encode(np.maximum(x, -3.38e38), t)
+        for renorm in (0, 1):
+            ids, w = run_route(ctx, stored, t, 8, "sigmoid", 3, renorm=renorm)
+            want, weights = Q.route(R.decode(stored, t), "sigmoid", 3, renorm=renorm)
+            assert np.array_equal(ids, want)
+            assert (np.abs(w - weights) <= 2.0 ** -17 * np.abs(weights) + 4 * LEAST).all()
+    b = np.zeros(8, np.float32)
+    b[2] = -5.0
+    x[1, 2] = 1.0
+    ids, w = run_route(ctx, x, "f32", 8, "softmax", 3, b, renorm=1)
+    assert np.array_equal(ids[1], [0, 1, 3]) and (w[1] == 0.0).all()  # expert 2 has all of the softmax
+    assert (np.abs(w[0] - 1 / 3) <= 2.0 ** -22).all()  # all alike

@@ -301,6 +301,35 @@ __device__ __forceinline__ void load_row(const T *x, int e0, int experts, float 
   }
 }
 
+// The chosen experts' scores, a lane a slot: l[r] the logit of slot lane + r LPT
+// or -Inf, `top` and `total` the row's of the softmax (total 1 for sigmoids).
+// `relative`: to the largest of them, for weights that are divided by their sum:
+// the scores themselves may all be below fp32's least number (sigmoids from -104
+// down; softmax where a bias or the groups keep the largest logits out). As 64
+// bits have it, what is below their least number is 0: a logit of the type's
+// lowest value is a mask. A softmax with a NaN or an Inf has no scores.
+constexpr float kLeastLogit = -745.0f;
+template <int LPT, int SLOTS>
+__device__ __forceinline__ void slot_scores(const float (&l)[SLOTS], bool sigmoid, bool relative, float top, float total,
+                                            float (&w)[SLOTS]) {
+  const float zero = sigmoid ? 0.0f : top;
+  float shift = zero;
+  if (relative) {
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int r = 0; r < SLOTS; ++r)
+      if (!(l[r] - zero < kLeastLogit)) most = fmaxf(most, l[r]);
+    most = over_lanes<LPT>(most, Max());
+    shift = sigmoid ? fminf(most, 0.0f) : most;
+  }
+#pragma unroll
+  for (int r = 0; r < SLOTS; ++r) {
+    const float r1 = 1.0f / (1.0f + expf(-fabsf(l[r]))), e = expf(l[r] - shift);
+    w[r] = l[r] - zero < kLeastLogit ? 0.0f : sigmoid ? (l[r] < 0.0f ? e * r1 : r1) : relative ? e : e / total;
+    if (l[r] != -__builtin_inff()) w[r] += total - total;
+  }
+}
+
 // LPT lanes a token, PER consecutive experts a lane. A token's choice values
 // stay in its lanes' registers; each round takes the largest.
 //
@@ -416,17 +445,15 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
   wave_sync();
 
   // the weights, a lane a choice
-  float w[kMaxTopk / LPT], sum = 0.0f;
+  float c[kMaxTopk / LPT], w[kMaxTopk / LPT], sum = 0.0f;
 #pragma unroll
   for (int r = 0; r < kMaxTopk / LPT; ++r) {
     const int s = lane + r * LPT;
-    w[r] = 0.0f;
-    if (s < p.topk && chosen[slot][s] >= 0) {
-      const float c = (float)x[chosen[slot][s]];
-      w[r] = p.sigmoid ? 1.0f / (1.0f + expf(-c)) : expf(c - top) / total;
-    }
-    sum += w[r];
+    c[r] = s < p.topk && chosen[slot][s] >= 0 ? (float)x[chosen[slot][s]] : -__builtin_inff();
   }
+  slot_scores<LPT>(c, p.sigmoid, p.renorm, top, total, w);
+#pragma unroll
+  for (int r = 0; r < kMaxTopk / LPT; ++r) sum += w[r];
   if (p.renorm) {
     sum = over_lanes<LPT>(sum, Sum());
     if (sum == 0.0f) sum = 1.0f;
