@@ -1,16 +1,22 @@
 """Routing where fp32 numbers lose what the definition needs: groups whose two best values nearly cancel, scores far below
-fp32's range that are divided by their sum. Against float64 by the definition (tests/routing.py). A weight is off by a
-relative 2 weight_bound (tests/test_gpu_route.py)."""
+fp32's range that are divided by their sum, one expert that has nearly all of the softmax, ids that a bias chose. Against
+float64 by the definition (tests/routing.py) and by sums that do not cancel (tests/routing_gradient.py).
+
+Bounds. A weight is off by a relative W = 2 weight_bound (tests/test_gpu_route.py). A logit's gradient is a sum of products
+of two scores or weights, the complement of one, and a difference of two of what came back: it is within (3 W + (slots + 8)
+2^-24) of the sum of the terms' magnitudes (each term's difference, products and place in the sum round once)."""
 import numpy as np
 import pytest
 
 from tests import ragged as R
 from tests import routing as Q
-from tests.test_gpu_route import run_route, weight_bound
+from tests import routing_gradient as G
+from tests.test_gpu_route import SCORING, STEP, run_route, weight_bound
 
 pytestmark = pytest.mark.gpu
 
 LEAST = 2.0 ** -149  # a step of fp32's subnormals
+SMALLEST = {"f32": 0.0, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}  # half a step of the type's
 
 
 # ---- the choice ----------------------------------------------------------------------
@@ -77,6 +83,29 @@ def test_groups_with_nan_come_after_numbers(ctx, experts):
 
 # ---- weights and their gradients -------------------------------------------------------
 
+
+def run_grad(ctx, x, t, scoring, ids, dw, renorm, scale=1.0):
+    n, experts = x.shape
+    dL, dI, dW = ctx.upload(R.encode(x, t)), ctx.upload(ids), ctx.upload(dw)
+    out = ctx.empty((n, experts), R.STORE[t])
+    ctx.route_grad(R.TYPES[t], SCORING[scoring], experts, n, ids.shape[1], dL, experts, dI, renorm, scale, dW, out, experts)
+    got = R.decode(out.to_host(), t)
+    for d in (dL, dI, dW, out):
+        d.free()
+    return got
+
+
+def check_grad(ctx, x, t, scoring, ids, dw, renorm, scale=1.0):
+    x = R.decode(R.encode(x, t), t)
+    got = run_grad(ctx, x, t, scoring, ids, dw, renorm, scale)
+    want, size = G.grad(x, scoring, ids, dw.astype(np.float64), renorm, scale)
+    bound = (3 * 2 * weight_bound(x, x.shape[1]) + (ids.shape[1] + 8) * STEP) * size
+    # the result's own rounding, and some of fp32's steps where it or a score is subnormal
+    bound += np.abs(want) * R.HALF_UNIT[t] + SMALLEST[t] + 8 * LEAST * max(np.abs(dw).max(), 1.0) * max(scale, 1.0)
+    off = np.abs(got - want)
+    assert np.isfinite(got).all() and (off <= bound).all(), (np.argwhere(~(off <= bound))[0], np.nanmax(off / bound))
+
+
 LEVELS = [-60.0, -80.0, -86.5, -88.5, -95.0, -104.0, -120.0, -300.0, -700.0]
 
 
@@ -111,6 +140,8 @@ def test_weights_of_experts_far_below_the_largest(ctx, ahead, experts, topk, gro
     assert np.array_equal(ids, want) and (ids != 1).all()
     # only differences of the logits and of the largest chosen one enter; the bound counts those from the largest of all
     assert (np.abs(w - weights) <= weight_bound(x, experts) * 2 * np.abs(weights)).all()
+    dw = rng.standard_normal((30, topk)).astype(np.float32)
+    check_grad(ctx, x, "f32", "softmax", ids, dw, 1, 2.5)
 
 
 def test_scores_that_64_bits_hold_as_zero(ctx):
@@ -125,9 +156,41 @@ def test_scores_that_64_bits_hold_as_zero(ctx):
             want, weights = Q.route(R.decode(stored, t), "sigmoid", 3, renorm=renorm)
             assert np.array_equal(ids, want)
             assert (np.abs(w - weights) <= 2.0 ** -17 * np.abs(weights) + 4 * LEAST).all()
+            check_grad(ctx, R.decode(stored, t), t, "sigmoid", want, np.full((3, 3), 1.5, np.float32), renorm)
     b = np.zeros(8, np.float32)
     b[2] = -5.0
     x[1, 2] = 1.0
     ids, w = run_route(ctx, x, "f32", 8, "softmax", 3, b, renorm=1)
     assert np.array_equal(ids[1], [0, 1, 3]) and (w[1] == 0.0).all()  # expert 2 has all of the softmax
     assert (np.abs(w[0] - 1 / 3) <= 2.0 ** -22).all()  # all alike
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("experts,topk", [(8, 2), (60, 6), (300, 64)])
+def test_gradient_of_small_sigmoids(ctx, t, level, experts, topk):
+    rng = np.random.default_rng(experts)
+    x = R.decode(R.encode(level + rng.standard_normal((30, experts)), t), t)
+    x[:4, ::2] = -np.inf
+    dw = (3.0 * rng.standard_normal((30, topk))).astype(np.float32)
+    for renorm, scale in ((1, 1.0), (1, 2.5), (0, 1.0)):
+        ids, _ = Q.route(x, "sigmoid", topk, renorm=renorm)
+        check_grad(ctx, x, t, "sigmoid", ids, dw, renorm, scale)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [0, 1])
+def test_nan_gradients_stay_in_their_row(ctx, scoring, renorm):
+    """A softmax with a NaN or an Inf has no scores, its row's gradients are NaN; a NaN sigmoid that is not chosen changes
+    no other's."""
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((4, 8)).astype(np.float32)
+    x[1, 5], x[2, 0] = np.nan, np.inf
+    ids = np.array([[0, 1], [0, 1], [2, 1], [3, 4]], np.int32)
+    dw = rng.standard_normal((4, 2)).astype(np.float32)
+    got = run_grad(ctx, x, "f32", scoring, ids, dw, renorm)
+    if scoring == "softmax":
+        assert np.array_equal(np.isnan(got), np.isin(np.arange(4), [1, 2])[:, None].repeat(8, 1))
+    else:
+        got[1, 5] = 0.0  # of the NaN itself: 0 times its slope
+        assert not np.isnan(got).any()

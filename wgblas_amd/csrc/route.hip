@@ -509,11 +509,13 @@ struct GradArgs {
   float scale;
 };
 
-// With p the scores, S the sum of the chosen ones and d_s what came back for
-// weight s (times scale): the chosen scores' gradients are q_s = d_s, or with
-// renormalised weights (d_s - sum_r d_r p_r / S) / S. Sigmoid: the chosen
-// logits get q p (1 - p), the others 0; softmax: every logit p (q - sum_r q_r
-// p_r). An expert that is there twice gets the sum, in the slots' order.
+// With p the scores and d_s what came back for weight s (times scale): a chosen
+// score's gradient is d_s; sigmoid: the chosen logits get d p (1 - p), the others
+// 0; softmax: every logit p (d - sum_r d_r p_r). With renormalised weights w = p /
+// S the sum of d_r w_r is taken from d_s, and p / S is w again: the chosen logits
+// get w_s (d_s - sum_r d_r w_r), times 1 - p of the sigmoid, the others nothing,
+// and neither S nor the scores need be in fp32's range. An expert that is there
+// twice gets the sum, in the slots' order.
 // A row is read and written once, in registers (16384 rows of 128 fp32 logits:
 // 6.9 us, 2.6 TB/s; as short as it is, half of that is the launch and the first
 // loads' way).
@@ -530,25 +532,14 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
   const T *x = (const T *)p.logits + row * p.ldl;
   const int e0 = lane * PER;
   float l[PER];
-  if (e0 + PER <= p.experts) {
-    struct __attribute__((packed, aligned(sizeof(T)))) V {
-      T v[PER];
-    };
-    const V v = *reinterpret_cast<const V *>(x + e0);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) l[j] = (float)v.v[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) l[j] = e0 + j < p.experts ? (float)x[e0 + j] : -__builtin_inff();
-  }
-  // scores, and for sigmoid p (1 - p)
+  load_row<T, PER>(x, e0, p.experts, -__builtin_inff(), l);
+  // softmax: scores; sigmoid: what an expert's slots are multiplied by
   float s[PER], slope[PER], top = 0.0f, total = 1.0f;
   if (p.sigmoid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const float t = expf(-fabsf(l[j])), r = 1.0f / (1.0f + t);
-      s[j] = l[j] < 0.0f ? t * r : r;
-      slope[j] = t * r * r;
+      slope[j] = p.renorm ? (l[j] < 0.0f ? r : t * r) : t * r * r;
     }
   } else {
     top = l[0];
@@ -565,39 +556,38 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
     for (int j = 0; j < PER; ++j) s[j] /= total;
   }
   // the chosen scores: a lane a slot
-  float w[SLOTS], d[SLOTS], sum = 0.0f, dot = 0.0f;
+  float c[SLOTS], w[SLOTS], d[SLOTS], sum = 0.0f, dot = 0.0f;
 #pragma unroll
   for (int r = 0; r < SLOTS; ++r) {
     const int i = lane + r * LPT;
-    w[r] = d[r] = 0.0f;
-    int id = -1;
+    c[r] = -__builtin_inff();
+    d[r] = 0.0f;
     if (i < p.topk) {
-      id = p.ids[row * p.topk + i];
+      int id = p.ids[row * p.topk + i];
       if (id >= p.experts) id = -1;
       if (id >= 0) {
-        const float c = (float)x[id];
-        w[r] = p.sigmoid ? 1.0f / (1.0f + expf(-c)) : expf(c - top) / total;
+        c[r] = (float)x[id];
         d[r] = p.dweights[row * p.topk + i] * p.scale;
       }
       at[slot][i] = id;
     }
-    sum += w[r];
-    dot += d[r] * w[r];
   }
-  sum = over_lanes<LPT>(sum, Sum());
+  slot_scores<LPT>(c, p.sigmoid, p.renorm, top, total, w);
+  if (p.renorm) {
+#pragma unroll
+    for (int r = 0; r < SLOTS; ++r) sum += w[r];
+    sum = over_lanes<LPT>(sum, Sum());
+#pragma unroll
+    for (int r = 0; r < SLOTS; ++r) w[r] /= sum == 0.0f ? 1.0f : sum;
+  }
+#pragma unroll
+  for (int r = 0; r < SLOTS; ++r) dot += d[r] * w[r];
   dot = over_lanes<LPT>(dot, Sum());
-  if (sum == 0.0f) sum = 1.0f;
-  float inner = 0.0f;  // sum of q p, of the softmax
 #pragma unroll
   for (int r = 0; r < SLOTS; ++r) {
     const int i = lane + r * LPT;
-    if (i < p.topk) {
-      const float g = p.renorm ? (d[r] - dot / sum) / sum : d[r];
-      q[slot][i] = g;
-      if (at[slot][i] >= 0) inner += g * w[r];
-    }
+    if (i < p.topk) q[slot][i] = p.renorm ? w[r] * (d[r] - dot) : d[r];
   }
-  inner = over_lanes<LPT>(inner, Sum());
 #pragma unroll
   for (int j = 0; j < PER; ++j) back[slot][e0 + j] = 0.0f;
   __syncthreads();
@@ -610,7 +600,8 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const float g = back[slot][e0 + j];
-    out[j] = (T)wgb::in_fp32(p.sigmoid ? g * slope[j] : s[j] * (g - inner));
+    // (total - total: 0, or NaN where the softmax has no scores)
+    out[j] = (T)wgb::in_fp32(p.sigmoid ? g * slope[j] : p.renorm ? g + (total - total) : s[j] * (g - dot));
   }
   T *y = (T *)p.dlogits + token * p.ldd;
   if (e0 + PER <= p.experts) {
