@@ -178,6 +178,54 @@ def test_gradient_of_small_sigmoids(ctx, t, level, experts, topk):
         check_grad(ctx, x, t, "sigmoid", ids, dw, renorm, scale)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm,scale", [(0, 1.0), (0, 2.5), (1, 2.5)])
+@pytest.mark.parametrize("ahead", [0.0, 6.0, 12.0, 16.0, 20.0, 40.0, 100.0])
+@pytest.mark.parametrize("experts,topk", [(8, 1), (8, 8), (60, 6), (128, 8), (600, 33)])
+def test_gradient_of_a_dominating_expert(ctx, t, scoring, renorm, scale, ahead, experts, topk):
+    """One logit far ahead: its score is nearly 1, its gradient what the others leave."""
+    rng = np.random.default_rng(experts + topk)
+    x = rng.standard_normal((20, experts))
+    x[np.arange(20), rng.integers(0, experts, 20)] += ahead
+    x = R.decode(R.encode(x, t), t)
+    dw = rng.standard_normal((20, topk)).astype(np.float32)
+    dw[5:10] = dw[5:10, :1] * (1 + 2.0 ** -12 * rng.standard_normal((5, topk)))  # nearly the same for all slots
+    ids, _ = Q.route(x, scoring, topk)
+    check_grad(ctx, x, t, scoring, ids, dw, renorm, scale)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("experts,topk,groups,top_groups", [(16, 4, 1, 1), (64, 6, 8, 2), (600, 5, 4, 1)])
+@pytest.mark.parametrize("ahead", [0.0, 14.0, 60.0])
+def test_gradient_of_what_a_bias_chose(ctx, scoring, renorm, experts, topk, groups, top_groups, ahead):
+    """ids of the forward call with a bias and groups, of which the largest logit may not be one."""
+    rng = np.random.default_rng(experts)
+    x = rng.standard_normal((40, experts)).astype(np.float32)
+    x[:, 3] += ahead
+    b = rng.standard_normal(experts).astype(np.float32)
+    b[3] = -3.0
+    ids, _ = run_route(ctx, x, "f32", experts, scoring, topk, b, groups, top_groups, 2, renorm)
+    want, _ = Q.route(x.astype(np.float64), scoring, topk, b.astype(np.float64), groups, top_groups, 2, renorm)
+    assert np.array_equal(ids, want)
+    dw = rng.standard_normal((40, topk)).astype(np.float32)
+    check_grad(ctx, x, "f32", scoring, ids, dw, renorm, 2.5)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [0, 1])
+def test_gradient_of_an_expert_that_is_there_twice(ctx, scoring, renorm):
+    """ids that a caller made, some of no expert: the slots' gradients add up, also where one expert has nearly all."""
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((50, 20)).astype(np.float32)
+    x[::2, 4] += 15.0
+    ids = rng.integers(-1, 6, (50, 7)).astype(np.int32)
+    ids[7, 2], ids[8, 0], ids[9] = 20, 2 ** 31 - 1, -5
+    dw = rng.standard_normal((50, 7)).astype(np.float32)
+    check_grad(ctx, x, "f32", scoring, ids, dw, renorm, 1.5)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [0, 1])
 def test_nan_gradients_stay_in_their_row(ctx, scoring, renorm):

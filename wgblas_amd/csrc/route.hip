@@ -514,15 +514,19 @@ struct GradArgs {
 // 0; softmax: every logit p (d - sum_r d_r p_r). With renormalised weights w = p /
 // S the sum of d_r w_r is taken from d_s, and p / S is w again: the chosen logits
 // get w_s (d_s - sum_r d_r w_r), times 1 - p of the sigmoid, the others nothing,
-// and neither S nor the scores need be in fp32's range. An expert that is there
-// twice gets the sum, in the slots' order.
+// and neither S nor the scores need be in fp32's range.
+// Where one expert has nearly all of the softmax or of S, that difference is of
+// nearly equal numbers. The weights add up to 1, the chosen scores to 1 less the
+// others' (R), so it is written as a sum that does not cancel: sum_r w_r (d_s -
+// d_r), and sum_r p_r (d_s - d_r) + d_s R. An expert that is there twice has the
+// sum of its slots, in their order.
 // A row is read and written once, in registers (16384 rows of 128 fp32 logits:
-// 6.9 us, 2.6 TB/s; as short as it is, half of that is the launch and the first
-// loads' way).
+// 7.9 us from call to call, 2.3 TB/s, and 7.1 with differences of sums; as short
+// as it is, nearly half of that is the launch and the first loads' way).
 template <class T, int LPT, int PER>
 __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
   constexpr int TOKENS = 256 / LPT, SLOTS = kMaxTopk / LPT;
-  __shared__ float q[TOKENS][kMaxTopk];
+  __shared__ float q[TOKENS][kMaxTopk], share[TOKENS][kMaxTopk];
   __shared__ int at[TOKENS][kMaxTopk];
   __shared__ float back[TOKENS][LPT * PER];
   const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT;
@@ -556,20 +560,18 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
     for (int j = 0; j < PER; ++j) s[j] /= total;
   }
   // the chosen scores: a lane a slot
-  float c[SLOTS], w[SLOTS], d[SLOTS], sum = 0.0f, dot = 0.0f;
+  float c[SLOTS], w[SLOTS], d[SLOTS], sum = 0.0f;
+  int id[SLOTS];
 #pragma unroll
   for (int r = 0; r < SLOTS; ++r) {
     const int i = lane + r * LPT;
     c[r] = -__builtin_inff();
     d[r] = 0.0f;
-    if (i < p.topk) {
-      int id = p.ids[row * p.topk + i];
-      if (id >= p.experts) id = -1;
-      if (id >= 0) {
-        c[r] = (float)x[id];
-        d[r] = p.dweights[row * p.topk + i] * p.scale;
-      }
-      at[slot][i] = id;
+    id[r] = i < p.topk ? p.ids[row * p.topk + i] : -1;
+    if (id[r] >= p.experts) id[r] = -1;
+    if (id[r] >= 0) {
+      c[r] = (float)x[id[r]];
+      d[r] = p.dweights[row * p.topk + i];
     }
   }
   slot_scores<LPT>(c, p.sigmoid, p.renorm, top, total, w);
@@ -580,20 +582,56 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
 #pragma unroll
     for (int r = 0; r < SLOTS; ++r) w[r] /= sum == 0.0f ? 1.0f : sum;
   }
+  auto each_slot = [&](auto f) {
 #pragma unroll
-  for (int r = 0; r < SLOTS; ++r) dot += d[r] * w[r];
-  dot = over_lanes<LPT>(dot, Sum());
-#pragma unroll
-  for (int r = 0; r < SLOTS; ++r) {
-    const int i = lane + r * LPT;
-    if (i < p.topk) q[slot][i] = p.renorm ? w[r] * (d[r] - dot) : d[r];
-  }
+    for (int r = 0; r < SLOTS; ++r)
+      if (lane + r * LPT < p.topk) f(r, lane + r * LPT);
+  };
+  // sum over the slots of share (x - q)
+  auto differences = [&](float x) {
+    float all = 0.0f;
+    for (int i = 0; i < p.topk; ++i) all = fmaf(share[slot][i], x - q[slot][i], all);
+    return all;
+  };
+  each_slot([&](int r, int i) {
+    at[slot][i] = id[r];
+    q[slot][i] = d[r];
+    share[slot][i] = w[r];
+  });
 #pragma unroll
   for (int j = 0; j < PER; ++j) back[slot][e0 + j] = 0.0f;
-  __syncthreads();
+  wave_sync();
+  if (p.renorm) {
+    each_slot([&](int r, int) { d[r] = w[r] * differences(d[r]); });
+    wave_sync();
+    each_slot([&](int r, int i) { q[slot][i] = d[r]; });
+    wave_sync();
+  }
+  uint32_t mine = 0;
   for (int i = 0; i < p.topk; ++i) {  // each expert's lane adds its own
-    const int id = at[slot][i];
-    if (id >= e0 && id < e0 + PER) back[slot][id] += q[slot][i];
+    const int e = at[slot][i];
+    if (e < e0 || e >= e0 + PER) continue;
+    back[slot][e] += q[slot][i];
+    if (mine >> (e - e0) & 1) share[slot][i] = 0.0f;  // its score counts once
+    mine |= 1u << (e - e0);
+  }
+  float inner = 0.0f, rest = 0.0f;
+  if (!p.sigmoid && !p.renorm) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) rest += mine >> j & 1 ? 0.0f : s[j];
+    rest = over_lanes<LPT>(rest, Sum());
+    wave_sync();
+    each_slot([&](int r, int i) {
+      d[r] = id[r] >= 0 ? back[slot][id[r]] : 0.0f;
+      q[slot][i] = d[r];
+      inner += share[slot][i] * d[r];
+    });
+    inner = over_lanes<LPT>(inner, Sum());
+    wave_sync();
+    each_slot([&](int r, int) {
+      if (id[r] >= 0) back[slot][id[r]] = differences(d[r]) + d[r] * rest;
+    });
+    wave_sync();
   }
   if (!here) return;
   T out[PER];
@@ -601,7 +639,8 @@ __global__ __launch_bounds__(256) void route_grad_kernel(GradArgs p) {
   for (int j = 0; j < PER; ++j) {
     const float g = back[slot][e0 + j];
     // (total - total: 0, or NaN where the softmax has no scores)
-    out[j] = (T)wgb::in_fp32(p.sigmoid ? g * slope[j] : p.renorm ? g + (total - total) : s[j] * (g - dot));
+    const float y = p.sigmoid ? g * slope[j] : p.renorm ? g + (total - total) : s[j] * (mine >> j & 1 ? g : -inner);
+    out[j] = (T)wgb::in_fp32(y * p.scale);
   }
   T *y = (T *)p.dlogits + token * p.ldd;
   if (e0 + PER <= p.experts) {
