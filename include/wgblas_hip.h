@@ -401,7 +401,8 @@ int wgb_mxfp4_gemm_grouped(wgb_ctx *ctx, int64_t groups, int64_t m, int64_t n,
  * least power of two that brings its largest magnitude to 448 or less, at
  * least 2^-126; x/scale goes to the nearest code, ties to the even code. A
  * block with an Inf or a NaN becomes NaN as a whole (scale NaN, codes 0).
- * Quantising and back take fewer than 2^26 columns. */
+ * Quantising and back take at most 2^26 - 4 columns, quantising with WGB_TRANS
+ * or in square blocks fewer than 2^23 tiles of 128 x 128 values. */
 int wgb_fp8_quantize(wgb_ctx *ctx, int type, int trans, int block, int64_t k,
                      int64_t n, const void *X, int64_t ldx, uint8_t *codes,
                      int64_t ld, float *scales, int64_t lds);

@@ -288,7 +288,8 @@ int quantize(wgb_ctx *ctx, int trans, int block, int64_t k, int64_t n, const voi
              int64_t ld, float *scales, int64_t lds) {
   const int blocks_k = (int)blocks128(k);
   const int64_t tiles = blocks_k * blocks128(n);
-  if ((trans == WGB_TRANS || block == 128) && tiles > INT32_MAX)
+  // as few threads as check_convert allows, 512 of a tile
+  if ((trans == WGB_TRANS || block == 128) && tiles >= (int64_t)1 << 23)
     return fail(WGB_ERR_INVALID_VALUE, "wgb_fp8_quantize: too many blocks");
   const T *x = (const T *)X;
   if (trans == WGB_TRANS) {
@@ -348,8 +349,8 @@ int check_convert(int type, int block, int64_t k, int64_t n) {
     return fail(WGB_ERR_INVALID_VALUE, "type must be WGB_F32, WGB_F16 or WGB_BF16");
   if (block != 1 && block != 128) return fail(WGB_ERR_INVALID_VALUE, "block must be 1 or 128");
   if (k < 0 || n < 0) return fail(WGB_ERR_INVALID_VALUE, "k and n must be non-negative");
-  // a launch has fewer than 2^32 threads, of which a column has 64
-  if (n >= (int64_t)1 << 26) return fail(WGB_ERR_INVALID_VALUE, "n must be below 2^26");
+  // a launch has fewer than 2^32 threads along an axis, of which a column has 64, in blocks of four columns
+  if (n > ((int64_t)1 << 26) - 4) return fail(WGB_ERR_INVALID_VALUE, "n must be at most 2^26 - 4");
   return WGB_OK;
 }
 
