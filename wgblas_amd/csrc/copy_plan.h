@@ -91,7 +91,9 @@ struct CopyPlan {
   // A last k-tile that K cuts can be copied too, chunks past K reading one
   // that exists: whoever reads the operands then clears what is past K
   // (tail_mask). Not where a cut chunk could reach past the matrix: at its
-  // last row (k-contiguous), or with cut rows (row-contiguous).
+  // last row (k-contiguous), or with cut rows (row-contiguous). Columns of
+  // 8-bit codes are whole runs of 128: no chunk is cut, and what a k-row past K
+  // is multiplied with is zeros; k-contiguous ones have no cut k-tile.
   __host__ __device__ __forceinline__ bool soft_tail() const {
     return BITS == 8 ? MC : MC ? rows_left >= BT : K % EPC == 0 || (rows_left > BT && K >= EPC);
   }

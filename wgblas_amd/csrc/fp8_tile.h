@@ -241,7 +241,7 @@ struct Fp8Kernel {
       sa.origin += first * sa.step();
       sb.origin += first * sb.step();
       ss.init(p, tile.g, m0, tile.lo + n0, cols - n0, first, wave, lane);
-      const int whole = AMC && depth < (int64_t)nt * TB ? nt - 1 : nt;
+      const int whole = sa.soft_tail() && sa.whole_tiles() < nt ? sa.whole_tiles() : nt;
 
       auto copy = [&](int kt) {
         char *st = smem + (kt % S) * STAGE;
@@ -388,7 +388,7 @@ struct Fp8Large {
     }
     // All of A of any k-tile: k-rows past k read the k-tile's first one again, B's codes there are zeros.
     __device__ __forceinline__ void all_a(char *smem, int wave, int kt) const {
-      const bool cut = AMC && kt >= sa.whole_tiles();
+      const bool cut = sa.soft_tail() && kt >= sa.whole_tiles();
 #pragma unroll
       for (int r = 0; r < SA::LOADS; ++r)
         copy_chunks(sa.origin + kt * sa.step(), cut ? sa.tail_voff(r) : sa.voff[r],
@@ -527,7 +527,7 @@ struct Fp8Large {
       });
     };
     auto k_tiles = [&](auto used) {
-      const int whole = AMC ? c.sa.whole_tiles() : depth, steady = (whole < depth ? whole : depth) - 2;
+      const int whole = c.sa.soft_tail() ? c.sa.whole_tiles() : depth, steady = (whole < depth ? whole : depth) - 2;
       int kt = 0;
       for (; kt < steady; ++kt) k_tile(used, std::true_type(), kt);
       for (; kt < depth; ++kt) k_tile(used, std::false_type(), kt);
