@@ -967,12 +967,12 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsArgs p) {
         C v[L::V];
       } out;
 #pragma unroll
-      for (int i = 0; i < L::V; ++i) out.v[i] = (C)sum[i];
+      for (int i = 0; i < L::V; ++i) out.v[i] = (C)wgb::in_fp32(sum[i]);
       *reinterpret_cast<Out *>(c + at) = out;
     } else {
 #pragma unroll
       for (int i = 0; i < L::V; ++i)
-        if (at + i < p.d) c[at + i] = (C)sum[i];
+        if (at + i < p.d) c[at + i] = (C)wgb::in_fp32(sum[i]);
     }
   }
 }
