@@ -137,7 +137,9 @@ __global__ __launch_bounds__(512) void quantize_square_kernel(const T *X, int64_
 // 16 rows: 2.9 TB/s). A lane's codes of a column, RG rows of k, go through LDS
 // (four dwords more after every lane's columns: two lanes in a bank) and out as
 // 128-byte lines. STREAM loads past the caches (bf16 16384 x 4096: 43 us,
-// 4.7 TB/s, and 50 us through them; stores past them too: 45 us).
+// 4.7 TB/s, and 50 us through them; stores past them too: 45 us), at whole dwords
+// only: at halves that is slower (bf16 16384 x 4096 at 4097: 46.8 us, 43.9 through
+// the caches; 4099 x 8191 at 8191: 32.7 and 28.1).
 template <class T, bool SQUARE, bool STREAM>
 __global__ __launch_bounds__(512) void quantize_strided_kernel(const T *X, int64_t ldx, int64_t k, int64_t n,
                                                                uint8_t *codes, int64_t ld, float *scales, int64_t lds,
@@ -310,7 +312,8 @@ int quantize(wgb_ctx *ctx, int trans, int block, int64_t k, int64_t n, const voi
 template <class T>
 int quantize_as(wgb_ctx *ctx, int trans, int block, int64_t k, int64_t n, const void *X, int64_t ldx, uint8_t *codes,
                 int64_t ld, float *scales, int64_t lds) {
-  return (streams<T>(k, n) ? quantize<T, true> : quantize<T, false>)(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds);
+  const bool stream = streams<T>(k, n) && (trans == WGB_NO_TRANS || (((uintptr_t)X | ldx * sizeof(T)) & 3) == 0);
+  return (stream ? quantize<T, true> : quantize<T, false>)(ctx, trans, block, k, n, X, ldx, codes, ld, scales, lds);
 }
 
 template <class T>
