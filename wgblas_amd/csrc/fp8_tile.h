@@ -10,11 +10,16 @@
 // That instruction adds up products in eights (k 8 i .. 8 i + 7 of a lane's
 // bytes), aligned to the largest of the eight: what is below 2^-13 of it is
 // lost (measured: 2^16 + 4 gives 2^16, the sums of eights among each other are
-// fp32's). On normal values that is 1.3e-5 of the result (2-norm), without
-// bias, a hundredth of a bf16 result's own rounding; an fp32 result would show
-// it, so there the codes are widened to bf16, which holds them exactly, and
-// multiplied by v_mfma_f32_16x16x32_bf16, whose sums are fp32's throughout, at
-// half the rate.
+// fp32's), so at most 7 2^-13 of the largest, less than 2^-10 of the eight's
+// magnitudes. Taken for 16-bit results, for twice the rate. On normal values it
+// is 1.3e-5 of the result (2-norm, no bias found), where rounding a bf16 result is
+// 1.7e-3 and an f16 one 2.07e-4 (2.08e-4 with it, 512 x 512 x 2048; about two of
+// a thousand bf16 elements are the neighbouring number). One channel of every eight
+// 1000 times as large: f16 2.27e-4, 2.08e-4 of it its rounding; two of eight whose
+// products cancel: 2.1e-3 of an f16 result and 2.7e-3 of a bf16 one, more than
+// their rounding. An fp32 result would show it everywhere: there the codes are
+// widened to bf16, which holds them exactly, and multiplied by
+// v_mfma_f32_16x16x32_bf16, whose sums are fp32's throughout, at half the rate.
 //
 // Operand layout: lane group g = lane / 16 has the bytes 16 g .. 16 g + 15 and
 // 64 + 16 g .. of its row's k-tile, in A and in B alike (any order of k that
@@ -184,8 +189,8 @@ __device__ __forceinline__ void multiply_codes(const v8i (&a)[COUNT], const type
 
 // One BM x BN tile of C a block, WM x WN waves, S stages of LDS. 128 x 128 with
 // exact sums and rows' own scales is bound by the conversions and v_fma (4096 x
-// 2048 x 16384: 264 us, 1.04 PFLOP/s), 128 x 32 by reading A (49 experts of 4096
-// x 2048 with 96 columns: 78 us, 5.3 TB/s).
+// 2048 x 16384: 259 us, 1.06 PFLOP/s), 128 x 32 by reading A (49 experts of 4096
+// x 2048 with 96 columns: 80 us, 5.1 TB/s).
 template <int BM, int BN, int WM, int WN, bool AMC, bool ROWS, bool EXACT, int S>
 struct Fp8Kernel {
   typedef Fp8 Element;
@@ -344,8 +349,9 @@ struct Fp8Kernel {
 // are issued before a tile is stored, when its operands' registers are free: in
 // the midst of a tile they would have to be spilled, and each return of one
 // waits for all copies and stores under way.
-// 8192 x 4096 x 8192 into bf16: 215 us, 2.56 PFLOP/s, and 226 with A
-// row-contiguous, bound by power; at k = 2048 1.97, for a tile's start and end.
+// 8192 x 4096 x 8192 into bf16: 224 us (2.45 PFLOP/s) and 226 with A
+// row-contiguous, one call at a time; from call to call 255 and 231, bound by
+// power; at k = 2048 2.0 to 2.1 PFLOP/s, for a tile's start and end.
 template <bool AMC, bool ROWS, bool EXACT>
 struct Fp8Large {
   static constexpr int BM = 256, BN = 256, WM = 2, WN = 4;
@@ -592,7 +598,7 @@ struct Fp8Large {
 // load both operands straight into MFMA operand registers, the next k-tile ahead
 // of the present one's MFMAs, and add their sums in LDS in the waves' order. A
 // k-contiguous only. One column, repeated: 8192 x 8192 12.4 us (5.4 TB/s), 4096 x
-// 4096 6.9; 16 columns, 8192 x 4096 8.6.
+// 4096 6.9; 16 columns, 8192 x 4096 9.0.
 template <int R, int CB, bool ROWS, bool EXACT>
 struct Fp8Skinny {
   static constexpr int kBM = 16 * R, kBN = 16 * CB;

@@ -341,8 +341,8 @@ __device__ __forceinline__ void slot_scores(const float (&l)[SLOTS], bool sigmoi
 // values that may be chosen, one at a time: few, and the code short, for it is
 // seldom run and comes from beyond the instruction cache (fp64 values of all 256
 // experts of such tokens alone: 10 us, for 16384 tokens that otherwise take 16).
-// Bound by the rounds' compares: 22.8 us for those tokens with 8 groups and a
-// bias (0.8 TB/s), 3.2 for 16 tokens of 64 experts.
+// Bound by the rounds' compares: 22.7 us for those tokens with 8 groups and a
+// bias (0.8 TB/s), 3.5 for 16 tokens of 64 experts.
 template <class T, bool WIDE, int LPT, int PER>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
   constexpr int TOKENS = 256 / LPT;
@@ -683,7 +683,7 @@ int grad(wgb_ctx *ctx, const GradArgs &p) {
 // their counts go to counts[block][expert] (order_count_kernel), then every
 // block adds up the counts before its own and of all, and places its pairs
 // (order_place_kernel). A single block counts for itself: one launch (2.4 us for
-// 128 pairs; 131072 pairs of 256 experts in 64 blocks: 3.2 + 7.3 us, bound by the
+// 128 pairs; 131072 pairs of 256 experts in 64 blocks: 2.1 + 7.3 us, bound by the
 // ranks within a block).
 __device__ __forceinline__ int expert_of(const int32_t *ids, int64_t p, int64_t end, int experts) {
   const int e = p < end ? ids[p] : -1;
